@@ -44,7 +44,7 @@ typedef enum kb_status {
   KB_ERR_TOO_LARGE = 5       /* problem exceeds a fixed-size internal buffer                 */
 } kb_status;
 
-typedef enum kb_dtype { KB_F32 = 0, KB_F16 = 1, KB_BF16 = 2 } kb_dtype;
+typedef enum kb_dtype { KB_F32 = 0, KB_F16 = 1, KB_BF16 = 2, KB_E4M3 = 3 /* paged caches only */ } kb_dtype;
 
 /* flags for the attention entry points */
 #define KB_FLAG_PRESCALE_QK 1u   /* accepted for signature parity; scaling is always done in fp32 */
@@ -373,6 +373,136 @@ KB_API int kb_out_proj(const kb_out_proj_params* p, void* stream);
  * (the dense schedule is the streaming schedule with a single chunk).
  */
 KB_API int kb_fa_fwd(const kb_sa_fwd_params* p, void* stream);
+
+/*
+ * Answering from a paged key/value cache (no counterpart in the reference, which runs whole sequences; its mask,
+ * src/streaming_attention/kernel.py:1540-1542, is what `context_size` / `back_contexts` mean below).
+ *
+ * The cache is P pages of `page` rows for every key/value head; row r of sequence b lies in page
+ * page_table[b][r / page] at r % page.  lens[b] is the sequence's length (clamped to [0, M * page]).  A table entry outside
+ * [0, P) holds nothing: its rows are masked when the cache is read and dropped when it is written.
+ * Strides are in elements; rows have unit stride along D.  An e4m3 cache has one fp32 scale per row and head.
+ */
+typedef struct kb_paged_cache {
+  void* k;             /* [P, H_kv, page, D] */
+  void* v;
+  int64_t k_stride[3]; /* page, head, row */
+  int64_t v_stride[3];
+  float* k_scale;      /* [P, H_kv, page], KB_E4M3 only, otherwise NULL */
+  float* v_scale;
+  int64_t k_scale_stride[3];
+  int64_t v_scale_stride[3];
+  const int32_t* page_table; /* [B, M] */
+  int64_t table_stride[2];
+  const int32_t* lens; /* [B] */
+  int64_t lens_stride;
+  int32_t B, H_kv, D, P, M, page;
+  int32_t dtype; /* kb_dtype of the pages */
+} kb_paged_cache;
+
+/*
+ * Rotary position embedding with positions on several axes (time, height, width of a video, say).  Pair d of a head,
+ * elements d and d + R for d < R ("rotate half"), is turned by positions[axis(d)][b][t] * inv_freq[d]; axis a takes the pairs
+ * [section_end[a - 1], section_end[a]).  What is behind the first 2 R elements is copied.  `inverse` turns the other way: the
+ * gradient.  Outputs are contiguous [B, H, T, D].  k.data NULL: q alone.
+ */
+typedef struct kb_rotary_params {
+  kb_tensor4 q, k;
+  void* q_out;
+  void* k_out;
+  const void* positions;  /* int32, or int64 with pos64 */
+  int64_t pos_stride[3];  /* axis, b, t; 0 broadcasts */
+  const double* inv_freq; /* [R], device memory */
+  int32_t B, H, H_kv, T, D, R;
+  int32_t axes;           /* 1 .. 8 */
+  int32_t section_end[8];
+  int32_t pos64;
+  int32_t dtype;
+  int32_t inverse;
+} kb_rotary_params;
+
+KB_API int kb_rotary(const kb_rotary_params* p, void* stream);
+
+/*
+ * New tokens into the cache.  `lens` counts them already: token t < new_lens[b] (NULL: T) of sequence b goes to row
+ * lens[b] - new_lens[b] + t; rows outside [0, M * page) and rows without a page are dropped.  The pages have the tokens' type,
+ * or e4m3 with scale = max(|x| of the row) / 448 (at least 1e-12).  A written row's entry of `weights` (or NULL) becomes 0 and its
+ * entry of `row_positions` (or NULL) the token's position (positions NULL: the row).
+ */
+typedef struct kb_paged_write_params {
+  kb_paged_cache cache;
+  kb_tensor4 k, v; /* [B, H_kv, T, D] */
+  const int32_t* new_lens;
+  int64_t new_lens_stride;
+  const int32_t* positions; /* [B, T] */
+  int64_t positions_stride[2];
+  float* weights;         /* [B, H_kv, M * page], unit stride along the rows */
+  int64_t weights_stride[2];
+  int32_t* row_positions; /* the same */
+  int64_t row_positions_stride[2];
+  int32_t T;
+  int32_t dtype; /* of k and v */
+} kb_paged_write_params;
+
+KB_API int kb_paged_write(const kb_paged_write_params* p, void* stream);
+
+/*
+ * Attention of one token per sequence, the one in row lens[b] - 1, over the sequence's rows; with context_size > 0 over those
+ * rows r with (lens[b] - 1) / context_size - r / context_size <= back_contexts.  A sequence without rows gives 0 and lse 0.
+ * `lse` is base 2.  With `weights`, every seen row's softmax weight, summed over the query heads of its key/value head, is
+ * added to weights[b][head][row]; `lse` must then be given.  `workspace`: kb_paged_attention_workspace_bytes bytes (host-only; it
+ * looks at sizes and at whether `weights` is NULL), 16-byte aligned.
+ */
+typedef struct kb_paged_attention_params {
+  kb_paged_cache cache;
+  const void* q;       /* [B, H, D] */
+  int64_t q_stride[3];
+  void* o;             /* [B, H, D] contiguous, q's type */
+  float* lse;          /* [B, H] contiguous, or NULL */
+  float* weights;      /* [B, H_kv, M * page], unit stride along the rows, or NULL */
+  int64_t weights_stride[2];
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t H;
+  int32_t dtype; /* of q and o: the pages' type unless that is KB_E4M3 */
+  int32_t context_size; /* 0: no window */
+  int32_t back_contexts;
+  float sm_scale;
+  uint32_t flags; /* KB_FLAG_FORCE_GENERIC */
+} kb_paged_attention_params;
+
+KB_API uint64_t kb_paged_attention_workspace_bytes(const kb_paged_attention_params* p);
+KB_API int kb_paged_attention(const kb_paged_attention_params* p, void* stream);
+
+/*
+ * Eviction down to `budget` rows per sequence and head.  Rows rank by (row_positions above the sequence's and head's largest
+ * minus `recent`, first), then by weight (a NaN is below every number), then the lower row first; the first `budget` stay.
+ * Kept rows below the budget do not move; the i-th kept row behind it, in the order of rows, goes to the i-th row below it that came
+ * free.  Rows behind the budget are left as they were.  Lengths become min(lens, budget).
+ * weights_out, row_positions_out, lens_out: the inputs themselves (in place, all three), or buffers that do not overlap them, whose
+ * entries below the new length are written.  No page may stand in the table of two sequences that lose rows, or twice
+ * in one.  `workspace`: kb_paged_evict_workspace_bytes bytes (host-only), 4-byte aligned.
+ */
+typedef struct kb_paged_evict_params {
+  kb_paged_cache cache;
+  const float* weights; /* [B, H_kv, M * page], unit stride along the rows */
+  int64_t weights_stride[2];
+  const int32_t* row_positions;
+  int64_t row_positions_stride[2];
+  float* weights_out;
+  int64_t weights_out_stride[2];
+  int32_t* row_positions_out;
+  int64_t row_positions_out_stride[2];
+  int32_t* lens_out;
+  int64_t lens_out_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t budget; /* >= 1 */
+  int32_t recent; /* >= 0 */
+} kb_paged_evict_params;
+
+KB_API uint64_t kb_paged_evict_workspace_bytes(const kb_paged_evict_params* p);
+KB_API int kb_paged_evict(const kb_paged_evict_params* p, void* stream);
 
 /*
  * Row softmax over the last axis of a [rows, cols] fp32/f16/bf16 matrix.

@@ -15,7 +15,7 @@ _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "lib", "libkernels_b200.so")
 
 KB_STATUS_WORDS = 4
-KB_F32, KB_F16, KB_BF16 = 0, 1, 2
+KB_F32, KB_F16, KB_BF16, KB_E4M3 = 0, 1, 2, 3
 KB_FLAG_PRESCALE_QK, KB_FLAG_ALLOW_TF32, KB_FLAG_FORCE_GENERIC = 1, 2, 4
 KB_FLAG_BWD_SKIP_DQ, KB_FLAG_BWD_SKIP_DKDV, KB_FLAG_BWD_TWO_PASS, KB_FLAG_BWD_SKIP_DELTA = 8, 16, 32, 64
 KB_PATH_GENERIC, KB_PATH_SM100 = 0, 1
@@ -27,6 +27,7 @@ _DTYPES = {torch.float32: KB_F32, torch.float16: KB_F16, torch.bfloat16: KB_BF16
 EXPORTS = (
     "kb_sa_fwd", "kb_sa_fwd_fp8", "kb_quantize_fp8", "kb_sa_bwd", "kb_sa_bwd_workspace_bytes", "kb_sa_bwd_generic_workspace_bytes", "kb_sa_bwd_noalloc", "kb_sa_fwd_varlen", "kb_sa_bwd_varlen",
     "kb_sa_bwd_varlen_workspace_bytes", "kb_qkv_rope_proj", "kb_out_proj", "kb_fa_fwd", "kb_softmax_fwd", "kb_sa_plan", "kb_sa_tile_config",
+    "kb_rotary", "kb_paged_write", "kb_paged_attention", "kb_paged_attention_workspace_bytes", "kb_paged_evict", "kb_paged_evict_workspace_bytes",
     "kb_launch_count", "kb_strerror", "kb_last_cuda_error", "kb_version", "kb_selftest_wait_timeout", "kb_selftest_reader_group",
 )
 
@@ -122,6 +123,54 @@ class SoftmaxParams(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """kb_paged_cache: the pages, the sequences' page tables and lengths."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("k_scale_stride", C.c_int64 * 3), ("v_scale_stride", C.c_int64 * 3),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64 * 2), ("lens", C.c_void_p), ("lens_stride", C.c_int64),
+        ("B", C.c_int32), ("H_kv", C.c_int32), ("D", C.c_int32), ("P", C.c_int32), ("M", C.c_int32), ("page", C.c_int32),
+        ("dtype", C.c_int32),
+    ]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [
+        ("q", Tensor4), ("k", Tensor4), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("positions", C.c_void_p), ("pos_stride", C.c_int64 * 3), ("inv_freq", C.c_void_p),
+        ("B", C.c_int32), ("H", C.c_int32), ("H_kv", C.c_int32), ("T", C.c_int32), ("D", C.c_int32), ("R", C.c_int32),
+        ("axes", C.c_int32), ("section_end", C.c_int32 * 8), ("pos64", C.c_int32), ("dtype", C.c_int32), ("inverse", C.c_int32),
+    ]
+
+
+class PagedWriteParams(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("k", Tensor4), ("v", Tensor4), ("new_lens", C.c_void_p), ("new_lens_stride", C.c_int64),
+        ("positions", C.c_void_p), ("positions_stride", C.c_int64 * 2), ("weights", C.c_void_p), ("weights_stride", C.c_int64 * 2),
+        ("row_positions", C.c_void_p), ("row_positions_stride", C.c_int64 * 2), ("T", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
+class PagedAttentionParams(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("q", C.c_void_p), ("q_stride", C.c_int64 * 3), ("o", C.c_void_p), ("lse", C.c_void_p),
+        ("weights", C.c_void_p), ("weights_stride", C.c_int64 * 2), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("H", C.c_int32), ("dtype", C.c_int32), ("context_size", C.c_int32), ("back_contexts", C.c_int32),
+        ("sm_scale", C.c_float), ("flags", C.c_uint32),
+    ]
+
+
+class PagedEvictParams(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("weights", C.c_void_p), ("weights_stride", C.c_int64 * 2),
+        ("row_positions", C.c_void_p), ("row_positions_stride", C.c_int64 * 2),
+        ("weights_out", C.c_void_p), ("weights_out_stride", C.c_int64 * 2),
+        ("row_positions_out", C.c_void_p), ("row_positions_out_stride", C.c_int64 * 2),
+        ("lens_out", C.c_void_p), ("lens_out_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+        ("budget", C.c_int32), ("recent", C.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -158,6 +207,14 @@ def load() -> C.CDLL:
     lib.kb_qkv_rope_proj.argtypes = [C.POINTER(QkvProjParams), C.c_void_p]
     lib.kb_out_proj.argtypes = [C.POINTER(OutProjParams), C.c_void_p]
     lib.kb_qkv_rope_proj.restype = lib.kb_out_proj.restype = C.c_int
+    lib.kb_rotary.argtypes = [C.POINTER(RotaryParams), C.c_void_p]
+    lib.kb_paged_write.argtypes = [C.POINTER(PagedWriteParams), C.c_void_p]
+    lib.kb_paged_attention.argtypes = [C.POINTER(PagedAttentionParams), C.c_void_p]
+    lib.kb_paged_evict.argtypes = [C.POINTER(PagedEvictParams), C.c_void_p]
+    lib.kb_rotary.restype = lib.kb_paged_write.restype = lib.kb_paged_attention.restype = lib.kb_paged_evict.restype = C.c_int
+    lib.kb_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedAttentionParams)]
+    lib.kb_paged_evict_workspace_bytes.argtypes = [C.POINTER(PagedEvictParams)]
+    lib.kb_paged_attention_workspace_bytes.restype = lib.kb_paged_evict_workspace_bytes.restype = C.c_uint64
     for f in (lib.kb_sa_fwd, lib.kb_fa_fwd, lib.kb_sa_bwd, lib.kb_softmax_fwd):
         f.restype = C.c_int
     lib.kb_sa_plan.argtypes = [C.c_int32] * 6 + [C.POINTER(C.c_int32), C.POINTER(C.c_int32)]

@@ -37,6 +37,18 @@ int check_common(const P* p) {
 
 bool empty(int32_t B, int32_t H, int32_t T) { return B == 0 || H == 0 || T == 0; }
 
+// What holds for every entry point with a paged cache.
+int check_paged_cache(const kb_paged_cache& c) {
+  if (c.B < 0 || c.H_kv < 0 || c.P < 0 || c.M < 0 || c.page < 1) return KB_ERR_BAD_ARGUMENT;
+  if (!(dtype_ok(c.dtype) || c.dtype == KB_E4M3) || !head_dim_ok(c.D)) return KB_ERR_UNSUPPORTED;
+  if (c.B > 65535 || c.H_kv > 65535 || (int64_t)c.M * c.page > (int64_t)1 << 30) return KB_ERR_TOO_LARGE;
+  if (c.B > 0 && (!c.lens || (c.M > 0 && !c.page_table))) return KB_ERR_BAD_ARGUMENT;
+  if (c.P > 0 && c.H_kv > 0 && (!c.k || !c.v)) return KB_ERR_BAD_ARGUMENT;
+  if (c.dtype == KB_E4M3 && c.P > 0 && c.H_kv > 0 && (!c.k_scale || !c.v_scale)) return KB_ERR_BAD_ARGUMENT;
+  return KB_OK;
+}
+bool no_rows(const kb_paged_cache& c) { return c.M == 0; }
+
 // The tcgen05 path wants 16-bit inputs, a head dim of 64 or 128, unit stride along the head
 // dim and 16-byte aligned rows (TMA's requirements on the tensor map).
 bool tma_ok(const kb_tensor4& t, size_t elsize) {
@@ -405,6 +417,64 @@ int kb_quantize_fp8(const kb_quantize_fp8_params* p, void* stream) {
   if (p->B == 0 || p->H == 0 || p->T == 0) return KB_OK;
   if (!p->x.data || !p->x8 || !p->scale) return KB_ERR_BAD_ARGUMENT;
   return kb::quantize_fp8(*p, static_cast<cudaStream_t>(stream));
+}
+
+int kb_rotary(const kb_rotary_params* p, void* stream) {
+  if (!p || p->B < 0 || p->H < 0 || p->H_kv < 0 || p->T < 0) return KB_ERR_BAD_ARGUMENT;
+  if (!kb::dtype_ok(p->dtype) || !kb::head_dim_ok(p->D)) return KB_ERR_UNSUPPORTED;
+  if (p->R < 1 || p->R > p->D / 2 || p->axes < 1 || p->axes > 8) return KB_ERR_BAD_ARGUMENT;
+  for (int i = 0; i < p->axes; ++i)
+    if (p->section_end[i] < (i ? p->section_end[i - 1] : 0)) return KB_ERR_BAD_ARGUMENT;
+  if (p->section_end[p->axes - 1] != p->R) return KB_ERR_BAD_ARGUMENT;
+  if (kb::empty(p->B, p->H + (p->k.data ? p->H_kv : 0), p->T)) return KB_OK;
+  if (!p->q.data || !p->q_out || (p->k.data && !p->k_out) || !p->positions || !p->inv_freq) return KB_ERR_BAD_ARGUMENT;
+  if ((int64_t)p->B * p->T > (int64_t)1 << 30 || p->H > 65535 || p->H_kv > 65535) return KB_ERR_TOO_LARGE;
+  return kb::rotary(*p, static_cast<cudaStream_t>(stream));
+}
+
+int kb_paged_write(const kb_paged_write_params* p, void* stream) {
+  if (!p || p->T < 0) return KB_ERR_BAD_ARGUMENT;
+  if (int rc = kb::check_paged_cache(p->cache)) return rc;
+  if (!kb::dtype_ok(p->dtype)) return KB_ERR_UNSUPPORTED;
+  if (kb::empty(p->cache.B, p->cache.H_kv, p->T) || kb::no_rows(p->cache)) return KB_OK;
+  if (!p->k.data || !p->v.data) return KB_ERR_BAD_ARGUMENT;
+  return kb::paged_write(*p, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t kb_paged_attention_workspace_bytes(const kb_paged_attention_params* p) {
+  if (!p || p->H < 0 || kb::check_paged_cache(p->cache) || kb::empty(p->cache.B, p->cache.H_kv, p->H)) return 0;
+  return kb::paged_attention_workspace_bytes(*p);
+}
+
+int kb_paged_attention(const kb_paged_attention_params* p, void* stream) {
+  if (!p || p->H < 0 || p->context_size < 0 || p->back_contexts < 0) return KB_ERR_BAD_ARGUMENT;
+  if (int rc = kb::check_paged_cache(p->cache)) return rc;
+  if (!kb::dtype_ok(p->dtype) || (p->cache.dtype != KB_E4M3 && p->cache.dtype != p->dtype)) return KB_ERR_UNSUPPORTED;
+  if (kb::empty(p->cache.B, 1, p->H)) return KB_OK;
+  if (p->cache.H_kv < 1 || p->H % p->cache.H_kv || !p->q || !p->o || (p->weights && !p->lse)) return KB_ERR_BAD_ARGUMENT;
+  if (p->H > 65535) return KB_ERR_TOO_LARGE;
+  const uint64_t need = kb::paged_attention_workspace_bytes(*p);
+  if (need && (!p->workspace || p->workspace_bytes < need || reinterpret_cast<uintptr_t>(p->workspace) % 16)) return KB_ERR_BAD_ARGUMENT;
+  return kb::paged_attention(*p, static_cast<cudaStream_t>(stream));
+}
+
+uint64_t kb_paged_evict_workspace_bytes(const kb_paged_evict_params* p) {
+  if (!p || p->budget < 1 || kb::check_paged_cache(p->cache)) return 0;
+  return kb::paged_evict_workspace_bytes(p->cache, p->budget);
+}
+
+int kb_paged_evict(const kb_paged_evict_params* p, void* stream) {
+  if (!p || p->budget < 1 || p->recent < 0) return KB_ERR_BAD_ARGUMENT;
+  if (int rc = kb::check_paged_cache(p->cache)) return rc;
+  if (p->cache.B == 0) return KB_OK;
+  if (!p->lens_out || p->cache.H_kv < 1) return KB_ERR_BAD_ARGUMENT;
+  if (!kb::no_rows(p->cache) && (!p->weights || !p->row_positions || !p->weights_out || !p->row_positions_out)) return KB_ERR_BAD_ARGUMENT;
+  const bool in_place = p->weights == p->weights_out;
+  if (!kb::no_rows(p->cache) && (in_place != (p->row_positions == p->row_positions_out) || in_place != (p->cache.lens == p->lens_out)))
+    return KB_ERR_BAD_ARGUMENT;
+  if (!p->workspace || p->workspace_bytes < kb::paged_evict_workspace_bytes(p->cache, p->budget) || reinterpret_cast<uintptr_t>(p->workspace) % 4)
+    return KB_ERR_BAD_ARGUMENT;
+  return kb::paged_evict(*p, static_cast<cudaStream_t>(stream));
 }
 
 int kb_softmax_fwd(const kb_softmax_params* p, void* stream) {

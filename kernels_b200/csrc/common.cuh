@@ -68,5 +68,11 @@ size_t sa_bwd_fused_workspace_bytes(int32_t B, int32_t H, int32_t T, int32_t c, 
 size_t sa_bwd_fused_workspace_bytes_packed(int32_t B, int32_t H, int32_t total, int32_t max_len, int32_t c, int32_t back);
 int quantize_fp8(const kb_quantize_fp8_params& p, cudaStream_t s);
 int softmax_rows(const kb_softmax_params& p, cudaStream_t s);
+int rotary(const kb_rotary_params& p, cudaStream_t s);
+int paged_write(const kb_paged_write_params& p, cudaStream_t s);
+size_t paged_attention_workspace_bytes(const kb_paged_attention_params& p);
+int paged_attention(const kb_paged_attention_params& p, cudaStream_t s);
+size_t paged_evict_workspace_bytes(const kb_paged_cache& c, int32_t budget);
+int paged_evict(const kb_paged_evict_params& p, cudaStream_t s);
 
 }  // namespace kb

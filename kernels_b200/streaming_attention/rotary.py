@@ -1,0 +1,92 @@
+"""Rotary position embedding with positions on several axes.
+
+The reference leaves rotary embedding to its callers; :func:`qkv_rope_projection` applies one table of positions, the same
+for every sequence.  Tokens of a video or an image stand on several axes (time, height, width), and the
+newest tokens of a batch of streams stand at positions of their own.  Here every token brings its position on each axis,
+and every axis turns its own band of the frequencies.
+
+One kernel (``kb_rotary``), differentiable in ``q`` and ``k``: the gradient is the same kernel turning the other way.
+There is no CPU path.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from .. import _lib
+
+
+def _rotate(q, k, positions, inv_freq, ends, inverse):
+    B, H, T, D = q.shape
+    p = _lib.RotaryParams()
+    q_out = torch.empty((B, H, T, D), dtype=q.dtype, device=q.device)
+    p.q, p.q_out = _lib.tensor4(q), q_out.data_ptr()
+    k_out = None
+    if k is not None:
+        k_out = torch.empty((B, k.shape[1], T, D), dtype=q.dtype, device=q.device)
+        p.k, p.k_out, p.H_kv = _lib.tensor4(k), k_out.data_ptr(), k.shape[1]
+        if k.numel() == 0:
+            p.k.data = None
+    p.positions, p.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+    strides = positions.stride()
+    p.pos_stride[:] = strides if len(strides) == 3 else (strides[0], 0, strides[1])
+    p.B, p.H, p.T, p.D, p.R, p.axes = B, H, T, D, ends[-1], len(ends)
+    p.section_end[: len(ends)] = ends
+    p.pos64 = positions.dtype == torch.int64
+    p.dtype = _lib.dtype_code(q.dtype)
+    p.inverse = inverse
+    _lib.check(_lib.launch(_lib.load().kb_rotary, p, q.device), "kb_rotary")
+    return q_out, k_out
+
+
+class _RotaryEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, ends, inverse):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.ends, ctx.inverse = ends, inverse
+        ctx.shapes = q.shape, None if k is None else k.shape
+        return _rotate(q, k, positions, inv_freq, ends, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, inv_freq = ctx.saved_tensors
+        # (turned by the same function, so that gradients have gradients)
+        dq, dk = _RotaryEmbedding.apply(dq, dk, positions, inv_freq, ctx.ends, not ctx.inverse)
+        return dq, dk, None, None, None, None
+
+
+def rotary_embedding(
+    q: torch.Tensor,
+    k: Optional[torch.Tensor],
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    sections: Optional[Sequence[int]] = None,
+):
+    """``(q', k')``: pair ``d`` of every head (elements ``d`` and ``d + R``, ``d < R``) turned by ``positions[axis(d)] *
+    inv_freq[d]``; contiguous, in the inputs' type.  Differentiable in ``q`` and ``k``.
+
+    ``q``: ``[B, H, T, D]``, ``k``: ``[B, H_kv, T, D]`` or None (then ``k'`` is None), fp32, fp16 or bf16, any strides.
+    ``positions``: int32 or int64, ``[A, B, T]``, or ``[A, T]`` for the same positions in every sequence; any whole numbers, far
+    ones too: the angle is formed modulo a turn before it is rounded.  ``inv_freq``: float64 ``[R]``, radians per step, ``R <= D / 2``;
+    elements from ``2 R`` on are copied.  ``sections``: how many frequencies each of the ``A`` axes (at most 8) takes, in order,
+    ``R`` in all; None for one axis.
+    """
+    if not q.is_cuda:
+        raise RuntimeError("rotary_embedding: the tensors must live on a CUDA device (there is no CPU path)")
+    assert q.ndim == 4 and positions.ndim in (2, 3) and inv_freq.ndim == 1
+    B, _, T, D = q.shape
+    if k is not None:
+        assert k.ndim == 4 and k.shape[0] == B and k.shape[2] == T and k.shape[3] == D and k.dtype == q.dtype and k.device == q.device
+    assert positions.dtype in (torch.int32, torch.int64) and positions.device == q.device
+    assert positions.shape[1:] == ((T,) if positions.ndim == 2 else (B, T)), "positions are [A, T] or [A, B, T]"
+    assert inv_freq.dtype == torch.float64 and inv_freq.device == q.device and 1 <= inv_freq.shape[0] <= D // 2
+    sections = (inv_freq.shape[0],) if sections is None else tuple(int(n) for n in sections)
+    assert 1 <= len(sections) <= 8 and len(sections) == positions.shape[0], "one section of frequencies per axis, at most 8"
+    assert min(sections) >= 0 and sum(sections) == inv_freq.shape[0], "the sections share out inv_freq"
+    ends = [sum(sections[: a + 1]) for a in range(len(sections))]
+    inv_freq = inv_freq.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryEmbedding.apply(q, k, positions, inv_freq, ends, False)
+    return _rotate(q, k, positions, inv_freq, ends, False)

@@ -1,0 +1,196 @@
+"""GPU: rotary positions with several axes against the 64-bit formula, and their gradients.
+
+Tolerance: an output is rounded once, by half a step of its type at most; before that it is ``x1 c - x2 s`` in fp32.
+The angle's part below a turn is rounded to fp32 (half a turn at most: pi 2^-24 off), ``sincospif`` is exact to 2 units of
+2^-24 of 1, the product and the FMA add 2^-24 each: below (pi + 2 + 2) 2^-24 < 5e-7 of ``|x1| + |x2|``.
+"""
+
+import pytest
+import torch
+
+from oracle import paged_oracle as PO
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def _tolerance(ref, x, R, dtype):
+    turned = torch.zeros_like(ref)
+    pair = x[..., :R].double().abs() + x[..., R: 2 * R].double().abs()
+    turned[..., : 2 * R] = torch.cat([pair, pair], -1) * 5e-7
+    least = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    return ref.abs() * torch.finfo(dtype).eps / 2 * (1 + 1e-3) + turned * (1 + torch.finfo(dtype).eps) + least
+
+
+def _inputs(B, H, H_kv, T, D, R, sections, dtype, far, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q, k = (torch.randn(B, h, T, D, generator=g).to(dtype) for h in (H, H_kv))
+    positions = torch.randint(-far, far + 1, (len(sections), B, T), generator=g)
+    inv_freq = 10000.0 ** (-torch.arange(R, dtype=torch.float64) / R)
+    return q, k, positions, inv_freq
+
+
+@pytest.mark.parametrize("B,H,H_kv,T,D,sections,dtype,far,pos_dtype", [
+    (2, 4, 2, 37, 64, (32,), BF16, 5000, torch.int32),
+    (3, 32, 8, 1, 128, (16, 24, 24), BF16, 1000000, torch.int32),       # one token per stream
+    (1, 2, 2, 300, 64, (8, 12, 12), F16, 2**31 - 1, torch.int32),       # the farthest 32-bit positions, negative ones too
+    (2, 3, 1, 65, 128, (64,), F32, 2**40, torch.int64),                 # farther still
+    (1, 1, 1, 1, 16, (8,), F32, 10, torch.int64),
+    (2, 5, 5, 33, 256, (64, 64), BF16, 4096, torch.int32),
+    (2, 4, 4, 50, 128, (16, 16), BF16, 4096, torch.int32),              # half of the head is not rotated
+    (2, 2, 2, 19, 64, (5, 2, 6), F16, 4096, torch.int32),               # an odd number of pairs: no vectors
+    (1, 2, 2, 7, 32, (0, 16), F32, 100, torch.int32),                   # an axis without frequencies
+    (1, 1, 1, 9, 32, (1,), BF16, 100, torch.int32),
+    (1, 2, 1, 40, 64, (4,) * 8, F16, 1000, torch.int32),                # eight axes
+    (70000, 1, 1, 1, 16, (8,), F16, 1000, torch.int32),                 # more sequences than a grid's second dimension
+])
+def test_rotary_matches_formula(B, H, H_kv, T, D, sections, dtype, far, pos_dtype):
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    R = sum(sections)
+    q, k, positions, inv_freq = _inputs(B, H, H_kv, T, D, R, sections, dtype, far)
+    got = rotary_embedding(q.cuda(), k.cuda(), positions.to(pos_dtype).cuda(), inv_freq.cuda(), sections)
+    if far > 2**31:
+        # 2^40 radians in fp64 are off by 2^-13: the reference takes the part below a turn exactly
+        from fractions import Fraction
+
+        two_pi = Fraction("6.28318530717958647692528676655900576839433879875021164194988918461563281257")
+        turns = [Fraction(float(f)) / two_pi for f in inv_freq]
+        small = torch.empty(R, *positions.shape[1:], dtype=torch.float64)
+        for d in range(R):
+            for b in range(B):
+                for t in range(T):
+                    x = int(positions[0, b, t]) * turns[d]
+                    small[d, b, t] = float((x - (x.numerator // x.denominator)) * two_pi)
+        # (one axis per frequency with the reduced angle as its position and frequency 1)
+        ref = [PO.rotary(x, small, torch.ones(R), (1,) * R) for x in (q, k)]
+        slack = far * 2**-51  # the kernel's frequency in turns is a product in fp64 of two numbers of 53 bits
+    else:
+        ref = [PO.rotary(x, positions, inv_freq, sections) for x in (q, k)]
+        # the reference's own angle in fp64, and the kernel's 53-bit frequency: p 2^-52 radians each
+        slack = 2 * far * 2**-52
+    for x, y, r in zip((q, k), got, ref):
+        assert y.dtype == dtype and y.is_contiguous()
+        pair = x.double().abs().max() * 2
+        assert ((y.cpu().double() - r).abs() <= _tolerance(r, x, R, dtype) + slack * pair).all()
+        assert torch.equal(y.cpu()[..., 2 * R:], x[..., 2 * R:])
+
+
+def test_rotary_takes_any_layout_and_broadcast_positions():
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    q, k, positions, inv_freq = _inputs(2, 4, 2, 21, 64, 32, (16, 16), F16, 500)
+    qs = q.transpose(1, 2).contiguous().cuda().transpose(1, 2)               # [B, T, H, D] underneath
+    ks = torch.zeros(2, 2, 21, 65, dtype=F16, device="cuda")[..., 1:]         # rows off the 16-byte boundaries
+    ks.copy_(k)
+    same = positions[:, :1].expand(2, 2, 21)
+    want = rotary_embedding(q.cuda(), k.cuda(), same.contiguous().cuda(), inv_freq.cuda(), (16, 16))
+    for pos in (positions[:, 0].cuda(), positions[:, :1].cuda().expand(2, 2, 21), positions[:, 0].t().contiguous().cuda().t()):
+        for a, b in ((qs, ks), (q.cuda(), ks), (qs, k.cuda())):
+            got = rotary_embedding(a, b, pos, inv_freq.cuda(), (16, 16))
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    alone = rotary_embedding(qs, None, positions[:, 0].cuda(), inv_freq.cuda(), (16, 16))
+    assert alone[1] is None and torch.equal(alone[0], want[0])
+    flipped = q.cuda().transpose(2, 3).contiguous().transpose(2, 3)           # D is not the inner axis
+    assert torch.equal(rotary_embedding(flipped, None, positions[:, 0].cuda(), inv_freq.cuda(), (16, 16))[0], want[0])
+
+
+def test_rotary_empty_calls():
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    f = torch.ones(8, dtype=torch.float64, device="cuda")
+    for B, H, T in ((0, 2, 3), (2, 0, 3), (2, 2, 0)):
+        x = torch.zeros(B, H, T, 16, device="cuda")
+        y, z = rotary_embedding(x, x, torch.zeros(1, B, T, dtype=torch.int32, device="cuda"), f)
+        assert y.shape == x.shape and z.shape == x.shape
+    q, k = torch.randn(2, 2, 3, 16, device="cuda"), torch.randn(2, 0, 3, 16, device="cuda")
+    y, z = rotary_embedding(q, k, torch.zeros(1, 2, 3, dtype=torch.int32, device="cuda"), f)
+    assert torch.equal(y, q) and z.shape == k.shape
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_rotary_gradient_is_the_opposite_turn(dtype):
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    sections, R = (4, 6, 6), 16
+    q, k, positions, inv_freq = _inputs(2, 4, 2, 33, 64, R, sections, dtype, 2000, seed=1)
+    gq, gk = _inputs(2, 4, 2, 33, 64, R, sections, dtype, 10, seed=2)[:2]
+    qc, kc = q.cuda().requires_grad_(), k.cuda().requires_grad_()
+    y = rotary_embedding(qc, kc, positions.cuda(), inv_freq.cuda(), sections)
+    dq, dk = torch.autograd.grad(y, (qc, kc), (gq.cuda(), gk.cuda().transpose(1, 2).contiguous().transpose(1, 2)))
+    for g, d in ((gq, dq), (gk, dk)):
+        ref = PO.rotary(g, -positions, inv_freq, sections)
+        assert ((d.cpu().double() - ref).abs() <= _tolerance(ref, g, R, dtype) + 4000 * 2**-52 * 20).all()
+
+
+def test_rotary_gradient_against_differences():
+    """fp32, central differences of a weighted sum: the operator is linear, so they are exact up to rounding.  The sum has
+    768 terms of about 1 in fp64 over fp32 outputs, each off by 5e-7 (|x1| + |x2|) < 5e-6 at a step of 1: far below 1e-4."""
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    sections = (3, 5)
+    q, _, positions, inv_freq = _inputs(1, 2, 1, 12, 32, 8, sections, F32, 50, seed=3)
+    g = torch.randn(q.shape, generator=torch.Generator().manual_seed(4)).double()
+    qc = q.cuda().requires_grad_()
+    f = lambda x: (rotary_embedding(x, None, positions.cuda(), inv_freq.cuda(), sections)[0].double().cpu() * g).sum()  # noqa: E731
+    (dq,) = torch.autograd.grad(f(qc), qc)
+    for i in ((0, 0, 0, 0), (0, 1, 7, 9), (0, 1, 11, 15), (0, 0, 3, 31), (0, 1, 5, 2)):
+        e = torch.zeros_like(q)
+        e[i] = 1.0
+        with torch.no_grad():
+            slope = (f((q + e).cuda()) - f((q - e).cuda())) / 2
+        assert abs(float(slope) - float(dq[i])) < 1e-4
+
+
+def test_rotary_second_gradients_and_unused_outputs():
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    sections = (8,)
+    q, k, positions, inv_freq = (x.cuda() for x in _inputs(1, 2, 2, 5, 16, 8, sections, F32, 9))
+    q.requires_grad_(), k.requires_grad_()
+    y, _ = rotary_embedding(q, k, positions, inv_freq)
+    (dq,) = torch.autograd.grad(y.square().sum() / 2, q, create_graph=True)
+    assert torch.allclose(dq, q, atol=1e-5)  # a rotation's transpose undoes it
+    (again,) = torch.autograd.grad(dq.square().sum() / 2, q)
+    assert torch.allclose(again, q, atol=1e-5)
+
+
+def test_rotary_in_a_graph_and_on_another_stream():
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    q, k, positions, inv_freq = (x.cuda() for x in _inputs(2, 4, 2, 17, 64, 32, (32,), BF16, 500))
+    want = rotary_embedding(q, k, positions, inv_freq)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = rotary_embedding(q, k, positions, inv_freq)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    x, pos = torch.empty_like(q), torch.zeros_like(positions)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, _ = rotary_embedding(x, k, pos, inv_freq)
+    x.copy_(q), pos.copy_(positions)
+    graph.replay()
+    assert torch.equal(y, want[0])
+
+
+def test_rotary_refusals():
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    q, k, positions, inv_freq = (x.cuda() for x in _inputs(2, 4, 2, 17, 64, 32, (32,), BF16, 500))
+    bad = [
+        dict(positions=positions.float()), dict(positions=positions[:, :1]), dict(positions=positions[0, 0]), dict(inv_freq=inv_freq.float()),
+        dict(sections=(16, 16)), dict(sections=(31,)), dict(sections=(33, -1), positions=positions.expand(2, 2, 17)), dict(k=k.half()),
+        dict(k=k[:1]), dict(inv_freq=torch.ones(33, dtype=torch.float64, device="cuda")), dict(positions=positions.cpu()),
+        dict(positions=positions.expand(9, 2, 17), sections=(32,) + (0,) * 8),
+    ]
+    for change in bad:
+        args = dict(q=q, k=k, positions=positions, inv_freq=inv_freq) | change
+        with pytest.raises(AssertionError):
+            rotary_embedding(**args)
+    with pytest.raises(RuntimeError, match="unsupported"):
+        rotary_embedding(q.double(), None, positions, inv_freq)
+    with pytest.raises(RuntimeError, match="unsupported"):
+        rotary_embedding(q[..., :48], None, positions, inv_freq[:24])
