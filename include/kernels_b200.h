@@ -468,7 +468,6 @@ typedef struct kb_paged_attention_params {
   int32_t context_size; /* 0: no window */
   int32_t back_contexts;
   float sm_scale;
-  uint32_t flags; /* KB_FLAG_FORCE_GENERIC */
 } kb_paged_attention_params;
 
 KB_API uint64_t kb_paged_attention_workspace_bytes(const kb_paged_attention_params* p);

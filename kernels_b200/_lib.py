@@ -156,7 +156,7 @@ class PagedAttentionParams(C.Structure):
         ("cache", PagedCache), ("q", C.c_void_p), ("q_stride", C.c_int64 * 3), ("o", C.c_void_p), ("lse", C.c_void_p),
         ("weights", C.c_void_p), ("weights_stride", C.c_int64 * 2), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
         ("H", C.c_int32), ("dtype", C.c_int32), ("context_size", C.c_int32), ("back_contexts", C.c_int32),
-        ("sm_scale", C.c_float), ("flags", C.c_uint32),
+        ("sm_scale", C.c_float),
     ]
 
 

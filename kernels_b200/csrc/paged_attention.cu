@@ -16,6 +16,7 @@
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "sm100_host.h"
 #include "sm100_ptx.cuh"
 
 namespace kb {
@@ -214,6 +215,411 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
   }
 }
 
+// ---- tensor-core kernel ----------------------------------------------------------------------------------------------
+//
+// 16-bit and e4m3 caches of head dim 64 and 128.  A warp multiplies the 16 (or 8) query heads of a block with 16 keys at a time
+// (m16n8k16): the heads are the rows, so up to 16 heads cost what one does, and what the tensor cores have to do is a
+// small part of the time that the keys take to arrive.  That time is all there is to hide, and every warp hides it for itself: it
+// has tiles of kR rows of its own (every fourth of the block's), a ring of kStages of them in shared memory filled by
+// 16-byte asynchronous copies, and a softmax of its own, so that no warp waits for another before the end.
+//
+// Rows are found one by one (a lane looks up a row), so pages of any size and order are read the same way; a row that is
+// masked is filled with zeros without being read, so that nothing in it can reach a sum.
+//
+// e4m3 elements become f16, exactly.  q does too (bf16 q after a multiplication by a power of two that brings its largest element to
+// 2^14: what is lost lies 2^-38 below the largest).  A row's value scale belongs to its weight: the weights that are
+// multiplied are p * v_scale, so the running maximum is taken over score + log2(v_scale), which keeps them within f16.
+// f16 weights start at 2^7 and may grow to 2^15 before sums are rescaled: seven bits more for the small ones.
+// Weights are rounded to 16 bits for the product with V (as in the operator's forward kernel); their sum is taken before that.
+
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t to, const void* from, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// c += a b, 16 x 8 x 16; with HALF the rows 8 .. 15 are not there
+template <bool BF16, bool HALF>
+__device__ __forceinline__ void mma16(float (&c)[HALF ? 2 : 4], const uint32_t (&a)[HALF ? 2 : 4], uint32_t b0, uint32_t b1) {
+  float x2, x3;
+  if constexpr (HALF) {
+    if constexpr (BF16)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %8, %5, %8}, {%6, %7}, {%0, %1, %9, %9};"
+          : "+f"(c[0]), "+f"(c[1]), "=f"(x2), "=f"(x3) : "r"(a[0]), "r"(a[1]), "r"(b0), "r"(b1), "r"(0), "f"(0.f));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %8, %5, %8}, {%6, %7}, {%0, %1, %9, %9};"
+          : "+f"(c[0]), "+f"(c[1]), "=f"(x2), "=f"(x3) : "r"(a[0]), "r"(a[1]), "r"(b0), "r"(b1), "r"(0), "f"(0.f));
+  } else {
+    if constexpr (BF16)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+
+// kF8: e4m3 cache (products in f16); kBf16: products in bf16, otherwise in f16; kHalf: at most eight query heads per block
+template <bool kF8, bool kBf16, int kD, bool kHalf>
+struct MmaTile {
+  static constexpr int kRowBytes = kF8 ? kD : 2 * kD, kChunks = kRowBytes / 16;
+  static constexpr int kR = kRowBytes == 256 ? 16 : 32;            // rows of a tile
+  static constexpr int kStages = kRowBytes == 64 ? 4 : 3;
+  static constexpr int kScaleBytes = kF8 ? 2 * kR * 4 : 0;
+  static constexpr int kStageBytes = 2 * kR * kRowBytes + kScaleBytes;
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kHeads = kHalf ? 8 : 16, kS = kHalf ? 1 : 2; // kS: heads per thread
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  // Where chunk c of row r lies: at c ^ swizzle(r).  The eight rows of a matrix load hit different banks, and so do the two rows
+  // and four chunks of a 16-byte load of e4m3 keys.
+  static __device__ __forceinline__ int swizzle(int r) { return !kF8 ? r & 7 : kD == 128 ? ((r & 1) << 2) | ((r >> 1) & 3) : (r >> 1) & 3; }
+  static_assert(kSmem >= kWarps * kHeads * kD * 4, "the warps' outputs are joined where the ring was");
+};
+
+template <bool kF8, bool kBf16, int kD, bool kHalf>
+__global__ void __launch_bounds__(kThreads) paged_attend_mma_kernel(const AttendArgs a) {
+  using Tile = MmaTile<kF8, kBf16, kD, kHalf>;
+  constexpr int kR = Tile::kR, kStages = Tile::kStages, kChunks = Tile::kChunks, kRowBytes = Tile::kRowBytes, kHeads = Tile::kHeads, kS = Tile::kS;
+  constexpr int kSteps = kD / 16, kNt = kR / 8, kDt = kD / 8, kA = 2 * kS;
+  constexpr float kOffset = kBf16 ? 0.f : 7.f, kSlack = 8.f;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float m_s[kWarps][16], l_s[kWarps][16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, oct = lane >> 2;
+  const int32_t split = blockIdx.x, hk = blockIdx.y / a.head_tiles, b = blockIdx.z;
+  const int32_t h0 = hk * a.group + (blockIdx.y - hk * a.head_tiles) * kHeads, heads = min(kHeads, (hk + 1) * a.group - h0);
+  int32_t first, end;
+  seen_rows(a, b, first, end);
+  split_rows(a, split, kWarps * kR, first, end);
+  const uint32_t ring = sm100::smem_u32(smem) + warp * Tile::kWarpBytes;
+
+  // ---- copies: lane r looks up row r of the tile
+  const char* kbase = a.c.k + hk * a.c.k_head * (kF8 ? 1 : 2);
+  const char* vbase = a.c.v + hk * a.c.v_head * (kF8 ? 1 : 2);
+  constexpr uint32_t kNoRow = 0xffffffffu;
+  int32_t next_row = first + warp * kR + (lane & (kR - 1));  // the row that this lane looks up next
+  uint32_t live_bits[kStages - 1];                           // of the tiles in the ring, oldest first
+  auto issue = [&](int stage) -> uint32_t {
+    uint32_t at16 = kNoRow;
+    int32_t at = 0, page = -1;
+    if (next_row < end) page = a.c.locate(b, next_row, at);
+    if (page >= 0) at16 = (uint32_t)((uint64_t)((page * a.c.k_page + at * a.c.k_row) * (kF8 ? 1 : 2)) >> 4);
+    const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
+    const uint32_t to = ring + stage * Tile::kStageBytes;
+    constexpr int kRowsAtOnce = 32 / kChunks;
+    const int chunk = lane % kChunks, sub = lane / kChunks;
+#pragma unroll
+    for (int i = 0; i < kR / kRowsAtOnce; ++i) {
+      const int r = i * kRowsAtOnce + sub;
+      const uint32_t row16 = __shfl_sync(0xffffffffu, at16, r);
+      const bool ok = row16 != kNoRow;
+      const uint64_t off = ok ? ((uint64_t)row16 + chunk) * 16 : 0;
+      const uint32_t place = r * kRowBytes + ((chunk ^ Tile::swizzle(r)) * 16);
+      cp_async16(to + place, kbase + off, ok);
+      cp_async16(to + kR * kRowBytes + place, vbase + off, ok);
+    }
+    if constexpr (kF8) {
+      const int64_t so = page >= 0 ? page * a.c.ks_page + hk * a.c.ks_head + at * a.c.ks_row : 0;
+      cp_async4(to + 2 * kR * kRowBytes + lane * 4, a.c.k_scale + so, page >= 0);
+      cp_async4(to + 2 * kR * kRowBytes + kR * 4 + lane * 4, a.c.v_scale + so, page >= 0);
+    }
+    next_row += kWarps * kR;
+    return live;
+  };
+  // (tiles behind the last are empty: nothing is read)
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    live_bits[s] = issue(s);
+    cp_async_commit();
+  }
+
+  // ---- q as the products' left operand; with an e4m3 cache a lane's elements are the ones its 16-byte key loads hold
+  uint32_t q[kSteps][kA];
+  float back_scale[kS];
+#pragma unroll
+  for (int s = 0; s < kS; ++s) {
+    const int g = oct + 8 * s;
+    const bool there = g < heads;
+    const int64_t base = b * a.q_b + (int64_t)(h0 + (there ? g : 0)) * a.q_h;
+    float up = 1.f;
+    back_scale[s] = a.scale_log2;
+    if (kF8 && a.dtype == KB_BF16) {
+      float top = 0.f;
+      for (int d = quad; d < kD; d += 4) top = fmaxf(top, there ? fabsf(load_any(a.q, base + d * a.q_d, a.dtype)) : 0.f);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = (int)(__float_as_uint(top) >> 23) - 127;  // top in [2^e, 2^(e+1))
+      if (top > 0.f && e < 128) {
+        const int by = max(-100, min(100, 14 - e));
+        up = __uint_as_float((uint32_t)(by + 127) << 23);
+        back_scale[s] *= __uint_as_float((uint32_t)(127 - by) << 23);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int d = kF8 ? t / 4 * 64 + quad * 16 + t % 4 * 4 + 2 * p : t * 16 + 8 * p + quad * 2;
+        const float x = there ? load_any(a.q, base + d * a.q_d, a.dtype) * up : 0.f;
+        const float y = there ? load_any(a.q, base + (d + 1) * a.q_d, a.dtype) * up : 0.f;
+        q[t][p * kS + s] = sm100::pack16x2<kBf16>(x, y);
+      }
+  }
+
+  float o[kDt][kA], m[kS], l[kS];
+#pragma unroll
+  for (int s = 0; s < kS; ++s) m[s] = -INFINITY, l[s] = 0.f;
+#pragma unroll
+  for (int j = 0; j < kDt; ++j)
+#pragma unroll
+    for (int i = 0; i < kA; ++i) o[j][i] = 0.f;
+
+  int stage = 0;
+  for (int32_t r0 = first + warp * kR; r0 < end; r0 += kWarps * kR) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    const uint32_t at = ring + stage * Tile::kStageBytes, vat = at + kR * kRowBytes;
+    const uint32_t live = live_bits[0];
+    // every lane is through with the tile before this one: the next copies take its place
+#pragma unroll
+    for (int s = 0; s < kStages - 2; ++s) live_bits[s] = live_bits[s + 1];
+    live_bits[kStages - 2] = issue(stage == 0 ? kStages - 1 : stage - 1);
+    cp_async_commit();
+
+    // scores
+    float sc[kNt][kA];
+#pragma unroll
+    for (int j = 0; j < kNt; ++j)
+#pragma unroll
+      for (int i = 0; i < kA; ++i) sc[j][i] = 0.f;
+    if constexpr (!kF8) {
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+        for (int j = 0; j < kNt; j += 2) {
+          const int key = j * 8 + (lane & 7) + (lane >> 4) * 8, chunk = t * 2 + ((lane >> 3) & 1);
+          uint32_t r[4];
+          ldsm4(r, at + key * kRowBytes + ((chunk ^ Tile::swizzle(key)) * 16));
+          mma16<kBf16, kHalf>(sc[j], q[t], r[0], r[1]);
+          mma16<kBf16, kHalf>(sc[j + 1], q[t], r[2], r[3]);
+        }
+    } else {
+#pragma unroll
+      for (int t4 = 0; t4 < kSteps / 4; ++t4)
+#pragma unroll
+        for (int j = 0; j < kNt; ++j) {
+          const int key = j * 8 + oct, chunk = t4 * 4 + quad;
+          uint32_t r[4];
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                       : "r"(at + key * kRowBytes + ((chunk ^ Tile::swizzle(key)) * 16)) : "memory");
+#pragma unroll
+          for (int t = 0; t < 4; ++t) mma16<kBf16, kHalf>(sc[j], q[t4 * 4 + t], e4m3x2_to_f16x2(r[t]), e4m3x2_to_f16x2(r[t] >> 16));
+        }
+    }
+    // base-2 logits; what a row's value scale adds to the maximum
+    float top[kS];
+#pragma unroll
+    for (int s = 0; s < kS; ++s) top[s] = -INFINITY;
+    float vs[kF8 ? kNt : 1][2];
+#pragma unroll
+    for (int j = 0; j < kNt; ++j) {
+      float ks[2] = {1.f, 1.f}, lift[2] = {0.f, 0.f};
+      if constexpr (kF8) {
+        const uint32_t sa = at + 2 * kR * kRowBytes + (j * 8 + quad * 2) * 4;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[0]), "=f"(ks[1]) : "r"(sa) : "memory");
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(vs[j][0]), "=f"(vs[j][1]) : "r"(sa + kR * 4) : "memory");
+#pragma unroll
+        for (int i = 0; i < 2; ++i) lift[i] = __log2f(fmaxf(fabsf(vs[j][i]), 7.9e-31f));  // 2^-100: no lower, or the sum of the weights leaves fp32
+      }
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = sc[j][2 * s + i] * back_scale[s];
+          if (kF8) x *= ks[i];
+          sc[j][2 * s + i] = x;
+        }
+      if (live != 0xffffffffu) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (!((live >> (j * 8 + quad * 2 + i)) & 1)) {
+#pragma unroll
+            for (int s = 0; s < kS; ++s) sc[j][2 * s + i] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) top[s] = fmaxf(top[s], kF8 ? sc[j][2 * s + i] + lift[i] : sc[j][2 * s + i]);
+    }
+    if (a.scores) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+        if (oct + 8 * s < heads) {
+          float* out = a.scores + ((int64_t)b * a.H + h0 + oct + 8 * s) * a.c.capacity + r0 + quad * 2;
+#pragma unroll
+          for (int j = 0; j < kNt; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (r0 + j * 8 + quad * 2 + i < end) out[j * 8 + i] = sc[j][2 * s + i];
+        }
+    }
+    bool raise = false;
+#pragma unroll
+    for (int s = 0; s < kS; ++s) {
+      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
+      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
+      raise = raise || top[s] > m[s] + kSlack;
+    }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        const float to = fmaxf(m[s], top[s]);
+        const float keep = to == -INFINITY ? 0.f : sm100::ex2_approx(m[s] - to);
+        m[s] = to;
+        l[s] *= keep;
+#pragma unroll
+        for (int j = 0; j < kDt; ++j) o[j][2 * s] *= keep, o[j][2 * s + 1] *= keep;
+      }
+    }
+    float base[kS];
+#pragma unroll
+    for (int s = 0; s < kS; ++s) base[s] = m[s] == -INFINITY ? 0.f : m[s] - kOffset;
+    // weights and their products with V, 16 keys at a time
+#pragma unroll
+    for (int j = 0; j < kNt; j += 2) {
+      uint32_t p[kA];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int s = 0; s < kS; ++s) {
+          float x = sm100::ex2_approx(sc[j + u][2 * s] - base[s]), y = sm100::ex2_approx(sc[j + u][2 * s + 1] - base[s]);
+          l[s] += x + y;
+          if constexpr (kF8) x *= vs[j + u][0], y *= vs[j + u][1];
+          p[u * kS + s] = sm100::pack16x2<kBf16>(x, y);
+        }
+      const int key = j * 8 + (lane & 15);
+      if constexpr (!kF8) {
+#pragma unroll
+        for (int d = 0; d < kDt; d += 2) {
+          uint32_t r[4];
+          ldsm4_t(r, vat + key * kRowBytes + (((d + (lane >> 4)) ^ Tile::swizzle(key)) * 16));
+          mma16<kBf16, kHalf>(o[d], p, r[0], r[1]);
+          mma16<kBf16, kHalf>(o[d + 1], p, r[2], r[3]);
+        }
+      } else {
+        // a 16-bit column of the transposed load is a pair of neighbouring elements; they go to products of their own
+#pragma unroll
+        for (int d = 0; d < kDt; d += 4) {
+          uint32_t r[4];
+          ldsm4_t(r, vat + key * kRowBytes + (((d / 2 + (lane >> 4)) ^ Tile::swizzle(key)) * 16));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t lo0 = e4m3x2_to_f16x2(r[2 * c]), lo1 = e4m3x2_to_f16x2(r[2 * c] >> 16);
+            const uint32_t hi0 = e4m3x2_to_f16x2(r[2 * c + 1]), hi1 = e4m3x2_to_f16x2(r[2 * c + 1] >> 16);
+            mma16<kBf16, kHalf>(o[d + 2 * c], p, __byte_perm(lo0, lo1, 0x5410), __byte_perm(hi0, hi1, 0x5410));
+            mma16<kBf16, kHalf>(o[d + 2 * c + 1], p, __byte_perm(lo0, lo1, 0x7632), __byte_perm(hi0, hi1, 0x7632));
+          }
+        }
+      }
+    }
+    stage = stage == kStages - 1 ? 0 : stage + 1;
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // ---- the warps joined; element i of thread (oct, quad) of output tile j
+#pragma unroll
+  for (int s = 0; s < kS; ++s) {
+    l[s] += __shfl_xor_sync(0xffffffffu, l[s], 1);
+    l[s] += __shfl_xor_sync(0xffffffffu, l[s], 2);
+    if (quad == 0) m_s[warp][oct + 8 * s] = m[s], l_s[warp][oct + 8 * s] = l[s];
+  }
+  float* o_s = reinterpret_cast<float*>(smem) + warp * kHeads * kD;
+#pragma unroll
+  for (int j = 0; j < kDt; ++j)
+#pragma unroll
+    for (int s = 0; s < kS; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int col = quad * 2 + i;
+        const int d = kF8 ? j / 2 * 16 + col * 2 + (j & 1) : j * 8 + col;
+        o_s[(oct + 8 * s) * kD + d] = o[j][2 * s + i];
+      }
+  __syncthreads();
+  for (int i = threadIdx.x; i < heads * kD; i += kThreads) {
+    const int g = i / kD, d = i % kD;
+    float top = m_s[0][g];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][g]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float keep = exp2f(m_s[w][g] - base);
+      sum += l_s[w][g] * keep;
+      x += reinterpret_cast<const float*>(smem)[(w * kHeads + g) * kD + d] * keep;
+    }
+    const int64_t bh = (int64_t)b * a.H + h0 + g;
+    if (a.splits == 1) {
+      store_any(a.o, bh * kD + d, a.dtype, sum == 0.f ? 0.f : x / sum);
+      if (a.lse && d == 0) a.lse[bh] = sum == 0.f ? 0.f : base - kOffset + log2f(sum);
+    } else {
+      a.part_o[(bh * a.splits + split) * kD + d] = x;
+      if (d == 0) a.part_ml[bh * a.splits + split] = make_float2(top - kOffset, sum);
+    }
+  }
+}
+
+template <bool kF8, bool kBf16, int kD, bool kHalf>
+int launch_mma(AttendArgs& a, cudaStream_t s) {
+  using Tile = MmaTile<kF8, kBf16, kD, kHalf>;
+  static std::atomic<bool> done[kMaxDevices];
+  int dev = 0, n_sm = 0;
+  if (!device_sm_count(&dev, &n_sm)) return KB_ERR_LAUNCH;
+  KB_CUDA_TRY(opt_in_smem_once(paged_attend_mma_kernel<kF8, kBf16, kD, kHalf>, Tile::kSmem, dev, done));
+  a.head_tiles = kb_cdiv_i32(a.group, Tile::kHeads);
+  paged_attend_mma_kernel<kF8, kBf16, kD, kHalf><<<dim3(a.splits, a.H_kv * a.head_tiles, a.B), kThreads, Tile::kSmem, s>>>(a);
+  KB_LAUNCH_CHECK("paged_attend_mma_kernel");
+  return KB_OK;
+}
+template <bool kF8, bool kBf16>
+int launch_mma(AttendArgs& a, cudaStream_t s) {
+  if (a.D == 64) return a.group <= 8 ? launch_mma<kF8, kBf16, 64, true>(a, s) : launch_mma<kF8, kBf16, 64, false>(a, s);
+  return a.group <= 8 ? launch_mma<kF8, kBf16, 128, true>(a, s) : launch_mma<kF8, kBf16, 128, false>(a, s);
+}
+
+// Whether the tensor-core kernel takes the call: a 16-bit q of head dim 64 or 128; keys and values of one layout, with rows on 16-byte
+// boundaries, within 2^32 such units.
+bool takes_mma(const kb_paged_attention_params& p) {
+  const kb_paged_cache& c = p.cache;
+  const int e = dtype_size(c.dtype);
+  if (p.dtype == KB_F32 || (c.D != 64 && c.D != 128) || !paged_rows_aligned(c, e)) return false;
+  int64_t last = 0;
+  const int32_t extent[3] = {c.P, c.H_kv, c.page};
+  for (int i = 0; i < 3; ++i) {
+    if (c.k_stride[i] != c.v_stride[i] || c.k_stride[i] < 0 || c.k_stride[i] > (int64_t)1 << 40) return false;
+    if (c.dtype == KB_E4M3 && c.k_scale_stride[i] != c.v_scale_stride[i]) return false;
+    if (i != 1) last += c.k_stride[i] * kb_max_i32(extent[i] - 1, 0);
+    if (last > (int64_t)1 << 40) return false;
+  }
+  return last * e / 16 < 0xffffffff - 64;
+}
+
 // ---- the parts of a head joined ------------------------------------------------------------------------------------------
 
 __global__ void paged_join_kernel(const AttendArgs a) {
@@ -321,7 +727,8 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
   if (p.weights) a.scores = w;
   const bool aligned = paged_rows_aligned(c, dtype_size(c.dtype));
   int rc;
-  switch (c.dtype) {
+  if (takes_mma(p)) rc = c.dtype == KB_E4M3 ? launch_mma<true, false>(a, s) : c.dtype == KB_BF16 ? launch_mma<false, true>(a, s) : launch_mma<false, false>(a, s);
+  else switch (c.dtype) {
     case KB_F32: rc = launch_dim<float>(a, aligned, s); break;
     case KB_F16: rc = launch_dim<__half>(a, aligned, s); break;
     case KB_BF16: rc = launch_dim<__nv_bfloat16>(a, aligned, s); break;
