@@ -48,6 +48,16 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// x / scale rounded to nearest, with r = 1 / scale rounded to nearest: one Newton correction of x r by its exact
+// remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990: correctly
+// rounded where nothing underflows).  Here scale >= 1e-12 and quotients below 2^-11 become 0 whatever their last bit,
+// so the remainders that matter stay far above the smallest normal number; scale <= 1e37 keeps r normal.
+__device__ __forceinline__ float div_by(float x, float scale, float r) {
+  const float q = __fmul_rn(x, r);
+  const float d = __fmaf_rn(__fmaf_rn(-q, scale, x), r, q);
+  return __uint_as_float(__float_as_uint(d) | (__float_as_uint(x) & 0x80000000u));  // -0 keeps its sign
+}
+
 // Problem description shared by the kernel launchers (dense == single chunk, no look-back).
 struct AttnShape {
   int32_t B, H, T, D;

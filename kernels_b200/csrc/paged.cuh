@@ -56,6 +56,25 @@ inline bool paged_rows_aligned(const kb_paged_cache& c, int elsize) {
   return true;
 }
 
+// Launches of one call overlap: a kernel started with `launch_after` may start while the one before it in the stream still
+// runs, and waits for it, its writes included, where it calls `wait_for_launch_before` (before it reads or writes anything that
+// the other touches).
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Args>
+int launch_after(void (*kernel)(Args...), dim3 grid, int threads, cudaStream_t s, const Args&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid, c.blockDim = dim3(threads), c.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at, c.numAttrs = 1;
+  KB_CUDA_TRY(cudaLaunchKernelEx(&c, kernel, args...));
+  count_launch();
+  return KB_OK;
+}
+
 inline int dtype_size(int32_t dtype) { return dtype == KB_F32 ? 4 : dtype == KB_E4M3 ? 1 : 2; }
 
 }  // namespace kb

@@ -2,16 +2,16 @@
 // token sees, its log-sum-exp, and on request every row's weight added to a running sum.
 //
 // HBM-bound: two FLOPs per byte and query head; all that counts is to read every cached row once, at full rate.  The query
-// heads that share a key/value head are therefore worked on together, and the rows of a sequence are split over so
-// many blocks that the GPU is full even for one sequence.  A block keeps, per head, the running maximum, the sum and the
-// unnormalised output (all fp32), and a second kernel joins the blocks of a head in their order:
+// heads that share a key/value head are therefore worked on together (an item: a sequence and up to 16 query heads), and the rows
+// of all items, cut into tiles, form one line that is shared out evenly: every unit (a warp of the tensor-core
+// kernel, a block of the generic one) walks over a stretch of it, whatever the lengths are, and as many units are
+// launched as the GPU holds.  A unit keeps, per head, the running maximum, the sum and the unnormalised output (fp32).  An item that lies
+// within a unit's stretch is finished there.  Of the others each unit leaves a part (its first and its last item
+// at most), and a second kernel joins an item's parts in their order:
 //   m = max m_s,  l = sum l_s 2^(m_s - m),  o = sum o_s 2^(m_s - m) / l.
 // Rows' weights need the final m and l, so the scores go to the workspace (4 bytes per row and query head, against
 // 2 D elements per row and key/value head read) and a third kernel turns them into weights and adds them up: every sum has one
 // writer, so results do not depend on the order of anything.
-//
-// Generic kernel (this file): CUDA cores, every type, head dim and alignment.  A row is a few neighbouring lanes, 16 bytes
-// each; a group of lanes has a softmax of its own, joined at the end of the block.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -23,6 +23,7 @@ namespace kb {
 namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kMostHeads = 16;  // of an item
 
 struct AttendArgs {
   PagedView c;
@@ -33,12 +34,14 @@ struct AttendArgs {
   float* weights;
   int64_t w_b, w_h;
   int32_t dtype, B, H, H_kv, D, group;   // group: query heads per key/value head
-  int32_t head_tiles;                    // blocks per group
+  int32_t heads, head_tiles;             // query heads of an item, items per group
   int32_t context, back;                 // context 0: every row is seen
-  int32_t splits;
+  int32_t units, least_tiles;            // least_tiles: no unit gets fewer, as far as there are any
+  int32_t by_item;                       // no more items than units
   float scale_log2;
-  float* part_o;    // [B, H, splits, D]
-  float2* part_ml;  // [B, H, splits]
+  int4* join;       // [items] with by_item, otherwise by the unit that starts the item, [units]: {first part (-1: none), its unit, last unit, item}
+  float* part_o;    // [2 units, heads, D]
+  float2* part_ml;  // [2 units, heads]
   float* scores;    // [B, H, capacity], base-2 logits
   KbFastDiv fd_context;
 };
@@ -48,14 +51,6 @@ __device__ __forceinline__ void seen_rows(const AttendArgs& a, int32_t b, int32_
   end = a.c.rows(b);
   first = 0;
   if (a.context && end > 0) first = kb_max_i32(0, kb_fastdiv(end - 1, a.fd_context) - a.back) * a.context;
-}
-
-// Part `split` of them, in whole tiles.
-__device__ __forceinline__ void split_rows(const AttendArgs& a, int32_t split, int32_t tile, int32_t& first, int32_t& end) {
-  const int32_t tiles = kb_cdiv_i32(end - first, tile), each = kb_cdiv_i32(tiles, a.splits);
-  const int64_t from = (int64_t)first + (int64_t)split * each * tile, to = from + (int64_t)each * tile;
-  first = from < end ? (int32_t)from : end;
-  end = to < end ? (int32_t)to : end;
 }
 
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int32_t dtype) {
@@ -69,149 +64,260 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int32_t dtype, flo
   else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
 }
 
+// ---- the line of tiles -------------------------------------------------------------------------------------------------
+
+// Where a unit stands: tile `tile` of the `tiles` of item (b, hy), with `left` tiles of its stretch to go.  A sequence without rows has one
+// tile, without rows, so that its output is written.
+struct Place {
+  int32_t b, hy, tile, tiles, first, end;
+  int64_t left;
+
+  __device__ __forceinline__ void enter(const AttendArgs& a, int32_t rows) {
+    seen_rows(a, b, first, end);
+    tiles = kb_max_i32(1, (end - first + rows - 1) / rows);
+  }
+  // n tiles on, to the end of the item at most
+  __device__ __forceinline__ void advance(const AttendArgs& a, int32_t rows, int32_t n) {
+    tile += n, left -= n;
+    if (tile == tiles && left > 0) {
+      tile = 0;
+      if (++hy == a.H_kv * a.head_tiles) {
+        hy = 0, ++b;
+        enter(a, rows);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ int64_t warp_sum(int64_t x) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+  return x;
+}
+
+struct Stretch {
+  Place at;           // left 0: nothing to do
+  int64_t begin, each;  // the unit's first tile, and tiles per unit
+};
+
+// Found by a whole warp.  `rows`: of a tile.
+__device__ __forceinline__ Stretch find_stretch(const AttendArgs& a, int32_t unit, int32_t rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t per_seq = (int64_t)a.H_kv * a.head_tiles;
+  Place p{};
+  int64_t total = 0;
+  for (p.b = lane; p.b < a.B; p.b += 32) {
+    p.enter(a, rows);
+    total += p.tiles;
+  }
+  total = warp_sum(total) * per_seq;
+  Stretch s;
+  s.each = total < (int64_t)a.units * a.least_tiles ? a.least_tiles : (total + a.units - 1) / a.units;
+  s.begin = unit * s.each;
+  p.left = s.begin >= total ? 0 : min(s.each, total - s.begin);
+  if (p.left) {
+    int64_t before = 0;
+    for (int32_t b0 = 0; b0 < a.B; b0 += 32) {
+      p.b = b0 + lane;
+      if (p.b < a.B) p.enter(a, rows);
+      const int64_t mine = p.b < a.B ? p.tiles * per_seq : 0;
+      int64_t upto = mine;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += y;
+      }
+      const uint32_t found = __ballot_sync(0xffffffffu, s.begin < before + upto);
+      if (found) {
+        const int src = __ffs(found) - 1;
+        const int64_t off = s.begin - (before + __shfl_sync(0xffffffffu, upto - mine, src));
+        p.b = b0 + src;
+        p.enter(a, rows);
+        p.hy = (int32_t)(off / p.tiles);
+        p.tile = (int32_t)(off - (int64_t)p.hy * p.tiles);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  s.at = p;
+  return s;
+}
+
+// What becomes of the unit's part of an item: -1, it is the whole item, otherwise where the part goes.  `seen` tiles of the stretch lie before it.
+// The unit that starts an item leaves word of its parts (one lane calls with `tell`).
+__device__ __forceinline__ int32_t part_of_item(const AttendArgs& a, const Stretch& s, const Place& p, int32_t unit, int64_t seen, int32_t n, bool tell) {
+  const int32_t slot = 2 * unit + (seen ? 1 : 0);
+  const bool starts = p.tile == 0;
+  const int64_t item = (int64_t)p.b * a.H_kv * a.head_tiles + p.hy;
+  const bool whole = starts && n == p.tiles;
+  if (tell && starts) {
+    const int32_t last = whole ? unit : (int32_t)((s.begin + seen + p.tiles - 1) / s.each);
+    if (a.by_item) a.join[item] = make_int4(whole ? -1 : slot, unit, last, (int32_t)item);
+    else if (!whole) a.join[unit] = make_int4(slot, unit, last, (int32_t)item);
+  }
+  return whole ? -1 : slot;
+}
+
 // ---- generic kernel --------------------------------------------------------------------------------------------------
+//
+// CUDA cores, every type, head dim and alignment.  A row is a few neighbouring lanes of 16 bytes each; a group of such lanes has a softmax of
+// its own, joined with the others' at the end of an item, and kAhead rows in flight.
 
-template <typename T, int N>
+template <int kBytes>
 struct RowPart {
-  float f[N];
-  __device__ __forceinline__ void load(const T* p, bool aligned) {
-    if (aligned && N * sizeof(T) % 16 == 0) {
-      T e[N];
+  uint4 raw[kBytes / 16];
+  __device__ __forceinline__ void load(const char* p, bool aligned) {
+    if (aligned) {
 #pragma unroll
-      for (int i = 0; i < (int)(N * sizeof(T)) / 16; ++i) reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = to_f32(e[i]);
+      for (int i = 0; i < kBytes / 16; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = to_f32(p[i]);
+      for (int i = 0; i < kBytes / 4; ++i) {
+        const uint8_t* e = reinterpret_cast<const uint8_t*>(p) + 4 * i;
+        reinterpret_cast<uint32_t*>(raw)[i] = e[0] | e[1] << 8 | e[2] << 16 | (uint32_t)e[3] << 24;
+      }
     }
   }
-};
-template <int N>
-struct RowPart<uint8_t, N> {  // e4m3
-  float f[N];
-  __device__ __forceinline__ void load(const uint8_t* p, bool aligned) {
-    uint8_t e[N];
-    if (aligned && N % 16 == 0) {
-#pragma unroll
-      for (int i = 0; i < N / 16; ++i) reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  template <typename T>
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 1) {
+      return __half2float(__half(__nv_cvt_fp8_to_halfraw(reinterpret_cast<const uint8_t*>(raw)[i], __NV_E4M3)));
     } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      __half_raw r = __nv_cvt_fp8_to_halfraw(e[i], __NV_E4M3);
-      f[i] = __half2float(__half(r));
+      return to_f32(reinterpret_cast<const T*>(raw)[i]);
     }
   }
 };
 
-// T: the cache's elements (uint8_t: e4m3); G: query heads per block
+template <typename T, int D>
+struct GenericTile {
+  static constexpr int kBytes = D * (int)sizeof(T) > 512 ? 32 : 16;  // of a lane
+  static constexpr int kLanes = D * (int)sizeof(T) / kBytes;         // per row
+  static constexpr int N = D / kLanes;                               // elements per lane
+  static constexpr int kAhead = 4;
+  static constexpr int kGroups = 32 / kLanes;                        // rows of a warp at a time
+  static constexpr int kRows = kWarps * kGroups * kAhead;
+};
+
+// T: the cache's elements (uint8_t: e4m3); G: query heads per item
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs a, bool aligned) {
-  constexpr int kLanes = D * (int)sizeof(T) / 16 < 1 ? 1 : D * (int)sizeof(T) / 16 > 32 ? 32 : D * (int)sizeof(T) / 16;  // per row
-  constexpr int N = D / kLanes;                     // elements per lane
-  constexpr int kRows = 32 / kLanes;                // rows of a warp at a time
-  constexpr int kTile = kWarps * kRows;
+  using Tile = GenericTile<T, D>;
+  constexpr int kLanes = Tile::kLanes, N = Tile::N, kGroups = Tile::kGroups, kAhead = Tile::kAhead, kRows = Tile::kRows;
   __shared__ float q_s[G][D];
   __shared__ float m_s[kWarps][G], l_s[kWarps][G], o_s[kWarps][G][D];
-  const int32_t split = blockIdx.x, hk = blockIdx.y / a.head_tiles, b = blockIdx.z;
-  const int32_t h0 = hk * a.group + (blockIdx.y - hk * a.head_tiles) * G, heads = min(G, (hk + 1) * a.group - h0);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / kLanes, part = lane % kLanes;
-  int32_t first, end;
-  seen_rows(a, b, first, end);
-  split_rows(a, split, kTile, first, end);
+  const int32_t unit = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / kLanes, piece = lane % kLanes;
+  if (threadIdx.x == 0 && !a.by_item) a.join[unit].x = -1;
+  const Stretch stretch = find_stretch(a, unit, kRows);
+  Place at = stretch.at;
+  for (int64_t seen = 0; at.left > 0;) {
+    const int32_t n = (int32_t)min((int64_t)(at.tiles - at.tile), at.left);
+    const int32_t b = at.b, hk = at.hy / a.head_tiles, h0 = hk * a.group + (at.hy - hk * a.head_tiles) * G, heads = min(G, (hk + 1) * a.group - h0);
+    const int32_t slot = part_of_item(a, stretch, at, unit, seen, n, threadIdx.x == 0);
+    const int32_t begin = at.first + at.tile * kRows, end = kb_min_i32(at.end, begin + n * kRows);
+    at.advance(a, kRows, n);
+    seen += n;
 
-  for (int i = threadIdx.x; i < G * D; i += kThreads) {
-    const int g = i / D, d = i % D;
-    q_s[g][d] = g < heads ? load_any(a.q, b * a.q_b + (h0 + g) * a.q_h + d * a.q_d, a.dtype) * a.scale_log2 : 0.f;
-  }
-  __syncthreads();
-  float q[G][N], o[G][N], m[G], l[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    m[g] = -INFINITY, l[g] = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) q[g][i] = q_s[g][part * N + i], o[g][i] = 0.f;
-  }
-  for (int32_t r0 = first; r0 < end; r0 += kTile) {
-    const int32_t r = r0 + warp * kRows + sub;
-    int32_t at = 0, page = -1;
-    if (r < end) page = a.c.locate(b, r, at);
-    const bool live = page >= 0;
-    RowPart<T, N> k, v;
-    float ks = 1.f, vs = 1.f;
-    if (live) {
-      k.load(reinterpret_cast<const T*>(a.c.k) + page * a.c.k_page + hk * a.c.k_head + at * a.c.k_row + part * N, aligned);
-      v.load(reinterpret_cast<const T*>(a.c.v) + page * a.c.v_page + hk * a.c.v_head + at * a.c.v_row + part * N, aligned);
-      if (sizeof(T) == 1) {
-        ks = a.c.k_scale[page * a.c.ks_page + hk * a.c.ks_head + at * a.c.ks_row];
-        vs = a.c.v_scale[page * a.c.vs_page + hk * a.c.vs_head + at * a.c.vs_row];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) k.f[i] = 0.f, v.f[i] = 0.f;
+    for (int i = threadIdx.x; i < G * D; i += kThreads) {
+      const int g = i / D, d = i % D;
+      q_s[g][d] = g < heads ? load_any(a.q, b * a.q_b + (h0 + g) * a.q_h + d * a.q_d, a.dtype) * a.scale_log2 : 0.f;
     }
+    __syncthreads();
+    float q[G][N], o[G][N], m[G], l[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float s = 0.f;
+      m[g] = -INFINITY, l[g] = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s = fmaf(q[g][i], k.f[i], s);
-#pragma unroll
-      for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s = live ? s * ks : -INFINITY;
-      if (a.scores && part == 0 && r < end && g < heads) a.scores[((int64_t)b * a.H + h0 + g) * a.c.capacity + r] = s;
-      const float top = fmaxf(m[g], s), base = top == -INFINITY ? 0.f : top;
-      const float p = live ? exp2f(s - base) : 0.f, keep = exp2f(m[g] - base);
-      m[g] = top;
-      l[g] = l[g] * keep + p;
-      const float pv = p * vs;
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[g][i] = fmaf(pv, v.f[i], o[g][i] * keep);
+      for (int i = 0; i < N; ++i) q[g][i] = q_s[g][piece * N + i], o[g][i] = 0.f;
     }
-  }
-  // the lane groups of a warp, then the warps
+    for (int32_t r0 = begin + warp * kGroups * kAhead + sub; r0 - sub < end; r0 += kRows) {
+      RowPart<Tile::kBytes> k[kAhead], v[kAhead];
+      float ks[kAhead], vs[kAhead];
+      int32_t page[kAhead], row[kAhead];
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    float top = m[g];
+      for (int j = 0; j < kAhead; ++j) {
+        page[j] = -1;
+        if (r0 + j * kGroups < end) page[j] = a.c.locate(b, r0 + j * kGroups, row[j]);
+      }
 #pragma unroll
-    for (int x = kLanes; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float keep = exp2f(m[g] - (top == -INFINITY ? 0.f : top));
-    float sum = l[g] * keep;
+      for (int j = 0; j < kAhead; ++j) {
+        ks[j] = vs[j] = 1.f;
+        if (page[j] < 0) continue;
+        k[j].load(a.c.k + (page[j] * a.c.k_page + hk * a.c.k_head + row[j] * a.c.k_row + piece * N) * (int64_t)sizeof(T), aligned);
+        v[j].load(a.c.v + (page[j] * a.c.v_page + hk * a.c.v_head + row[j] * a.c.v_row + piece * N) * (int64_t)sizeof(T), aligned);
+        if (sizeof(T) == 1) {
+          ks[j] = a.c.k_scale[page[j] * a.c.ks_page + hk * a.c.ks_head + row[j] * a.c.ks_row];
+          vs[j] = a.c.v_scale[page[j] * a.c.vs_page + hk * a.c.vs_head + row[j] * a.c.vs_row];
+        }
+      }
 #pragma unroll
-    for (int x = kLanes; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (lane == 0) m_s[warp][g] = top, l_s[warp][g] = sum;
+      for (int j = 0; j < kAhead; ++j) {
+        const bool live = page[j] >= 0;
+        const int32_t r = r0 + j * kGroups;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float x = o[g][i] * keep;
+        for (int g = 0; g < G; ++g) {
+          float s = 0.f;
 #pragma unroll
-      for (int y = kLanes; y < 32; y <<= 1) x += __shfl_xor_sync(0xffffffffu, x, y);
-      if (sub == 0) o_s[warp][g][part * N + i] = x;
+          for (int i = 0; i < N; ++i) s = fmaf(q[g][i], live ? k[j].template get<T>(i) : 0.f, s);
+#pragma unroll
+          for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+          s = live ? s * ks[j] : -INFINITY;
+          if (a.scores && piece == 0 && r < end && g < heads) a.scores[((int64_t)b * a.H + h0 + g) * a.c.capacity + r] = s;
+          if (!live) continue;
+          const float top = fmaxf(m[g], s), base = top == -INFINITY ? 0.f : top;
+          const float p = exp2f(s - base), keep = exp2f(m[g] - base);
+          m[g] = top;
+          l[g] = l[g] * keep + p;
+          const float pv = p * vs[j];
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[g][i] = fmaf(pv, v[j].template get<T>(i), o[g][i] * keep);
+        }
+      }
     }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * D; i += kThreads) {
-    const int g = i / D, d = i % D;
-    float top = m_s[0][g];
+    // the lane groups of a warp, then the warps
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][g]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x = 0.f;
+    for (int g = 0; g < G; ++g) {
+      float top = m[g];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float keep = exp2f(m_s[w][g] - base);
-      sum += l_s[w][g] * keep;
-      x += o_s[w][g][d] * keep;
+      for (int x = kLanes; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float keep = exp2f(m[g] - (top == -INFINITY ? 0.f : top));
+      float sum = l[g] * keep;
+#pragma unroll
+      for (int x = kLanes; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (lane == 0) m_s[warp][g] = top, l_s[warp][g] = sum;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float x = o[g][i] * keep;
+#pragma unroll
+        for (int y = kLanes; y < 32; y <<= 1) x += __shfl_xor_sync(0xffffffffu, x, y);
+        if (sub == 0) o_s[warp][g][piece * N + i] = x;
+      }
     }
-    const int64_t bh = (int64_t)b * a.H + h0 + g;
-    if (a.splits == 1) {
-      store_any(a.o, bh * D + d, a.dtype, sum == 0.f ? 0.f : x / sum);
-      if (a.lse && d == 0) a.lse[bh] = sum == 0.f ? 0.f : base + log2f(sum);
-    } else {
-      a.part_o[(bh * a.splits + split) * D + d] = x;
-      if (d == 0) a.part_ml[bh * a.splits + split] = make_float2(top, sum);
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * D; i += kThreads) {
+      const int g = i / D, d = i % D;
+      float top = m_s[0][g];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][g]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float keep = exp2f(m_s[w][g] - base);
+        sum += l_s[w][g] * keep;
+        x += o_s[w][g][d] * keep;
+      }
+      const int64_t bh = (int64_t)b * a.H + h0 + g;
+      if (slot < 0) {
+        store_any(a.o, bh * D + d, a.dtype, sum == 0.f ? 0.f : x / sum);
+        if (a.lse && d == 0) a.lse[bh] = sum == 0.f ? 0.f : base + log2f(sum);
+      } else {
+        a.part_o[((int64_t)slot * G + g) * D + d] = x;
+        if (d == 0) a.part_ml[(int64_t)slot * G + g] = make_float2(top, sum);
+      }
     }
+    __syncthreads();  // (q_s and o_s are the next item's)
   }
 }
 
@@ -220,8 +326,8 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
 // 16-bit and e4m3 caches of head dim 64 and 128.  A warp multiplies the 16 (or 8) query heads of a block with 16 keys at a time
 // (m16n8k16): the heads are the rows, so up to 16 heads cost what one does, and what the tensor cores have to do is a
 // small part of the time that the keys take to arrive.  That time is all there is to hide, and every warp hides it for itself: it
-// has tiles of kR rows of its own (every fourth of the block's), a ring of kStages of them in shared memory filled by
-// 16-byte asynchronous copies, and a softmax of its own, so that no warp waits for another before the end.
+// is a unit with a ring of kStages tiles of kR rows in shared memory, filled by 16-byte asynchronous copies that run on from one item
+// into the next, and it never waits for another warp.
 //
 // Rows are found one by one (a lane looks up a row), so pages of any size and order are read the same way; a row that is
 // masked is filled with zeros without being read, so that nothing in it can reach a sum.
@@ -268,78 +374,82 @@ __device__ __forceinline__ void mma16(float (&c)[HALF ? 2 : 4], const uint32_t (
           : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(r) : "r"(two));
-  return r;
+// four e4m3 to two pairs of f16
+__device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 
-// kF8: e4m3 cache (products in f16); kBf16: products in bf16, otherwise in f16; kHalf: at most eight query heads per block
+// kF8: e4m3 cache (products in f16); kBf16: products in bf16, otherwise in f16; kHalf: at most eight query heads per item
 template <bool kF8, bool kBf16, int kD, bool kHalf>
 struct MmaTile {
   static constexpr int kRowBytes = kF8 ? kD : 2 * kD, kChunks = kRowBytes / 16;
-  static constexpr int kR = kRowBytes == 256 ? 16 : 32;            // rows of a tile
-  static constexpr int kStages = kRowBytes == 64 ? 4 : 3;
+  static constexpr int kR = kRowBytes == 256 ? 16 : 32;        // rows of a tile
+  static constexpr int kStages = kRowBytes == 256 ? 2 : kRowBytes == 64 ? 4 : 3;
   static constexpr int kScaleBytes = kF8 ? 2 * kR * 4 : 0;
   static constexpr int kStageBytes = 2 * kR * kRowBytes + kScaleBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
-  static constexpr int kHeads = kHalf ? 8 : 16, kS = kHalf ? 1 : 2; // kS: heads per thread
+  static constexpr int kHeads = kHalf ? 8 : 16, kS = kHalf ? 1 : 2;  // kS: heads per thread
   static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kBlocks = kRowBytes == 256 && kHalf ? 3 : 2;      // per SM
+  static_assert(kStageBytes % 128 == 0, "matrix loads address a tile by exclusive or");
   // Where chunk c of row r lies: at c ^ swizzle(r).  The eight rows of a matrix load hit different banks, and so do the two rows
   // and four chunks of a 16-byte load of e4m3 keys.
   static __device__ __forceinline__ int swizzle(int r) { return !kF8 ? r & 7 : kD == 128 ? ((r & 1) << 2) | ((r >> 1) & 3) : (r >> 1) & 3; }
-  static_assert(kSmem >= kWarps * kHeads * kD * 4, "the warps' outputs are joined where the ring was");
 };
 
 template <bool kF8, bool kBf16, int kD, bool kHalf>
-__global__ void __launch_bounds__(kThreads) paged_attend_mma_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlocks) paged_attend_mma_kernel(const AttendArgs a) {
   using Tile = MmaTile<kF8, kBf16, kD, kHalf>;
   constexpr int kR = Tile::kR, kStages = Tile::kStages, kChunks = Tile::kChunks, kRowBytes = Tile::kRowBytes, kHeads = Tile::kHeads, kS = Tile::kS;
   constexpr int kSteps = kD / 16, kNt = kR / 8, kDt = kD / 8, kA = 2 * kS;
   constexpr float kOffset = kBf16 ? 0.f : 7.f, kSlack = 8.f;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float m_s[kWarps][16], l_s[kWarps][16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, oct = lane >> 2;
-  const int32_t split = blockIdx.x, hk = blockIdx.y / a.head_tiles, b = blockIdx.z;
-  const int32_t h0 = hk * a.group + (blockIdx.y - hk * a.head_tiles) * kHeads, heads = min(kHeads, (hk + 1) * a.group - h0);
-  int32_t first, end;
-  seen_rows(a, b, first, end);
-  split_rows(a, split, kWarps * kR, first, end);
+  const int32_t unit = blockIdx.x * kWarps + warp;
+  if (lane == 0 && unit < a.units && !a.by_item) a.join[unit].x = -1;
+  const Stretch stretch = find_stretch(a, unit, kR);
   const uint32_t ring = sm100::smem_u32(smem) + warp * Tile::kWarpBytes;
 
-  // ---- copies: lane r looks up row r of the tile
-  const char* kbase = a.c.k + hk * a.c.k_head * (kF8 ? 1 : 2);
-  const char* vbase = a.c.v + hk * a.c.v_head * (kF8 ? 1 : 2);
-  constexpr uint32_t kNoRow = 0xffffffffu;
-  int32_t next_row = first + warp * kR + (lane & (kR - 1));  // the row that this lane looks up next
-  uint32_t live_bits[kStages - 1];                           // of the tiles in the ring, oldest first
+  // ---- copies: lane r looks up row r of a tile, a tile ahead of its copy
+  constexpr int kElem = kF8 ? 1 : 2, kRowsAtOnce = 32 / kChunks;
+  const int chunk = lane % kChunks, sub = lane / kChunks;
+  const char *kfrom = a.c.k + chunk * 16, *vfrom = a.c.v + chunk * 16;
+  const uint32_t place = sub * kRowBytes + ((chunk ^ Tile::swizzle(sub)) * 16);
+  Place ahead = stretch.at;
+  int32_t next_at = 0, next_page = -1, next_head = 0;
+  auto look_up = [&]() {
+    next_page = -1;
+    if (ahead.left == 0) return;
+    const int32_t row = ahead.first + ahead.tile * kR + (lane & (kR - 1));
+    if (row < ahead.end) next_page = a.c.locate(ahead.b, row, next_at);
+    next_head = a.head_tiles == 1 ? ahead.hy : ahead.hy / a.head_tiles;
+    ahead.advance(a, kR, 1);
+  };
+  uint32_t live_bits[kStages - 1];  // of the tiles in the ring, oldest first
   auto issue = [&](int stage) -> uint32_t {
-    uint32_t at16 = kNoRow;
-    int32_t at = 0, page = -1;
-    if (next_row < end) page = a.c.locate(b, next_row, at);
-    if (page >= 0) at16 = (uint32_t)((uint64_t)((page * a.c.k_page + at * a.c.k_row) * (kF8 ? 1 : 2)) >> 4);
+    const int32_t page = next_page, at = next_at, head = next_head;
+    const uint32_t row16 = page >= 0 ? (uint32_t)((uint64_t)((page * a.c.k_page + head * a.c.k_head + at * a.c.k_row) * kElem) >> 4) : 0;
     const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
     const uint32_t to = ring + stage * Tile::kStageBytes;
-    constexpr int kRowsAtOnce = 32 / kChunks;
-    const int chunk = lane % kChunks, sub = lane / kChunks;
 #pragma unroll
     for (int i = 0; i < kR / kRowsAtOnce; ++i) {
-      const int r = i * kRowsAtOnce + sub;
-      const uint32_t row16 = __shfl_sync(0xffffffffu, at16, r);
-      const bool ok = row16 != kNoRow;
-      const uint64_t off = ok ? ((uint64_t)row16 + chunk) * 16 : 0;
-      const uint32_t place = r * kRowBytes + ((chunk ^ Tile::swizzle(r)) * 16);
-      cp_async16(to + place, kbase + off, ok);
-      cp_async16(to + kR * kRowBytes + place, vbase + off, ok);
+      const uint64_t off = (uint64_t)__shfl_sync(0xffffffffu, row16, i * kRowsAtOnce + sub) * 16;
+      const bool ok = (live >> (i * kRowsAtOnce + sub)) & 1;
+      const uint32_t there = to + i * kRowsAtOnce * kRowBytes + (place ^ (Tile::swizzle(i * kRowsAtOnce) * 16));
+      cp_async16(there, kfrom + off, ok);
+      cp_async16(there + kR * kRowBytes, vfrom + off, ok);
     }
     if constexpr (kF8) {
-      const int64_t so = page >= 0 ? page * a.c.ks_page + hk * a.c.ks_head + at * a.c.ks_row : 0;
-      cp_async4(to + 2 * kR * kRowBytes + lane * 4, a.c.k_scale + so, page >= 0);
-      cp_async4(to + 2 * kR * kRowBytes + kR * 4 + lane * 4, a.c.v_scale + so, page >= 0);
+      const int64_t so = page >= 0 ? page * a.c.ks_page + head * a.c.ks_head + at * a.c.ks_row : 0;
+      if (lane < kR) {
+        cp_async4(to + 2 * kR * kRowBytes + lane * 4, a.c.k_scale + so, page >= 0);
+        cp_async4(to + 2 * kR * kRowBytes + kR * 4 + lane * 4, a.c.v_scale + so, page >= 0);
+      }
     }
-    next_row += kWarps * kR;
+    look_up();
     return live;
   };
+  look_up();
   // (tiles behind the last are empty: nothing is read)
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
@@ -347,302 +457,315 @@ __global__ void __launch_bounds__(kThreads) paged_attend_mma_kernel(const Attend
     cp_async_commit();
   }
 
-  // ---- q as the products' left operand; with an e4m3 cache a lane's elements are the ones its 16-byte key loads hold
-  uint32_t q[kSteps][kA];
-  float back_scale[kS];
-#pragma unroll
-  for (int s = 0; s < kS; ++s) {
-    const int g = oct + 8 * s;
-    const bool there = g < heads;
-    const int64_t base = b * a.q_b + (int64_t)(h0 + (there ? g : 0)) * a.q_h;
-    float up = 1.f;
-    back_scale[s] = a.scale_log2;
-    if (kF8 && a.dtype == KB_BF16) {
-      float top = 0.f;
-      for (int d = quad; d < kD; d += 4) top = fmaxf(top, there ? fabsf(load_any(a.q, base + d * a.q_d, a.dtype)) : 0.f);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = (int)(__float_as_uint(top) >> 23) - 127;  // top in [2^e, 2^(e+1))
-      if (top > 0.f && e < 128) {
-        const int by = max(-100, min(100, 14 - e));
-        up = __uint_as_float((uint32_t)(by + 127) << 23);
-        back_scale[s] *= __uint_as_float((uint32_t)(127 - by) << 23);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < kSteps; ++t)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int d = kF8 ? t / 4 * 64 + quad * 16 + t % 4 * 4 + 2 * p : t * 16 + 8 * p + quad * 2;
-        const float x = there ? load_any(a.q, base + d * a.q_d, a.dtype) * up : 0.f;
-        const float y = there ? load_any(a.q, base + (d + 1) * a.q_d, a.dtype) * up : 0.f;
-        q[t][p * kS + s] = sm100::pack16x2<kBf16>(x, y);
-      }
-  }
-
-  float o[kDt][kA], m[kS], l[kS];
-#pragma unroll
-  for (int s = 0; s < kS; ++s) m[s] = -INFINITY, l[s] = 0.f;
-#pragma unroll
-  for (int j = 0; j < kDt; ++j)
-#pragma unroll
-    for (int i = 0; i < kA; ++i) o[j][i] = 0.f;
-
+  // where this lane's matrix loads start in a tile; chunks and keys further on are an exclusive or and an offset away
+  const int kkey = kF8 ? oct : (lane & 7) + (lane >> 4) * 8, vkey = lane & 15;
+  const uint32_t kplace = kkey * kRowBytes + (((kF8 ? quad : (lane >> 3) & 1) ^ Tile::swizzle(kkey)) * 16);
+  const uint32_t vplace = (kR + vkey) * kRowBytes + (((lane >> 4) ^ Tile::swizzle(vkey)) * 16);
   int stage = 0;
-  for (int32_t r0 = first + warp * kR; r0 < end; r0 += kWarps * kR) {
-    cp_async_wait<kStages - 2>();
-    __syncwarp();
-    const uint32_t at = ring + stage * Tile::kStageBytes, vat = at + kR * kRowBytes;
-    const uint32_t live = live_bits[0];
-    // every lane is through with the tile before this one: the next copies take its place
-#pragma unroll
-    for (int s = 0; s < kStages - 2; ++s) live_bits[s] = live_bits[s + 1];
-    live_bits[kStages - 2] = issue(stage == 0 ? kStages - 1 : stage - 1);
-    cp_async_commit();
+  Place now = stretch.at;
+  for (int64_t seen = 0; now.left > 0;) {
+    const int32_t n = (int32_t)min((int64_t)(now.tiles - now.tile), now.left);
+    const int32_t b = now.b, hk = now.hy / a.head_tiles, h0 = hk * a.group + (now.hy - hk * a.head_tiles) * kHeads, heads = min(kHeads, (hk + 1) * a.group - h0);
+    const int32_t slot = part_of_item(a, stretch, now, unit, seen, n, lane == 0);
+    int32_t r0 = now.first + now.tile * kR;
+    const int32_t end = now.end;
+    now.advance(a, kR, n);
+    seen += n;
 
-    // scores
-    float sc[kNt][kA];
+    // ---- q as the products' left operand; with an e4m3 cache a lane's elements are the ones its 16-byte key loads hold
+    uint32_t q[kSteps][kA];
+    float back_scale[kS];
 #pragma unroll
-    for (int j = 0; j < kNt; ++j)
-#pragma unroll
-      for (int i = 0; i < kA; ++i) sc[j][i] = 0.f;
-    if constexpr (!kF8) {
+    for (int s = 0; s < kS; ++s) {
+      const int g = oct + 8 * s;
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) + b * a.q_b + (int64_t)(h0 + (g < heads ? g : 0)) * a.q_h;
+      back_scale[s] = a.scale_log2;
 #pragma unroll
       for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-        for (int j = 0; j < kNt; j += 2) {
-          const int key = j * 8 + (lane & 7) + (lane >> 4) * 8, chunk = t * 2 + ((lane >> 3) & 1);
-          uint32_t r[4];
-          ldsm4(r, at + key * kRowBytes + ((chunk ^ Tile::swizzle(key)) * 16));
-          mma16<kBf16, kHalf>(sc[j], q[t], r[0], r[1]);
-          mma16<kBf16, kHalf>(sc[j + 1], q[t], r[2], r[3]);
+        for (int p = 0; p < 2; ++p) {
+          const int d = kF8 ? t / 4 * 64 + quad * 16 + t % 4 * 4 + 2 * p : t * 16 + 8 * p + quad * 2;
+          q[t][p * kS + s] = g < heads ? __ldg(reinterpret_cast<const uint32_t*>(from + d)) : 0u;
         }
-    } else {
+      if (kF8 && a.dtype == KB_BF16) {
+        // (bf16 magnitudes without their signs order like whole numbers; what is not a number stays above)
+        uint32_t most = 0;
 #pragma unroll
-      for (int t4 = 0; t4 < kSteps / 4; ++t4)
+        for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-        for (int j = 0; j < kNt; ++j) {
-          const int key = j * 8 + oct, chunk = t4 * 4 + quad;
-          uint32_t r[4];
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                       : "r"(at + key * kRowBytes + ((chunk ^ Tile::swizzle(key)) * 16)) : "memory");
+          for (int p = 0; p < 2; ++p) most = __vmaxu2(most, q[t][p * kS + s] & 0x7fff7fffu);
+        most = max(most & 0xffffu, most >> 16);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = (int)(most >> 7) - 127;  // the largest lies in [2^e, 2^(e + 1))
+        const int by = most == 0 || e == 128 ? 0 : max(-100, min(100, 14 - e));
+        const float up = __uint_as_float((uint32_t)(by + 127) << 23);
+        back_scale[s] *= __uint_as_float((uint32_t)(127 - by) << 23);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) mma16<kBf16, kHalf>(sc[j], q[t4 * 4 + t], e4m3x2_to_f16x2(r[t]), e4m3x2_to_f16x2(r[t] >> 16));
-        }
-    }
-    // base-2 logits; what a row's value scale adds to the maximum
-    float top[kS];
+        for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-    for (int s = 0; s < kS; ++s) top[s] = -INFINITY;
-    float vs[kF8 ? kNt : 1][2];
-#pragma unroll
-    for (int j = 0; j < kNt; ++j) {
-      float ks[2] = {1.f, 1.f}, lift[2] = {0.f, 0.f};
-      if constexpr (kF8) {
-        const uint32_t sa = at + 2 * kR * kRowBytes + (j * 8 + quad * 2) * 4;
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[0]), "=f"(ks[1]) : "r"(sa) : "memory");
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(vs[j][0]), "=f"(vs[j][1]) : "r"(sa + kR * 4) : "memory");
-#pragma unroll
-        for (int i = 0; i < 2; ++i) lift[i] = __log2f(fmaxf(fabsf(vs[j][i]), 7.9e-31f));  // 2^-100: no lower, or the sum of the weights leaves fp32
-      }
-#pragma unroll
-      for (int s = 0; s < kS; ++s)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float x = sc[j][2 * s + i] * back_scale[s];
-          if (kF8) x *= ks[i];
-          sc[j][2 * s + i] = x;
-        }
-      if (live != 0xffffffffu) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (!((live >> (j * 8 + quad * 2 + i)) & 1)) {
-#pragma unroll
-            for (int s = 0; s < kS; ++s) sc[j][2 * s + i] = -INFINITY;
+          for (int p = 0; p < 2; ++p) {
+            const uint32_t w = q[t][p * kS + s];
+            q[t][p * kS + s] = sm100::pack_f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
           }
       }
-#pragma unroll
-      for (int s = 0; s < kS; ++s)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) top[s] = fmaxf(top[s], kF8 ? sc[j][2 * s + i] + lift[i] : sc[j][2 * s + i]);
     }
-    if (a.scores) {
+
+    float o[kDt][kA], m[kS], l[kS];
 #pragma unroll
-      for (int s = 0; s < kS; ++s)
-        if (oct + 8 * s < heads) {
-          float* out = a.scores + ((int64_t)b * a.H + h0 + oct + 8 * s) * a.c.capacity + r0 + quad * 2;
+    for (int s = 0; s < kS; ++s) m[s] = -INFINITY, l[s] = 0.f;
 #pragma unroll
-          for (int j = 0; j < kNt; ++j)
+    for (int j = 0; j < kDt; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (r0 + j * 8 + quad * 2 + i < end) out[j * 8 + i] = sc[j][2 * s + i];
-        }
-    }
-    bool raise = false;
+      for (int i = 0; i < kA; ++i) o[j][i] = 0.f;
+
+    for (int32_t i_tile = 0; i_tile < n; ++i_tile, r0 += kR) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      const uint32_t at = ring + stage * Tile::kStageBytes, kat = at + kplace, vat = at + vplace;
+      const uint32_t live = live_bits[0];
+      // every lane is through with the tile before this one: the next copies take its place
 #pragma unroll
-    for (int s = 0; s < kS; ++s) {
-      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
-      top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
-      raise = raise || top[s] > m[s] + kSlack;
-    }
-    if (__any_sync(0xffffffffu, raise)) {
+      for (int s = 0; s < kStages - 2; ++s) live_bits[s] = live_bits[s + 1];
+      live_bits[kStages - 2] = issue(stage == 0 ? kStages - 1 : stage - 1);
+      cp_async_commit();
+
+      // scores
+      float sc[kNt][kA];
 #pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        const float to = fmaxf(m[s], top[s]);
-        const float keep = to == -INFINITY ? 0.f : sm100::ex2_approx(m[s] - to);
-        m[s] = to;
-        l[s] *= keep;
+      for (int j = 0; j < kNt; ++j)
 #pragma unroll
-        for (int j = 0; j < kDt; ++j) o[j][2 * s] *= keep, o[j][2 * s + 1] *= keep;
-      }
-    }
-    float base[kS];
-#pragma unroll
-    for (int s = 0; s < kS; ++s) base[s] = m[s] == -INFINITY ? 0.f : m[s] - kOffset;
-    // weights and their products with V, 16 keys at a time
-#pragma unroll
-    for (int j = 0; j < kNt; j += 2) {
-      uint32_t p[kA];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int s = 0; s < kS; ++s) {
-          float x = sm100::ex2_approx(sc[j + u][2 * s] - base[s]), y = sm100::ex2_approx(sc[j + u][2 * s + 1] - base[s]);
-          l[s] += x + y;
-          if constexpr (kF8) x *= vs[j + u][0], y *= vs[j + u][1];
-          p[u * kS + s] = sm100::pack16x2<kBf16>(x, y);
-        }
-      const int key = j * 8 + (lane & 15);
+        for (int i = 0; i < kA; ++i) sc[j][i] = 0.f;
       if constexpr (!kF8) {
 #pragma unroll
-        for (int d = 0; d < kDt; d += 2) {
-          uint32_t r[4];
-          ldsm4_t(r, vat + key * kRowBytes + (((d + (lane >> 4)) ^ Tile::swizzle(key)) * 16));
-          mma16<kBf16, kHalf>(o[d], p, r[0], r[1]);
-          mma16<kBf16, kHalf>(o[d + 1], p, r[2], r[3]);
-        }
+        for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+          for (int j = 0; j < kNt; j += 2) {
+            uint32_t r[4];
+            ldsm4(r, (kat ^ (t * 32)) + j * 8 * kRowBytes);
+            mma16<kBf16, kHalf>(sc[j], q[t], r[0], r[1]);
+            mma16<kBf16, kHalf>(sc[j + 1], q[t], r[2], r[3]);
+          }
       } else {
-        // a 16-bit column of the transposed load is a pair of neighbouring elements; they go to products of their own
 #pragma unroll
-        for (int d = 0; d < kDt; d += 4) {
-          uint32_t r[4];
-          ldsm4_t(r, vat + key * kRowBytes + (((d / 2 + (lane >> 4)) ^ Tile::swizzle(key)) * 16));
+        for (int t4 = 0; t4 < kSteps / 4; ++t4)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t lo0 = e4m3x2_to_f16x2(r[2 * c]), lo1 = e4m3x2_to_f16x2(r[2 * c] >> 16);
-            const uint32_t hi0 = e4m3x2_to_f16x2(r[2 * c + 1]), hi1 = e4m3x2_to_f16x2(r[2 * c + 1] >> 16);
-            mma16<kBf16, kHalf>(o[d + 2 * c], p, __byte_perm(lo0, lo1, 0x5410), __byte_perm(hi0, hi1, 0x5410));
-            mma16<kBf16, kHalf>(o[d + 2 * c + 1], p, __byte_perm(lo0, lo1, 0x7632), __byte_perm(hi0, hi1, 0x7632));
+          for (int j = 0; j < kNt; ++j) {
+            uint32_t r[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                         : "r"((kat ^ (t4 * 64)) + j * 8 * kRowBytes) : "memory");
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              uint32_t b0, b1;
+              e4m3x4_to_f16x2(r[t], b0, b1);
+              mma16<kBf16, kHalf>(sc[j], q[t4 * 4 + t], b0, b1);
+            }
+          }
+      }
+      // base-2 logits; what a row's value scale adds to the maximum
+      float top[kS];
+#pragma unroll
+      for (int s = 0; s < kS; ++s) top[s] = -INFINITY;
+      float vs[kF8 ? kNt : 1][2];
+#pragma unroll
+      for (int j = 0; j < kNt; ++j) {
+        float ks[2] = {1.f, 1.f}, lift[2] = {0.f, 0.f};
+        if constexpr (kF8) {
+          const uint32_t sa = at + 2 * kR * kRowBytes + (j * 8 + quad * 2) * 4;
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[0]), "=f"(ks[1]) : "r"(sa) : "memory");
+          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(vs[j][0]), "=f"(vs[j][1]) : "r"(sa + kR * 4) : "memory");
+#pragma unroll
+          for (int i = 0; i < 2; ++i) lift[i] = __log2f(fmaxf(fabsf(vs[j][i]), 7.9e-31f));  // 2^-100: no lower, or the sum of the weights leaves fp32
+        }
+#pragma unroll
+        for (int s = 0; s < kS; ++s)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x = sc[j][2 * s + i] * back_scale[s];
+            if (kF8) x *= ks[i];
+            sc[j][2 * s + i] = x;
+          }
+        if (live != 0xffffffffu) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (!((live >> (j * 8 + quad * 2 + i)) & 1)) {
+#pragma unroll
+              for (int s = 0; s < kS; ++s) sc[j][2 * s + i] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kS; ++s)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) top[s] = fmaxf(top[s], kF8 ? sc[j][2 * s + i] + lift[i] : sc[j][2 * s + i]);
+      }
+      if (a.scores) {
+#pragma unroll
+        for (int s = 0; s < kS; ++s)
+          if (oct + 8 * s < heads) {
+            float* out = a.scores + ((int64_t)b * a.H + h0 + oct + 8 * s) * a.c.capacity + r0 + quad * 2;
+#pragma unroll
+            for (int j = 0; j < kNt; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (r0 + j * 8 + quad * 2 + i < end) out[j * 8 + i] = sc[j][2 * s + i];
+          }
+      }
+      bool raise = false;
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
+        top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
+        raise = raise || top[s] > m[s] + kSlack;
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int s = 0; s < kS; ++s) {
+          const float to = fmaxf(m[s], top[s]);
+          const float keep = to == -INFINITY ? 0.f : sm100::ex2_approx(m[s] - to);
+          m[s] = to;
+          l[s] *= keep;
+#pragma unroll
+          for (int j = 0; j < kDt; ++j) o[j][2 * s] *= keep, o[j][2 * s + 1] *= keep;
+        }
+      }
+      float base[kS];
+#pragma unroll
+      for (int s = 0; s < kS; ++s) base[s] = m[s] == -INFINITY ? 0.f : m[s] - kOffset;
+      // weights and their products with V, 16 keys at a time
+#pragma unroll
+      for (int j = 0; j < kNt; j += 2) {
+        uint32_t p[kA];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int s = 0; s < kS; ++s) {
+            float x = sm100::ex2_approx(sc[j + u][2 * s] - base[s]), y = sm100::ex2_approx(sc[j + u][2 * s + 1] - base[s]);
+            l[s] += x + y;
+            if constexpr (kF8) x *= vs[j + u][0], y *= vs[j + u][1];
+            p[u * kS + s] = sm100::pack16x2<kBf16>(x, y);
+          }
+        if constexpr (!kF8) {
+#pragma unroll
+          for (int d = 0; d < kDt; d += 2) {
+            uint32_t r[4];
+            ldsm4_t(r, (vat ^ (d * 16)) + j * 8 * kRowBytes);
+            mma16<kBf16, kHalf>(o[d], p, r[0], r[1]);
+            mma16<kBf16, kHalf>(o[d + 1], p, r[2], r[3]);
+          }
+        } else {
+          // a 16-bit column of the transposed load is a pair of neighbouring elements; they go to products of their own
+#pragma unroll
+          for (int d = 0; d < kDt; d += 4) {
+            uint32_t r[4];
+            ldsm4_t(r, (vat ^ (d * 8)) + j * 8 * kRowBytes);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t lo0, lo1, hi0, hi1;  // (keys 2 quad and 2 quad + 1 of one element side by side, then of its neighbour)
+              e4m3x4_to_f16x2(__byte_perm(r[2 * c], 0, 0x3120), lo0, lo1);
+              e4m3x4_to_f16x2(__byte_perm(r[2 * c + 1], 0, 0x3120), hi0, hi1);
+              mma16<kBf16, kHalf>(o[d + 2 * c], p, lo0, hi0);
+              mma16<kBf16, kHalf>(o[d + 2 * c + 1], p, lo1, hi1);
+            }
           }
         }
       }
+      stage = stage == kStages - 1 ? 0 : stage + 1;
     }
-    stage = stage == kStages - 1 ? 0 : stage + 1;
-  }
-  cp_async_wait<0>();
-  __syncthreads();
 
-  // ---- the warps joined; element i of thread (oct, quad) of output tile j
+    // ---- what the item, or this part of it, comes to: a lane's elements lie in pairs, with an e4m3 cache in fours
 #pragma unroll
-  for (int s = 0; s < kS; ++s) {
-    l[s] += __shfl_xor_sync(0xffffffffu, l[s], 1);
-    l[s] += __shfl_xor_sync(0xffffffffu, l[s], 2);
-    if (quad == 0) m_s[warp][oct + 8 * s] = m[s], l_s[warp][oct + 8 * s] = l[s];
-  }
-  float* o_s = reinterpret_cast<float*>(smem) + warp * kHeads * kD;
-#pragma unroll
-  for (int j = 0; j < kDt; ++j)
-#pragma unroll
-    for (int s = 0; s < kS; ++s)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int col = quad * 2 + i;
-        const int d = kF8 ? j / 2 * 16 + col * 2 + (j & 1) : j * 8 + col;
-        o_s[(oct + 8 * s) * kD + d] = o[j][2 * s + i];
+    for (int s = 0; s < kS; ++s) {
+      l[s] += __shfl_xor_sync(0xffffffffu, l[s], 1);
+      l[s] += __shfl_xor_sync(0xffffffffu, l[s], 2);
+      const int g = oct + 8 * s;
+      if (g >= heads) continue;
+      const int64_t bh = (int64_t)b * a.H + h0 + g, part = (int64_t)slot * kHeads + g;
+      const float by = slot >= 0 ? 1.f : l[s] == 0.f ? 0.f : 1.f / l[s];
+      if (quad == 0) {
+        if (slot >= 0) a.part_ml[part] = make_float2(m[s] - kOffset, l[s]);
+        else if (a.lse) a.lse[bh] = l[s] == 0.f ? 0.f : m[s] - kOffset + log2f(l[s]);
       }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * kD; i += kThreads) {
-    const int g = i / kD, d = i % kD;
-    float top = m_s[0][g];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][g]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x = 0.f;
+      for (int j = 0; j < kDt; j += kF8 ? 2 : 1) {
+        const int d = kF8 ? j * 8 + quad * 4 : j * 8 + quad * 2;
+        constexpr int kN = kF8 ? 4 : 2;
+        float x[kN];
+        if constexpr (kF8) x[0] = o[j][2 * s], x[1] = o[j + 1][2 * s], x[2] = o[j][2 * s + 1], x[3] = o[j + 1][2 * s + 1];
+        else x[0] = o[j][2 * s], x[1] = o[j][2 * s + 1];
+        // (a head without weights is 0 even where what it would be divided by is not: 0 * 0)
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float keep = exp2f(m_s[w][g] - base);
-      sum += l_s[w][g] * keep;
-      x += reinterpret_cast<const float*>(smem)[(w * kHeads + g) * kD + d] * keep;
-    }
-    const int64_t bh = (int64_t)b * a.H + h0 + g;
-    if (a.splits == 1) {
-      store_any(a.o, bh * kD + d, a.dtype, sum == 0.f ? 0.f : x / sum);
-      if (a.lse && d == 0) a.lse[bh] = sum == 0.f ? 0.f : base - kOffset + log2f(sum);
-    } else {
-      a.part_o[(bh * a.splits + split) * kD + d] = x;
-      if (d == 0) a.part_ml[bh * a.splits + split] = make_float2(top - kOffset, sum);
+        for (int i = 0; i < kN; ++i) x[i] = l[s] == 0.f ? 0.f : x[i] * by;
+        if (slot >= 0) {
+          float* to = a.part_o + part * kD + d;
+          if constexpr (kF8) *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+          else *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
+        } else {
+          uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + bh * kD + d);
+#pragma unroll
+          for (int i = 0; i < kN; i += 2)
+            to[i / 2] = (kF8 ? a.dtype == KB_BF16 : kBf16) ? sm100::pack_bf16x2(x[i], x[i + 1]) : sm100::pack_f16x2(x[i], x[i + 1]);
+        }
+      }
     }
   }
+  let_next_launch_start();
+  cp_async_wait<0>();
 }
 
-template <bool kF8, bool kBf16, int kD, bool kHalf>
-int launch_mma(AttendArgs& a, cudaStream_t s) {
-  using Tile = MmaTile<kF8, kBf16, kD, kHalf>;
-  static std::atomic<bool> done[kMaxDevices];
-  int dev = 0, n_sm = 0;
-  if (!device_sm_count(&dev, &n_sm)) return KB_ERR_LAUNCH;
-  KB_CUDA_TRY(opt_in_smem_once(paged_attend_mma_kernel<kF8, kBf16, kD, kHalf>, Tile::kSmem, dev, done));
-  a.head_tiles = kb_cdiv_i32(a.group, Tile::kHeads);
-  paged_attend_mma_kernel<kF8, kBf16, kD, kHalf><<<dim3(a.splits, a.H_kv * a.head_tiles, a.B), kThreads, Tile::kSmem, s>>>(a);
-  KB_LAUNCH_CHECK("paged_attend_mma_kernel");
-  return KB_OK;
-}
-template <bool kF8, bool kBf16>
-int launch_mma(AttendArgs& a, cudaStream_t s) {
-  if (a.D == 64) return a.group <= 8 ? launch_mma<kF8, kBf16, 64, true>(a, s) : launch_mma<kF8, kBf16, 64, false>(a, s);
-  return a.group <= 8 ? launch_mma<kF8, kBf16, 128, true>(a, s) : launch_mma<kF8, kBf16, 128, false>(a, s);
-}
+// ---- the parts of an item joined -----------------------------------------------------------------------------------------
 
-// Whether the tensor-core kernel takes the call: a 16-bit q of head dim 64 or 128; keys and values of one layout, with rows on 16-byte
-// boundaries, within 2^32 such units.
-bool takes_mma(const kb_paged_attention_params& p) {
-  const kb_paged_cache& c = p.cache;
-  const int e = dtype_size(c.dtype);
-  if (p.dtype == KB_F32 || (c.D != 64 && c.D != 128) || !paged_rows_aligned(c, e)) return false;
-  int64_t last = 0;
-  const int32_t extent[3] = {c.P, c.H_kv, c.page};
-  for (int i = 0; i < 3; ++i) {
-    if (c.k_stride[i] != c.v_stride[i] || c.k_stride[i] < 0 || c.k_stride[i] > (int64_t)1 << 40) return false;
-    if (c.dtype == KB_E4M3 && c.k_scale_stride[i] != c.v_scale_stride[i]) return false;
-    if (i != 1) last += c.k_stride[i] * kb_max_i32(extent[i] - 1, 0);
-    if (last > (int64_t)1 << 40) return false;
-  }
-  return last * e / 16 < 0xffffffff - 64;
-}
+constexpr int kJoinThreads = 256;
 
-// ---- the parts of a head joined ------------------------------------------------------------------------------------------
-
-__global__ void paged_join_kernel(const AttendArgs a) {
-  const int64_t bh = blockIdx.x;
-  const int d = threadIdx.x;
-  const float2* ml = a.part_ml + bh * a.splits;
+// A block per item and head.  Groups of D / 4 threads take every so many-th part, four elements per thread; the groups are added up in order.
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendArgs a) {
+  __shared__ float red[kJoinThreads / 32], sums[kJoinThreads / 4], o_s[kJoinThreads * 4];
+  wait_for_launch_before();
+  const int4 word = a.join[blockIdx.x];  // first part, its unit, last unit, item
+  const int32_t g = blockIdx.y;
+  if (word.x < 0) return;
+  const int32_t per_seq = a.H_kv * a.head_tiles, b = word.w / per_seq, hy = word.w - b * per_seq, hk = hy / a.head_tiles;
+  const int32_t h = hk * a.group + (hy - hk * a.head_tiles) * a.heads + g;
+  if (h >= (hk + 1) * a.group) return;
+  const int32_t n = word.z - word.y + 1;
+  auto part_at = [&](int32_t i) { return (int64_t)(i == 0 ? word.x : 2 * (word.y + i)) * a.heads + g; };
   float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s].x);
+  for (int i = threadIdx.x; i < n; i += kJoinThreads) top = fmaxf(top, a.part_ml[part_at(i)].x);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[w]);
   const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, x = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float keep = exp2f(ml[s].x - base);
-    sum += ml[s].y * keep;
-    x += a.part_o[(bh * a.splits + s) * a.D + d] * keep;
+
+  const int width = a.D / 4, groups = kJoinThreads / width, group = threadIdx.x / width, d = (threadIdx.x - group * width) * 4;
+  float sum = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = group; i < n; i += groups) {
+    const float2 e = a.part_ml[part_at(i)];
+    const float4 y = *reinterpret_cast<const float4*>(a.part_o + part_at(i) * a.D + d);
+    const float keep = exp2f(e.x - base);
+    sum = fmaf(e.y, keep, sum);
+    x.x = fmaf(y.x, keep, x.x), x.y = fmaf(y.y, keep, x.y), x.z = fmaf(y.z, keep, x.z), x.w = fmaf(y.w, keep, x.w);
   }
-  store_any(a.o, bh * a.D + d, a.dtype, sum == 0.f ? 0.f : x / sum);
-  if (a.lse && d == 0) a.lse[bh] = sum == 0.f ? 0.f : base + log2f(sum);
+  *reinterpret_cast<float4*>(o_s + group * a.D + d) = x;
+  if (d == 0) sums[group] = sum;
+  __syncthreads();
+  const int64_t bh = (int64_t)b * a.H + h;
+  for (int i = threadIdx.x; i < a.D; i += kJoinThreads) {
+    float s = 0.f, y = 0.f;
+    for (int k = 0; k < groups; ++k) s += sums[k], y += o_s[k * a.D + i];
+    store_any(a.o, bh * a.D + i, a.dtype, s == 0.f ? 0.f : y / s);
+    if (a.lse && i == 0) a.lse[bh] = s == 0.f ? 0.f : base + log2f(s);
+  }
 }
 
 // ---- rows' weights -------------------------------------------------------------------------------------------------------
 
 __global__ void __launch_bounds__(256) paged_weigh_kernel(const AttendArgs a) {
   const int32_t hk = blockIdx.y, b = blockIdx.z;
+  wait_for_launch_before();
   int32_t first, end;
   seen_rows(a, b, first, end);
   for (int64_t r = (int64_t)first + blockIdx.x * 256 + threadIdx.x; r < end; r += (int64_t)gridDim.x * 256) {
@@ -655,51 +778,122 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const AttendArgs a) {
   }
 }
 
-template <typename T, int D>
-int launch_heads(AttendArgs& a, bool aligned, cudaStream_t s) {
-  if (a.group == 1) {
-    a.head_tiles = 1;
-    paged_attend_kernel<T, D, 1><<<dim3(a.splits, a.H_kv, a.B), kThreads, 0, s>>>(a, aligned);
-  } else {
-    a.head_tiles = (a.group + 3) / 4;
-    paged_attend_kernel<T, D, 4><<<dim3(a.splits, a.H_kv * a.head_tiles, a.B), kThreads, 0, s>>>(a, aligned);
+// Whether the tensor-core kernel takes the call: a 16-bit q of head dim 64 or 128 with dense heads; keys and values of one layout, with rows on
+// 16-byte boundaries, within 2^32 such units.
+bool takes_mma(const kb_paged_attention_params& p) {
+  const kb_paged_cache& c = p.cache;
+  const int e = dtype_size(c.dtype);
+  if (p.dtype == KB_F32 || (c.D != 64 && c.D != 128) || !paged_rows_aligned(c, e)) return false;
+  if (p.q_stride[2] != 1 || p.q_stride[0] % 2 || p.q_stride[1] % 2 || reinterpret_cast<uintptr_t>(p.q) % 4 || reinterpret_cast<uintptr_t>(p.o) % 4) return false;
+  int64_t last = 0;
+  const int32_t extent[3] = {c.P, c.H_kv, c.page};
+  for (int i = 0; i < 3; ++i) {
+    if (c.k_stride[i] != c.v_stride[i] || c.k_stride[i] < 0 || c.k_stride[i] > (int64_t)1 << 40) return false;
+    if (c.dtype == KB_E4M3 && c.k_scale_stride[i] != c.v_scale_stride[i]) return false;
+    if (c.k_stride[i] > 0 && extent[i] > 1 && c.k_stride[i] > ((int64_t)1 << 40) / extent[i]) return false;
+    last += c.k_stride[i] * kb_max_i32(extent[i] - 1, 0);
   }
-  KB_LAUNCH_CHECK("paged_attend_kernel");
-  return KB_OK;
+  return last * e / 16 < 0xffffffff - 64;
 }
 
-template <typename T>
-int launch_dim(AttendArgs& a, bool aligned, cudaStream_t s) {
-  switch (a.D) {
-    case 16: return launch_heads<T, 16>(a, aligned, s);
-    case 32: return launch_heads<T, 32>(a, aligned, s);
-    case 64: return launch_heads<T, 64>(a, aligned, s);
-    case 128: return launch_heads<T, 128>(a, aligned, s);
-    default: return launch_heads<T, 256>(a, aligned, s);
+// ---- launches --------------------------------------------------------------------------------------------------------------
+
+constexpr int kSms = 148;
+
+template <bool kF8, bool kBf16, int kD, bool kHalf>
+struct MmaKernel {
+  using Tile = MmaTile<kF8, kBf16, kD, kHalf>;
+  static constexpr int kHeads = Tile::kHeads, kRows = Tile::kR, kUnits = kSms * Tile::kBlocks * kWarps;
+  static constexpr int kLeast = 64 / kRows;  // tiles: short stretches leave parts that cost more to join than they save
+  static int launch(const AttendArgs& a, bool, cudaStream_t s) {
+    static std::atomic<bool> done[kMaxDevices];
+    int dev = 0, n_sm = 0;
+    if (!device_sm_count(&dev, &n_sm)) return KB_ERR_LAUNCH;
+    KB_CUDA_TRY(opt_in_smem_once(paged_attend_mma_kernel<kF8, kBf16, kD, kHalf>, Tile::kSmem, dev, done));
+    paged_attend_mma_kernel<kF8, kBf16, kD, kHalf><<<kb_cdiv_i32(a.units, kWarps), kThreads, Tile::kSmem, s>>>(a);
+    KB_LAUNCH_CHECK("paged_attend_mma_kernel");
+    return KB_OK;
+  }
+};
+template <typename T, int D, int G>
+struct GenericKernel {
+  static constexpr int kHeads = G, kRows = GenericTile<T, D>::kRows, kUnits = kSms * (G == 1 ? 4 : 2), kLeast = 1;
+  static int launch(const AttendArgs& a, bool aligned, cudaStream_t s) {
+    paged_attend_kernel<T, D, G><<<a.units, kThreads, 0, s>>>(a, aligned);
+    KB_LAUNCH_CHECK("paged_attend_kernel");
+    return KB_OK;
+  }
+};
+
+// f(a kernel): the one for the call
+template <bool kF8, bool kBf16, typename F>
+auto with_mma(const kb_paged_attention_params& p, F f) {
+  const bool half = p.H / p.cache.H_kv <= 8;
+  if (p.cache.D == 64) return half ? f(MmaKernel<kF8, kBf16, 64, true>()) : f(MmaKernel<kF8, kBf16, 64, false>());
+  return half ? f(MmaKernel<kF8, kBf16, 128, true>()) : f(MmaKernel<kF8, kBf16, 128, false>());
+}
+template <typename T, int D, typename F>
+auto with_group(const kb_paged_attention_params& p, F f) {
+  return p.H == p.cache.H_kv ? f(GenericKernel<T, D, 1>()) : f(GenericKernel<T, D, 4>());
+}
+template <typename T, typename F>
+auto with_generic(const kb_paged_attention_params& p, F f) {
+  switch (p.cache.D) {
+    case 16: return with_group<T, 16>(p, f);
+    case 32: return with_group<T, 32>(p, f);
+    case 64: return with_group<T, 64>(p, f);
+    case 128: return with_group<T, 128>(p, f);
+    default: return with_group<T, 256>(p, f);
+  }
+}
+template <typename F>
+auto with_kernel(const kb_paged_attention_params& p, F f) {
+  const int32_t dtype = p.cache.dtype;
+  if (takes_mma(p)) return dtype == KB_E4M3 ? with_mma<true, false>(p, f) : dtype == KB_BF16 ? with_mma<false, true>(p, f) : with_mma<false, false>(p, f);
+  switch (dtype) {
+    case KB_F32: return with_generic<float>(p, f);
+    case KB_F16: return with_generic<__half>(p, f);
+    case KB_BF16: return with_generic<__nv_bfloat16>(p, f);
+    default: return with_generic<uint8_t>(p, f);
   }
 }
 
-// Rows that a token can see at most, from sizes alone: the lengths are on the device.
-int32_t most_rows(const kb_paged_attention_params& p) {
-  const int64_t capacity = (int64_t)p.cache.M * p.cache.page;
-  const int64_t window = p.context_size > 0 ? ((int64_t)p.back_contexts + 1) * p.context_size : capacity;
-  return (int32_t)(window < capacity ? window : capacity);
-}
+// What follows from the sizes alone (the lengths are on the device).
+struct Plan {
+  int32_t heads, head_tiles, units, least, most_rows;
+  bool by_item, joins;
+  size_t join_bytes, part_bytes, ml_bytes, score_bytes;
+};
 
-// Blocks per head: as many as fill the GPU a few times over, none shorter than 256 rows.
-int32_t split_count(const kb_paged_attention_params& p) {
-  const int64_t items = (int64_t)p.cache.B * p.cache.H_kv;
-  const int64_t fill = (148 * 8 + items - 1) / items, most = kb_cdiv_i32(most_rows(p), 256);
-  return (int32_t)(fill < most ? fill : most < 1 ? 1 : most);
+template <typename K>
+Plan make_plan(const kb_paged_attention_params& p) {
+  Plan n{};
+  const kb_paged_cache& c = p.cache;
+  n.heads = K::kHeads;
+  n.head_tiles = kb_cdiv_i32(p.H / c.H_kv, K::kHeads);
+  n.least = K::kLeast;
+  const int64_t capacity = (int64_t)c.M * c.page, window = p.context_size > 0 ? ((int64_t)p.back_contexts + 1) * p.context_size : capacity;
+  n.most_rows = (int32_t)(window < capacity ? window : capacity);
+  const int64_t items = (int64_t)c.B * c.H_kv * n.head_tiles, tiles = (n.most_rows + K::kRows - 1) / K::kRows;
+  const int64_t stretches = (items * (tiles < 1 ? 1 : tiles) + K::kLeast - 1) / K::kLeast;
+  n.units = (int32_t)(stretches < K::kUnits ? stretches : K::kUnits);
+  n.by_item = items <= n.units;
+  n.joins = n.units > 1;
+  const size_t entries = n.by_item ? items : n.units, parts = 2 * (size_t)n.units * n.heads;
+  n.join_bytes = entries * sizeof(int4);
+  n.part_bytes = parts * c.D * sizeof(float);
+  n.ml_bytes = parts * sizeof(float2);
+  n.score_bytes = p.weights ? (size_t)c.B * p.H * capacity * sizeof(float) : 0;
+  return n;
 }
 
 }  // namespace
 
 size_t paged_attention_workspace_bytes(const kb_paged_attention_params& p) {
-  const size_t heads = (size_t)p.cache.B * p.H, splits = split_count(p);
-  size_t n = splits > 1 ? heads * splits * (p.cache.D + 2) : 0;
-  if (p.weights) n += heads * p.cache.M * p.cache.page;
-  return n * sizeof(float);
+  return with_kernel(p, [&](auto kernel) {
+    const Plan n = make_plan<decltype(kernel)>(p);
+    return n.join_bytes + n.part_bytes + n.ml_bytes + n.score_bytes;
+  });
 }
 
 int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
@@ -715,36 +909,27 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
     a.back = kb_clamp_back(p.back_contexts, a.c.capacity, a.context);
     a.fd_context = kb_fastdiv_make(a.context);
   }
-  a.splits = split_count(p);
   a.scale_log2 = p.sm_scale * kLog2e;
-  float* w = static_cast<float*>(p.workspace);
-  const size_t heads = (size_t)c.B * p.H;
-  if (a.splits > 1) {
-    a.part_ml = reinterpret_cast<float2*>(w);
-    a.part_o = w + heads * a.splits * 2;
-    w = a.part_o + heads * a.splits * c.D;
-  }
-  if (p.weights) a.scores = w;
-  const bool aligned = paged_rows_aligned(c, dtype_size(c.dtype));
-  int rc;
-  if (takes_mma(p)) rc = c.dtype == KB_E4M3 ? launch_mma<true, false>(a, s) : c.dtype == KB_BF16 ? launch_mma<false, true>(a, s) : launch_mma<false, false>(a, s);
-  else switch (c.dtype) {
-    case KB_F32: rc = launch_dim<float>(a, aligned, s); break;
-    case KB_F16: rc = launch_dim<__half>(a, aligned, s); break;
-    case KB_BF16: rc = launch_dim<__nv_bfloat16>(a, aligned, s); break;
-    default: rc = launch_dim<uint8_t>(a, aligned, s); break;
-  }
-  if (rc) return rc;
-  if (a.splits > 1) {
-    paged_join_kernel<<<(unsigned)heads, a.D, 0, s>>>(a);
-    KB_LAUNCH_CHECK("paged_join_kernel");
-  }
-  if (p.weights) {
-    const int32_t blocks = kb_cdiv_i32(most_rows(p), 256), fill = kb_max_i32(1, 148 * 16 / kb_max_i32(1, c.B * c.H_kv));
-    paged_weigh_kernel<<<dim3(blocks < fill ? kb_max_i32(1, blocks) : fill, c.H_kv, c.B), 256, 0, s>>>(a);
-    KB_LAUNCH_CHECK("paged_weigh_kernel");
-  }
-  return KB_OK;
+  return with_kernel(p, [&](auto kernel) {
+    const Plan n = make_plan<decltype(kernel)>(p);
+    a.heads = n.heads, a.head_tiles = n.head_tiles, a.units = n.units, a.least_tiles = n.least, a.by_item = n.by_item;
+    char* w = static_cast<char*>(p.workspace);
+    a.join = reinterpret_cast<int4*>(w), w += n.join_bytes;
+    a.part_o = reinterpret_cast<float*>(w), w += n.part_bytes;
+    a.part_ml = reinterpret_cast<float2*>(w), w += n.ml_bytes;
+    if (p.weights) a.scores = reinterpret_cast<float*>(w);
+    if (int rc = kernel.launch(a, paged_rows_aligned(c, dtype_size(c.dtype)), s)) return rc;
+    if (n.joins) {
+      const dim3 grid((unsigned)(n.join_bytes / sizeof(int4)), kb_min_i32(n.heads, a.group));
+      if (int rc = launch_after(paged_join_kernel, grid, kJoinThreads, s, a)) return rc;
+    }
+    if (p.weights) {
+      const int32_t blocks = kb_cdiv_i32(n.most_rows, 256), fill = kb_max_i32(1, kSms * 16 / (c.B * c.H_kv));
+      const dim3 grid(kb_max_i32(1, kb_min_i32(blocks, fill)), c.H_kv, c.B);
+      if (int rc = launch_after(paged_weigh_kernel, grid, 256, s, a)) return rc;
+    }
+    return (int)KB_OK;
+  });
 }
 
 }  // namespace kb

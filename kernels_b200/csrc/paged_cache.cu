@@ -15,12 +15,14 @@
 #include "paged.cuh"
 #include "sm100_ptx.cuh"
 
+#include <type_traits>
+
 namespace kb {
 namespace {
 
 // ---- write -----------------------------------------------------------------------------------------------------------
 
-constexpr int kWriteThreads = 256, kPerThread = 8;
+constexpr int kWriteThreads = 256, kPerThread = 8, kHeadsAtOnce = 4;
 
 struct WriteArgs {
   PagedView c;
@@ -33,112 +35,151 @@ struct WriteArgs {
   float* weights;
   int32_t* row_positions;
   int64_t w_b, w_h, p_b, p_h;
-  int32_t B, H_kv, T, D, rows_per_cta;
-  KbFastDiv fd_T, fd_H;
-  bool aligned;
+  int32_t B, H_kv, T, D, heads_per_cta;
+  KbFastDiv fd_T;
 };
 
-// x / scale, correctly rounded: the row's elements as its 8-bit form holds them
-__device__ __forceinline__ uint2 quantize8(const float (&f)[8], float scale) {
-  return make_uint2(sm100::pack_e4m3x4(__fdiv_rn(f[0], scale), __fdiv_rn(f[1], scale), __fdiv_rn(f[2], scale), __fdiv_rn(f[3], scale)),
-                    sm100::pack_e4m3x4(__fdiv_rn(f[4], scale), __fdiv_rn(f[5], scale), __fdiv_rn(f[6], scale), __fdiv_rn(f[7], scale)));
+template <typename T>
+struct Eight { T v[kPerThread]; };
+
+template <typename T, bool kAligned>
+__device__ __forceinline__ void load8(Eight<T>& e, const T* x, int64_t sd) {
+  if constexpr (kAligned) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(&e)[i] = __ldcs(reinterpret_cast<const uint4*>(x) + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) e.v[i] = x[i * sd];
+  }
+}
+template <typename T, bool kAligned>
+__device__ __forceinline__ void store8(T* out, const Eight<T>& e) {
+  if constexpr (kAligned && sizeof(T) == 1) {
+    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(&e);
+  } else if constexpr (kAligned) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(&e)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) out[i] = e.v[i];
+  }
 }
 
-// T: the tokens' type; F8: the cache holds e4m3, otherwise T
-template <typename T, bool F8>
+// The row's elements as its 8-bit form holds them, x / scale correctly rounded.
+template <typename T>
+__device__ __forceinline__ Eight<uint8_t> quantize8(const Eight<T>& e, float scale) {
+  float f[kPerThread];
+  if (scale <= 1e37f) {
+    const float r = 1.f / scale;
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) f[i] = div_by(to_f32(e.v[i]), scale, r);
+  } else {  // an infinity or a NaN in the row
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) f[i] = to_f32(e.v[i]) / scale;
+  }
+  Eight<uint8_t> out;
+  reinterpret_cast<uint32_t*>(&out)[0] = sm100::pack_e4m3x4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<uint32_t*>(&out)[1] = sm100::pack_e4m3x4(f[4], f[5], f[6], f[7]);
+  return out;
+}
+
+// T: the tokens' type; kF8: the cache holds e4m3, otherwise T
+template <typename T, bool kF8, bool kAligned>
 __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteArgs a) {
   const int lanes = a.D / kPerThread;  // 2, 4, 8, 16 or 32 threads per row
-  const int lane = threadIdx.x & (lanes - 1);
-  const int64_t row_id = (int64_t)blockIdx.x * a.rows_per_cta + threadIdx.x / lanes;  // (b, h, t)
-  const int which = blockIdx.y;
-  bool live = row_id < (int64_t)a.B * a.H_kv * a.T;
-  int32_t b = 0, h = 0, t = 0, at = 0, page = -1;
+  const int lane = threadIdx.x & (lanes - 1), d = lane * kPerThread;
+  const int64_t token = (int64_t)blockIdx.x * (kWriteThreads / lanes) + threadIdx.x / lanes;
+  const int32_t h0 = blockIdx.y * a.heads_per_cta, h1 = kb_min_i32(h0 + a.heads_per_cta, a.H_kv);
+  bool live = token < (int64_t)a.B * a.T;
+  int32_t b = 0, t = 0, at = 0, page = -1;
+  int64_t row = 0;
   if (live) {
-    const int32_t bh = kb_fastdiv((int32_t)row_id, a.fd_T);
-    t = (int32_t)row_id - bh * a.T;
-    b = kb_fastdiv(bh, a.fd_H);
-    h = bh - b * a.H_kv;
+    b = kb_fastdiv((int32_t)token, a.fd_T);
+    t = (int32_t)token - b * a.T;
     const int32_t n = a.new_lens ? kb_clamp_len(a.new_lens[b * a.new_lens_b], a.T) : a.T;
-    const int64_t row = (int64_t)a.c.lens[b * a.c.lens_b] - n + t;
+    row = (int64_t)a.c.lens[b * a.c.lens_b] - n + t;
     live = t < n && row >= 0 && row < a.c.capacity;
-    if (live) {
-      page = a.c.locate(b, (int32_t)row, at);
-      if (which == 0 && lane == 0) {
-        if (a.weights) a.weights[b * a.w_b + h * a.w_h + row] = 0.f;
-        if (a.row_positions) a.row_positions[b * a.p_b + h * a.p_h + row] = a.positions ? a.positions[b * a.pos_b + t * a.pos_t] : (int32_t)row;
-      }
+  }
+  if (live) {
+    page = a.c.locate(b, (int32_t)row, at);
+    const int32_t position = a.positions ? a.positions[b * a.pos_b + t * a.pos_t] : (int32_t)row;
+    for (int32_t h = h0 + lane; h < h1; h += lanes) {
+      if (a.weights) a.weights[b * a.w_b + h * a.w_h + row] = 0.f;
+      if (a.row_positions) a.row_positions[b * a.p_b + h * a.p_h + row] = position;
     }
   }
   live = live && page >= 0;
-  T e[kPerThread];
-  const int d = lane * kPerThread;
-  if (live) {
-    const T* x = static_cast<const T*>(a.x[which]) + b * a.sb[which] + h * a.sh[which] + t * a.st[which] + d * a.sd[which];
-    if (a.aligned) {
+  if (!__any_sync(0xffffffffu, live)) return;
+  const T* from[2];
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) * kPerThread / 16; ++i) reinterpret_cast<uint4*>(e)[i] = __ldcs(reinterpret_cast<const uint4*>(x) + i);
-    } else {
+  for (int w = 0; w < 2; ++w) from[w] = static_cast<const T*>(a.x[w]) + b * a.sb[w] + t * a.st[w] + d * a.sd[w];
+  const int64_t to[2] = {page * a.c.k_page + at * a.c.k_row + d, page * a.c.v_page + at * a.c.v_row + d};
+  const int64_t head[2] = {a.c.k_head, a.c.v_head};
+  char* base[2] = {a.c.k, a.c.v};
+  for (int32_t h2 = h0; h2 < h1; h2 += kHeadsAtOnce) {
+    Eight<T> e[2][kHeadsAtOnce];
 #pragma unroll
-      for (int i = 0; i < kPerThread; ++i) e[i] = x[i * a.sd[which]];
-    }
-  } else {
+    for (int u = 0; u < kHeadsAtOnce; ++u)
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) e[i] = from_f32<T>(0.f);
-  }
-  const int64_t at_page = which ? page * a.c.v_page + h * a.c.v_head + at * a.c.v_row : page * a.c.k_page + h * a.c.k_head + at * a.c.k_row;
-  char* base = which ? a.c.v : a.c.k;
-  if constexpr (F8) {
-    float f[kPerThread];
-    // as bits without the sign: numbers keep their order, and a NaN is above them all, so that it reaches the scale
-    uint32_t m = 0;
+      for (int w = 0; w < 2; ++w) {
+        if (live && h2 + u < h1) {
+          load8<T, kAligned>(e[w][u], from[w] + (h2 + u) * a.sh[w], a.sd[w]);
+        } else {
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      f[i] = to_f32(e[i]);
-      m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-    }
-    for (int s = lanes / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
-    float scale = __fmul_rn(__uint_as_float(m), 1.f / 448.f);
-    if (scale < 1e-12f) scale = 1e-12f;  // (a NaN stays)
-    if (live) {
-      if (lane == 0) {
-        if (which) a.c.v_scale[page * a.c.vs_page + h * a.c.vs_head + at * a.c.vs_row] = scale;
-        else a.c.k_scale[page * a.c.ks_page + h * a.c.ks_head + at * a.c.ks_row] = scale;
+          for (int i = 0; i < kPerThread; ++i) e[w][u].v[i] = from_f32<T>(0.f);
+        }
       }
-      const uint2 w = quantize8(f, scale);
-      uint8_t* out = reinterpret_cast<uint8_t*>(base) + at_page + d;
-      if (a.aligned) {
-        *reinterpret_cast<uint2*>(out) = w;
-      } else {
-        const uint8_t* wb = reinterpret_cast<const uint8_t*>(&w);
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) out[i] = wb[i];
+    for (int u = 0; u < kHeadsAtOnce; ++u)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int32_t h = h2 + u;
+        const bool write = live && h < h1;
+        if constexpr (kF8) {
+          // as bits without the sign: numbers keep their order, and a NaN is above them all, so that it reaches the scale
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < kPerThread; ++i) m = max(m, __float_as_uint(to_f32(e[w][u].v[i])) & 0x7fffffffu);
+          for (int s = lanes / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
+          float scale = __fmul_rn(__uint_as_float(m), 1.f / 448.f);
+          if (scale < 1e-12f) scale = 1e-12f;  // (a NaN stays)
+          if (write) {
+            if (lane == 0) {
+              if (w) a.c.v_scale[page * a.c.vs_page + h * a.c.vs_head + at * a.c.vs_row] = scale;
+              else a.c.k_scale[page * a.c.ks_page + h * a.c.ks_head + at * a.c.ks_row] = scale;
+            }
+            store8<uint8_t, kAligned>(reinterpret_cast<uint8_t*>(base[w]) + to[w] + h * head[w], quantize8(e[w][u], scale));
+          }
+        } else if (write) {
+          store8<T, kAligned>(reinterpret_cast<T*>(base[w]) + to[w] + h * head[w], e[w][u]);
+        }
       }
-    }
-  } else if (live) {
-    T* out = reinterpret_cast<T*>(base) + at_page + d;
-    if (a.aligned) {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) * kPerThread / 16; ++i) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(e)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) out[i] = e[i];
-    }
   }
 }
 
 template <typename T>
-int launch_write(const WriteArgs& a, bool f8, cudaStream_t s) {
-  const int64_t rows = (int64_t)a.B * a.H_kv * a.T;
-  const dim3 grid((unsigned)((rows + a.rows_per_cta - 1) / a.rows_per_cta), 2);
-  if (f8) paged_write_kernel<T, true><<<grid, kWriteThreads, 0, s>>>(a);
-  else paged_write_kernel<T, false><<<grid, kWriteThreads, 0, s>>>(a);
+int launch_write(const WriteArgs& in, bool f8, bool aligned, cudaStream_t s) {
+  WriteArgs a = in;
+  const int64_t tokens = (int64_t)a.B * a.T, each = kWriteThreads / (a.D / kPerThread), ctas = (tokens + each - 1) / each;
+  // few tokens: the heads go to blocks of their own
+  a.heads_per_cta = ctas >= 148 * 4 ? a.H_kv : kHeadsAtOnce;
+  const dim3 grid((unsigned)ctas, (unsigned)kb_cdiv_i32(a.H_kv, a.heads_per_cta));
+  if (f8) {
+    if (aligned) paged_write_kernel<T, true, true><<<grid, kWriteThreads, 0, s>>>(a);
+    else paged_write_kernel<T, true, false><<<grid, kWriteThreads, 0, s>>>(a);
+  } else {
+    if (aligned) paged_write_kernel<T, false, true><<<grid, kWriteThreads, 0, s>>>(a);
+    else paged_write_kernel<T, false, false><<<grid, kWriteThreads, 0, s>>>(a);
+  }
   KB_LAUNCH_CHECK("paged_write_kernel");
   return KB_OK;
 }
 
 // ---- evict -----------------------------------------------------------------------------------------------------------
 
-constexpr int kSelectThreads = 1024, kMoveThreads = 256;
+constexpr int kMoveThreads = 256;
+constexpr int kKeys = 16, kWarpRows = 32 * kKeys;     // rows of a warp whose keys its lanes hold
+constexpr int kBlockRows = 32 * kWarpRows, kMostCluster = 8;
 
 struct EvictArgs {
   PagedView c;
@@ -148,11 +189,11 @@ struct EvictArgs {
   int32_t* positions_out;
   int32_t* lens_out;
   int64_t w_b, w_h, p_b, p_h, wo_b, wo_h, po_b, po_h, lens_out_b;
-  int32_t H_kv, D, budget, recent, most_moves, elsize;
+  int32_t H_kv, D, budget, recent, most_moves, elsize, cluster;
   int32_t* counts;  // [B, H_kv]
   int32_t* src;     // [B, H_kv, most_moves]
   int32_t* dst;
-  bool in_place, aligned;
+  bool in_place;
 };
 
 // Weights as whole numbers of the same order; a NaN is below them all, the newest rows are above.
@@ -163,128 +204,216 @@ __device__ __forceinline__ uint32_t rank_key(float w, bool newest) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ int block_sum(int x, int* red) {
-  x = __reduce_add_sync(0xffffffffu, x);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, (int)(threadIdx.x & 31) < (int)(blockDim.x >> 5) ? red[threadIdx.x & 31] : 0);
-}
+// What the warps of a cluster's blocks have in common.  Each value goes through shared memory once; buffers alternate, so that one
+// barrier per value is enough.
+struct Team {
+  int (*red)[32];       // [2][warps]: this block's
+  int (*of_rank)[8];    // [2][ranks]
+  int size, rank, turn; // of the cluster
 
-// Sum over the warps before this one of x (the same in all lanes of a warp).
-__device__ __forceinline__ int warps_before(int x, int* red) {
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, (threadIdx.x & 31) < (threadIdx.x >> 5) ? red[threadIdx.x & 31] : 0);
-}
+  // op over the team's warps of `x` (the same in a warp's lanes); `before`: over the warps before this one only
+  template <typename Op>
+  __device__ __forceinline__ int all(int x, int none, Op op, int* before = nullptr) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int(&buf)[32] = red[turn];
+    if (lane == 0) buf[warp] = x;
+    __syncthreads();
+    const int mine = lane < warps ? buf[lane] : none;
+    int sum = op(mine);
+    if (before) *before = op(lane < warp ? mine : none);
+    if (size > 1) {
+      if (threadIdx.x < size) {
+        uint32_t to;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sm100::smem_u32(&of_rank[turn][rank])), "r"(threadIdx.x));
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to), "r"(sum) : "memory");
+      }
+      sm100::cluster_sync_all();
+      const int theirs = lane < size ? of_rank[turn][lane] : none;
+      if (before) {
+        const int lower = op(lane < rank ? theirs : none);
+        *before = op(lane == 0 ? *before : lane == 1 ? lower : none);
+      }
+      sum = op(theirs);
+    }
+    turn ^= 1;
+    return sum;
+  }
+  __device__ __forceinline__ int sum(int x, int* before = nullptr) {
+    return all(x, 0, [](int v) { return __reduce_add_sync(0xffffffffu, v); }, before);
+  }
+  __device__ __forceinline__ int max(int x) {
+    return all(x, INT32_MIN, [](int v) { return __reduce_max_sync(0xffffffffu, v); });
+  }
+};
 
-__global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const EvictArgs a) {
-  __shared__ int red[32];
-  const int32_t h = blockIdx.x, b = blockIdx.y;
+// A team (a block, or a cluster of them) per sequence and head; warp w of it has the rows [w S, (w + 1) S), 32 at a time so that ranks
+// within it are ballots.  kHeld: S = kWarpRows and the keys stay in registers; otherwise the rows are as many as there are, and
+// the keys are formed again from memory whenever they are needed.
+template <bool kHeld>
+__global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
+  __shared__ int red[2][32], of_rank[2][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  Team team{red, of_rank, a.cluster, (int)blockIdx.x % a.cluster, 0};
+  const int32_t h = blockIdx.x / a.cluster, b = blockIdx.y;
   const int32_t n = a.c.rows(b);
   const float* w = a.weights + b * a.w_b + h * a.w_h;
   const int32_t* pos = a.positions + b * a.p_b + h * a.p_h;
   float* wo = a.weights_out + b * a.wo_b + h * a.wo_h;
   int32_t* po = a.positions_out + b * a.po_b + h * a.po_h;
-  if (!a.in_place)
-    for (int i = threadIdx.x; i < min(n, a.budget); i += kSelectThreads) wo[i] = w[i], po[i] = pos[i];
   int32_t* count = a.counts + (int64_t)b * a.H_kv + h;
-  if (n <= a.budget) {
-    if (threadIdx.x == 0) *count = 0;
-    return;
-  }
-  int32_t newest = INT32_MIN;
-  for (int i = threadIdx.x; i < n; i += kSelectThreads) newest = max(newest, pos[i]);
-  newest = __reduce_max_sync(0xffffffffu, newest);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = newest;
-  __syncthreads();
-  newest = __reduce_max_sync(0xffffffffu, red[threadIdx.x & 31]);
-  const int64_t from = (int64_t)newest - a.recent;  // positions above it are among the newest
-  auto key = [&](int i) { return rank_key(w[i], pos[i] > from); };
-
-  // the largest threshold that at least `budget` keys reach, bit by bit
-  uint32_t least = 0;
-  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-    int reach = 0;
-    for (int i = threadIdx.x; i < n; i += kSelectThreads) reach += key(i) >= (least | bit);
-    if (block_sum(reach, red) >= a.budget) least |= bit;
-  }
-  // A warp owns a run of rows, 32 at a time, so that ranks within it are ballots.
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per_warp = kHeld ? kWarpRows : kb_cdiv_i32(kb_max_i32(n, 1), warps * 32) * 32;
+  const int begin = kb_min_i32((team.rank * warps + warp) * per_warp, n), end = kb_min_i32(begin + per_warp, n);
   const uint32_t below = (1u << lane) - 1;
-  const int per_warp = ((n + kSelectThreads - 1) / kSelectThreads) * 32;
-  const int begin = min(warp * per_warp, n), end = min(begin + per_warp, n);
-  int above = 0, equal = 0;
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const uint32_t k = i0 + lane < end ? key(i0 + lane) : 0;
-    above += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && k > least));
-    equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < end && k == least));
+
+  if (a.cluster > 1) sm100::cluster_sync_all();  // (a block's shared memory may be written once the block has started)
+  uint32_t held[kHeld ? kKeys : 1];
+  int32_t newest = INT32_MIN;
+  if constexpr (kHeld) {
+    float x[kKeys];
+    int32_t y[kKeys];
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const int i = begin + j * 32 + lane;
+      x[j] = i < end ? w[i] : 0.f;
+      y[j] = i < end ? pos[i] : INT32_MIN;
+    }
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const int i = begin + j * 32 + lane;
+      if (!a.in_place && i < end && i < a.budget) wo[i] = x[j], po[i] = y[j];
+      newest = max(newest, y[j]);
+    }
+    if (n <= a.budget) {
+      if (threadIdx.x == 0 && team.rank == 0) *count = 0;
+      return;
+    }
+    newest = team.max(__reduce_max_sync(0xffffffffu, newest));
+    const int64_t from = (int64_t)newest - a.recent;  // positions above it are among the newest
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) held[j] = begin + j * 32 + lane < end ? rank_key(x[j], y[j] > from) : 0u;
+  } else {
+    for (int i = begin + lane; i < end; i += 32) {
+      if (!a.in_place && i < a.budget) wo[i] = w[i], po[i] = pos[i];
+      newest = max(newest, pos[i]);
+    }
+    if (n <= a.budget) {
+      if (threadIdx.x == 0) *count = 0;
+      return;
+    }
+    newest = team.max(__reduce_max_sync(0xffffffffu, newest));
   }
-  const int ties = a.budget - block_sum(lane == 0 ? above : 0, red);  // so many of the equal keys stay, the lowest rows
-  const int equal_before = warps_before(equal, red);
-  for (int pass = 0, holes = 0, movers = 0; pass < 2; ++pass) {
-    int ties_seen = equal_before, hole_at = 0, mover_at = 0;
-    if (pass) hole_at = warps_before(holes, red), mover_at = warps_before(movers, red);
-    for (int i0 = begin; i0 < end; i0 += 32) {
-      const int i = i0 + lane;
-      const bool in = i < end;
-      const uint32_t k = in ? key(i) : 0;
+  const int64_t from = (int64_t)newest - a.recent;
+  // f(key, row, whether there is such a row) for the warp's rows, all lanes together
+  auto each = [&](auto f) {
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < kKeys; ++j)
+        if (begin + j * 32 < end) f(held[j], begin + j * 32 + lane, begin + j * 32 + lane < end);
+    } else {
+      for (int i0 = begin; i0 < end; i0 += 32) {
+        const int i = i0 + lane;
+        f(i < end ? rank_key(w[i], pos[i] > from) : 0u, i, i < end);
+      }
+    }
+  };
+  // the largest threshold that at least `budget` keys reach, bit by bit; done where exactly so many reach it
+  uint32_t least = 0;
+  int reached = n;
+  for (uint32_t bit = 0x80000000u; bit && reached != a.budget; bit >>= 1) {
+    int reach = 0;
+    each([&](uint32_t k, int, bool) { reach += k >= (least | bit); });  // (a row that is not there has key 0)
+    reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
+    if (reach >= a.budget) least |= bit, reached = reach;
+  }
+  int above = 0, equal = 0, equal_before;
+  each([&](uint32_t k, int, bool in) {
+    above += __popc(__ballot_sync(0xffffffffu, in && k > least));
+    equal += __popc(__ballot_sync(0xffffffffu, in && k == least));
+  });
+  team.sum(equal, &equal_before);
+  const int ties = a.budget - team.sum(above);  // so many of the equal keys stay, the lowest rows
+  let_next_launch_start();
+  const int64_t list = ((int64_t)b * a.H_kv + h) * a.most_moves;
+  int holes = 0, movers = 0, hole_at = 0, mover_at = 0;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+    int ties_seen = equal_before;
+    each([&](uint32_t k, int i, bool in) {
       const uint32_t eq = __ballot_sync(0xffffffffu, in && k == least);
       const bool keep = in && (k > least || (k == least && ties_seen + __popc(eq & below) < ties));
       ties_seen += __popc(eq);
       const bool hole = in && !keep && i < a.budget, mover = keep && i >= a.budget;
       const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
       if (pass) {
-        const int64_t list = ((int64_t)b * a.H_kv + h) * a.most_moves;
         if (hole) a.dst[list + hole_at + __popc(hb & below)] = i;
         if (mover) a.src[list + mover_at + __popc(mb & below)] = i;
         hole_at += __popc(hb), mover_at += __popc(mb);
       } else {
         holes += __popc(hb), movers += __popc(mb);
       }
-    }
+    });
     if (pass == 0) {
-      const int moves = block_sum(lane == 0 ? movers : 0, red);
-      if (threadIdx.x == 0) *count = moves;
+      team.sum(holes, &hole_at);
+      const int moves = team.sum(movers, &mover_at);
+      if (threadIdx.x == 0 && team.rank == 0) *count = moves;
     }
   }
 }
 
-__device__ __forceinline__ void copy_row(char* to, const char* from, int bytes, int lane, bool aligned) {
-  if (aligned) {
-    if (lane * 16 < bytes) *reinterpret_cast<uint4*>(to + lane * 16) = *reinterpret_cast<const uint4*>(from + lane * 16);
-    if ((lane + 32) * 16 < bytes) *reinterpret_cast<uint4*>(to + (lane + 32) * 16) = *reinterpret_cast<const uint4*>(from + (lane + 32) * 16);
-  } else {
-    for (int i = lane; i < bytes; i += 32) to[i] = from[i];
-  }
-}
-
-// A warp moves a row at a time.
+// A warp takes 32 moves at a time: a lane looks up one of them and moves its entries of the bookkeeping, then the lanes copy the rows together.
+template <bool kAligned>
 __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const EvictArgs a) {
-  const int32_t h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
+  constexpr int kUnit = kAligned ? 16 : 1, kAtOnce = 4;
+  __shared__ longlong2 k_at[kMoveThreads], v_at[kMoveThreads];  // {from, to} in bytes; from -1: no such row
+  const int32_t h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t bh = (int64_t)b * a.H_kv + h;
+  const PagedView& c = a.c;
+  wait_for_launch_before();
   // (in place, no other block reads the lengths any more: the rows come from the lists)
-  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.lens_out[b * a.lens_out_b] = min(max(a.c.lens[b * a.c.lens_b], 0), a.budget);
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.lens_out[b * a.lens_out_b] = min(max(c.lens[b * c.lens_b], 0), a.budget);
   const int32_t moves = a.counts[bh];
-  const int row_bytes = a.D * a.elsize;
-  for (int32_t i = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); i < moves; i += gridDim.x * (kMoveThreads / 32)) {
-    const int32_t src = a.src[bh * a.most_moves + i], dst = a.dst[bh * a.most_moves + i];
-    int32_t sr, dr;
-    const int32_t sp = a.c.locate(b, src, sr), dp = a.c.locate(b, dst, dr);
-    if (lane == 0) {
+  const int units = a.D * a.elsize / kUnit;  // of a row: a power of two
+  const int shift = __ffs(units) - 1;
+  for (int32_t i0 = (blockIdx.x * (kMoveThreads / 32) + warp) * 32; i0 < moves; i0 += gridDim.x * kMoveThreads) {
+    const int32_t many = min(32, moves - i0);
+    longlong2 k = make_longlong2(-1, 0), v = k;
+    if (lane < many) {
+      const int32_t src = a.src[bh * a.most_moves + i0 + lane], dst = a.dst[bh * a.most_moves + i0 + lane];
+      int32_t sr, dr;
+      const int32_t sp = c.locate(b, src, sr), dp = c.locate(b, dst, dr);
       a.weights_out[b * a.wo_b + h * a.wo_h + dst] = a.weights[b * a.w_b + h * a.w_h + src];
       a.positions_out[b * a.po_b + h * a.po_h + dst] = a.positions[b * a.p_b + h * a.p_h + src];
+      if (sp >= 0 && dp >= 0) {
+        k = make_longlong2((sp * c.k_page + h * c.k_head + sr * c.k_row) * a.elsize, (dp * c.k_page + h * c.k_head + dr * c.k_row) * a.elsize);
+        v = make_longlong2((sp * c.v_page + h * c.v_head + sr * c.v_row) * a.elsize, (dp * c.v_page + h * c.v_head + dr * c.v_row) * a.elsize);
+        if (c.k_scale) {
+          c.k_scale[dp * c.ks_page + h * c.ks_head + dr * c.ks_row] = c.k_scale[sp * c.ks_page + h * c.ks_head + sr * c.ks_row];
+          c.v_scale[dp * c.vs_page + h * c.vs_head + dr * c.vs_row] = c.v_scale[sp * c.vs_page + h * c.vs_head + sr * c.vs_row];
+        }
+      }
     }
-    if (sp < 0 || dp < 0) continue;
-    const PagedView& c = a.c;
-    copy_row(c.k + (dp * c.k_page + h * c.k_head + dr * c.k_row) * a.elsize, c.k + (sp * c.k_page + h * c.k_head + sr * c.k_row) * a.elsize,
-             row_bytes, lane, a.aligned);
-    copy_row(c.v + (dp * c.v_page + h * c.v_head + dr * c.v_row) * a.elsize, c.v + (sp * c.v_page + h * c.v_head + sr * c.v_row) * a.elsize,
-             row_bytes, lane, a.aligned);
-    if (c.k_scale && lane == 0) {
-      c.k_scale[dp * c.ks_page + h * c.ks_head + dr * c.ks_row] = c.k_scale[sp * c.ks_page + h * c.ks_head + sr * c.ks_row];
-      c.v_scale[dp * c.vs_page + h * c.vs_head + dr * c.vs_row] = c.v_scale[sp * c.vs_page + h * c.vs_head + sr * c.vs_row];
+    __syncwarp();
+    k_at[threadIdx.x] = k, v_at[threadIdx.x] = v;
+    __syncwarp();
+    using Unit = typename std::conditional<kAligned, uint4, uint8_t>::type;
+    for (int u0 = lane; u0 < many << shift; u0 += 32 * kAtOnce) {
+      Unit x[kAtOnce], y[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int u = u0 + j * 32, r = warp * 32 + (u >> shift), off = (u & (units - 1)) * kUnit;
+        if (u < many << shift && k_at[r].x >= 0) {
+          x[j] = *reinterpret_cast<const Unit*>(c.k + k_at[r].x + off);
+          y[j] = *reinterpret_cast<const Unit*>(c.v + v_at[r].x + off);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int u = u0 + j * 32, r = warp * 32 + (u >> shift), off = (u & (units - 1)) * kUnit;
+        if (u < many << shift && k_at[r].x >= 0) {
+          *reinterpret_cast<Unit*>(c.k + k_at[r].y + off) = x[j];
+          *reinterpret_cast<Unit*>(c.v + v_at[r].y + off) = y[j];
+        }
+      }
     }
   }
 }
@@ -295,35 +424,53 @@ int32_t most_moves(const kb_paged_cache& c, int32_t budget) {
   return (int32_t)(capacity <= budget ? 0 : kb_min_i32(budget, (int32_t)(capacity - budget)));
 }
 
+int launch_select(const EvictArgs& in, int32_t heads, int32_t B, cudaStream_t s) {
+  EvictArgs a = in;
+  const int32_t capacity = kb_max_i32(1, a.c.capacity);
+  a.cluster = 1;
+  while (a.cluster < kMostCluster && capacity > a.cluster * kBlockRows) a.cluster *= 2;
+  const bool held = capacity <= a.cluster * kBlockRows;
+  if (!held) a.cluster = 1;
+  cudaLaunchConfig_t c = {};
+  c.blockDim = dim3(held && a.cluster == 1 ? 32 * kb_cdiv_i32(capacity, kWarpRows) : 1024);
+  c.gridDim = dim3((unsigned)(heads * a.cluster), (unsigned)B);
+  c.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = a.cluster, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  c.attrs = &at, c.numAttrs = a.cluster > 1 ? 1 : 0;
+  KB_CUDA_TRY(held ? cudaLaunchKernelEx(&c, paged_select_kernel<true>, a) : cudaLaunchKernelEx(&c, paged_select_kernel<false>, a));
+  count_launch();
+  return KB_OK;
+}
+
 }  // namespace
 
 int paged_write(const kb_paged_write_params& p, cudaStream_t s) {
   const bool f8 = p.cache.dtype == KB_E4M3;
   if (!f8 && p.cache.dtype != p.dtype) return KB_ERR_UNSUPPORTED;
-  const int64_t rows = (int64_t)p.cache.B * p.cache.H_kv * p.T;
-  if (rows > (int64_t)1 << 30) return KB_ERR_TOO_LARGE;
+  if ((int64_t)p.cache.B * p.T > (int64_t)1 << 30) return KB_ERR_TOO_LARGE;
   WriteArgs a{};
   a.c = make_paged_view(p.cache);
   const kb_tensor4* x[2] = {&p.k, &p.v};
   const int elsize = dtype_size(p.dtype);
-  a.aligned = paged_rows_aligned(p.cache, dtype_size(p.cache.dtype));
+  bool aligned = paged_rows_aligned(p.cache, dtype_size(p.cache.dtype));
   for (int i = 0; i < 2; ++i) {
     a.x[i] = x[i]->data;
     a.sb[i] = x[i]->stride[0], a.sh[i] = x[i]->stride[1], a.st[i] = x[i]->stride[2], a.sd[i] = x[i]->stride[3];
-    a.aligned = a.aligned && a.sd[i] == 1 && reinterpret_cast<uintptr_t>(a.x[i]) % 16 == 0 && a.sb[i] * elsize % 16 == 0 && a.sh[i] * elsize % 16 == 0 &&
-                a.st[i] * elsize % 16 == 0;
+    aligned = aligned && a.sd[i] == 1 && reinterpret_cast<uintptr_t>(a.x[i]) % 16 == 0 && a.sb[i] * elsize % 16 == 0 && a.sh[i] * elsize % 16 == 0 &&
+              a.st[i] * elsize % 16 == 0;
   }
   a.new_lens = p.new_lens, a.new_lens_b = p.new_lens_stride;
   a.positions = p.positions, a.pos_b = p.positions_stride[0], a.pos_t = p.positions_stride[1];
   a.weights = p.weights, a.w_b = p.weights_stride[0], a.w_h = p.weights_stride[1];
   a.row_positions = p.row_positions, a.p_b = p.row_positions_stride[0], a.p_h = p.row_positions_stride[1];
   a.B = p.cache.B, a.H_kv = p.cache.H_kv, a.T = p.T, a.D = p.cache.D;
-  a.rows_per_cta = kWriteThreads / (a.D / kPerThread);
-  a.fd_T = kb_fastdiv_make(a.T), a.fd_H = kb_fastdiv_make(a.H_kv);
+  a.fd_T = kb_fastdiv_make(a.T);
   switch (p.dtype) {
-    case KB_F32: return launch_write<float>(a, f8, s);
-    case KB_F16: return launch_write<__half>(a, f8, s);
-    default: return launch_write<__nv_bfloat16>(a, f8, s);
+    case KB_F32: return launch_write<float>(a, f8, aligned, s);
+    case KB_F16: return launch_write<__half>(a, f8, aligned, s);
+    default: return launch_write<__nv_bfloat16>(a, f8, aligned, s);
   }
 }
 
@@ -343,19 +490,16 @@ int paged_evict(const kb_paged_evict_params& p, cudaStream_t s) {
   a.H_kv = c.H_kv, a.D = c.D, a.budget = p.budget, a.recent = p.recent;
   a.most_moves = most_moves(c, p.budget);
   a.elsize = dtype_size(c.dtype);
-  a.aligned = paged_rows_aligned(c, a.elsize);
   a.in_place = p.weights == p.weights_out;
   const size_t heads = (size_t)c.B * c.H_kv;
   a.counts = static_cast<int32_t*>(p.workspace);
   a.src = a.counts + heads;
   a.dst = a.src + heads * a.most_moves;
-  paged_select_kernel<<<dim3((unsigned)c.H_kv, (unsigned)c.B), kSelectThreads, 0, s>>>(a);
-  KB_LAUNCH_CHECK("paged_select_kernel");
-  // eight rows per block at a time; a few blocks per head are enough where there are many heads
-  const int64_t most = ((int64_t)a.most_moves + 7) / 8, want = kb_max_i32(1, (int32_t)((148 * 16 + heads - 1) / heads));
-  paged_move_kernel<<<dim3((unsigned)(most < want ? (most < 1 ? 1 : most) : want), (unsigned)c.H_kv, (unsigned)c.B), kMoveThreads, 0, s>>>(a);
-  KB_LAUNCH_CHECK("paged_move_kernel");
-  return KB_OK;
+  if (int rc = launch_select(a, c.H_kv, c.B, s)) return rc;
+  // 256 moves per block at a time; a few blocks per head are enough where there are many heads
+  const int64_t most = ((int64_t)a.most_moves + kMoveThreads - 1) / kMoveThreads, want = kb_max_i32(1, (int32_t)((148 * 8 + heads - 1) / heads));
+  const dim3 grid((unsigned)(most < want ? (most < 1 ? 1 : most) : want), (unsigned)c.H_kv, (unsigned)c.B);
+  return launch_after(paged_rows_aligned(c, a.elsize) ? paged_move_kernel<true> : paged_move_kernel<false>, grid, kMoveThreads, s, a);
 }
 
 }  // namespace kb

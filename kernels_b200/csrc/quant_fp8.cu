@@ -36,16 +36,6 @@ __device__ __forceinline__ uint32_t abs_bits_max(uint32_t m, float, uint32_t w) 
 template <typename T>
 __device__ __forceinline__ uint32_t abs_bits_max(uint32_t m, T, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }
 
-// x / scale rounded to nearest, with r = 1 / scale rounded to nearest: one Newton correction of x r by its exact
-// remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990: correctly
-// rounded where nothing underflows).  Here scale >= 1e-12 and quotients below 2^-11 become 0 whatever their last bit,
-// so the remainders that matter stay far above the smallest normal number; scale <= 1e37 keeps r normal.
-__device__ __forceinline__ float div_by(float x, float scale, float r) {
-  const float q = __fmul_rn(x, r);
-  const float d = __fmaf_rn(__fmaf_rn(-q, scale, x), r, q);
-  return __uint_as_float(__float_as_uint(d) | (__float_as_uint(x) & 0x80000000u));  // -0 keeps its sign
-}
-
 template <typename T>
 __global__ void __launch_bounds__(QuantTraits<T>::kThreads) quantize_fp8_tiles_kernel(const QuantArgs a) {
   constexpr int E = QuantTraits<T>::kElems, kThreads = QuantTraits<T>::kThreads, kVecsPerRow = kD / E;

@@ -138,12 +138,16 @@ def paged_attention(
     assert c.dtype == _lib.KB_E4M3 or q.dtype == k_pages.dtype, "q has the pages' type"
     assert context_size is None or context_size >= 1
     assert back_contexts >= 0
+    strides = q.stride()
+    if strides[2] != 1 or strides[0] % 2 or strides[1] % 2 or q.data_ptr() % 4:
+        q = q.contiguous()  # (the tensor-core kernel takes pairs of elements)
+        strides = q.stride()
     p = _lib.PagedAttentionParams()
     p.cache = c
     o = torch.empty((B, H, D), dtype=q.dtype, device=device)
     lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_lse or weights is not None else None
     p.q, p.o, p.lse = q.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None
-    p.q_stride[:] = q.stride()
+    p.q_stride[:] = strides
     if weights is not None:
         p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, device)
     p.H, p.dtype = H, _lib.dtype_code(q.dtype)

@@ -76,7 +76,7 @@ def test_call_refusals():
                            (dict(weights=4096, lse=4096, workspace=4100), BAD), (dict(cache=_cache(H_kv=0)), BAD)]:
         assert _attention(**change) == status, change
     assert _attention(H=0) == 0 and _attention(cache=_cache(B=0)) == 0
-    for change, status in [(dict(T=-1), BAD), (dict(dtype=_lib.KB_F32), UNSUPPORTED), (dict(dtype=3), UNSUPPORTED), (dict(T=1 << 29), TOO_LARGE)]:
+    for change, status in [(dict(T=-1), BAD), (dict(dtype=_lib.KB_F32), UNSUPPORTED), (dict(dtype=3), UNSUPPORTED), (dict(T=1 << 30), TOO_LARGE)]:
         assert _write(**change) == status, change
     assert _write(T=0) == 0 and _write(cache=_cache(B=0)) == 0 and _write(cache=_cache(M=0)) == 0
     for change, status in [(dict(budget=0), BAD), (dict(recent=-1), BAD), (dict(lens_out=None), BAD), (dict(weights=None), BAD), (dict(row_positions_out=None), BAD),

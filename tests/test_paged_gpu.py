@@ -404,7 +404,9 @@ def check_evict(c, w, pos, budget, recent, in_place=True):
     (2, 32, 16, [200, 90], F8, 128, 16),
     (1, 256, 16, [200, 90], F32, 64, 16),
     (2, 64, 16, [50, 60], F16, 10**9, 4),
-    (1, 64, 64, [40000], F16, 5000, 100),                   # longer than a block holds at a time
+    (1, 64, 64, [40000, 16385, 30], F16, 5000, 100),        # longer than a block holds, shorter than its cluster
+    (1, 16, 64, [140000, 100], F16, 70000, 0),              # longer than a cluster holds
+    (2, 16, 64, [20000, 8000], F16, 8100, 16),              # half of a cluster without rows
 ])
 @pytest.mark.parametrize("ties", [False, True])
 def test_evict_matches_definition(H_kv, D, page, lens, dtype, budget, recent, ties):
