@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
   const int32_t unit = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / kLanes, piece = lane % kLanes;
   if (threadIdx.x == 0 && !a.by_item) a.join[unit].x = -1;
+  let_next_launch_start();
   const Stretch stretch = find_stretch(a, unit, kRows);
   Place at = stretch.at;
   for (int64_t seen = 0; at.left > 0;) {
@@ -407,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, oct = lane >> 2;
   const int32_t unit = blockIdx.x * kWarps + warp;
   if (lane == 0 && unit < a.units && !a.by_item) a.join[unit].x = -1;
+  let_next_launch_start();
   const Stretch stretch = find_stretch(a, unit, kR);
   const uint32_t ring = sm100::smem_u32(smem) + warp * Tile::kWarpBytes;
 
@@ -708,17 +710,18 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
       }
     }
   }
-  let_next_launch_start();
   cp_async_wait<0>();
 }
 
 // ---- the parts of an item joined -----------------------------------------------------------------------------------------
 
-constexpr int kJoinThreads = 256;
+constexpr int kMostJoinThreads = 1024;
 
 // A block per item and head.  Groups of D / 4 threads take every so many-th part, four elements per thread; the groups are added up in order.
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendArgs a) {
-  __shared__ float red[kJoinThreads / 32], sums[kJoinThreads / 4], o_s[kJoinThreads * 4];
+__global__ void __launch_bounds__(kMostJoinThreads) paged_join_kernel(const AttendArgs a) {
+  __shared__ float red[kMostJoinThreads / 32], sums[kMostJoinThreads / 4], o_s[kMostJoinThreads * 4];
+  const int threads = blockDim.x;
+  let_next_launch_start();
   wait_for_launch_before();
   const int4 word = a.join[blockIdx.x];  // first part, its unit, last unit, item
   const int32_t g = blockIdx.y;
@@ -729,16 +732,15 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendAr
   const int32_t n = word.z - word.y + 1;
   auto part_at = [&](int32_t i) { return (int64_t)(i == 0 ? word.x : 2 * (word.y + i)) * a.heads + g; };
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kJoinThreads) top = fmaxf(top, a.part_ml[part_at(i)].x);
+  for (int i = threadIdx.x; i < n; i += threads) top = fmaxf(top, a.part_ml[part_at(i)].x);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[w]);
+  for (int w = 0; w < threads / 32; ++w) top = fmaxf(top, red[w]);
   const float base = top == -INFINITY ? 0.f : top;
 
-  const int width = a.D / 4, groups = kJoinThreads / width, group = threadIdx.x / width, d = (threadIdx.x - group * width) * 4;
+  const int width = a.D / 4, groups = threads / width, group = threadIdx.x / width, d = (threadIdx.x - group * width) * 4;
   float sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -753,7 +755,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendAr
   if (d == 0) sums[group] = sum;
   __syncthreads();
   const int64_t bh = (int64_t)b * a.H + h;
-  for (int i = threadIdx.x; i < a.D; i += kJoinThreads) {
+  for (int i = threadIdx.x; i < a.D; i += threads) {
     float s = 0.f, y = 0.f;
     for (int k = 0; k < groups; ++k) s += sums[k], y += o_s[k * a.D + i];
     store_any(a.o, bh * a.D + i, a.dtype, s == 0.f ? 0.f : y / s);
@@ -861,6 +863,7 @@ auto with_kernel(const kb_paged_attention_params& p, F f) {
 // What follows from the sizes alone (the lengths are on the device).
 struct Plan {
   int32_t heads, head_tiles, units, least, most_rows;
+  int64_t items;
   bool by_item, joins;
   size_t join_bytes, part_bytes, ml_bytes, score_bytes;
 };
@@ -874,7 +877,7 @@ Plan make_plan(const kb_paged_attention_params& p) {
   n.least = K::kLeast;
   const int64_t capacity = (int64_t)c.M * c.page, window = p.context_size > 0 ? ((int64_t)p.back_contexts + 1) * p.context_size : capacity;
   n.most_rows = (int32_t)(window < capacity ? window : capacity);
-  const int64_t items = (int64_t)c.B * c.H_kv * n.head_tiles, tiles = (n.most_rows + K::kRows - 1) / K::kRows;
+  const int64_t items = n.items = (int64_t)c.B * c.H_kv * n.head_tiles, tiles = (n.most_rows + K::kRows - 1) / K::kRows;
   const int64_t stretches = (items * (tiles < 1 ? 1 : tiles) + K::kLeast - 1) / K::kLeast;
   n.units = (int32_t)(stretches < K::kUnits ? stretches : K::kUnits);
   n.by_item = items <= n.units;
@@ -921,7 +924,10 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
     if (int rc = kernel.launch(a, paged_rows_aligned(c, dtype_size(c.dtype)), s)) return rc;
     if (n.joins) {
       const dim3 grid((unsigned)(n.join_bytes / sizeof(int4)), kb_min_i32(n.heads, a.group));
-      if (int rc = launch_after(paged_join_kernel, grid, kJoinThreads, s, a)) return rc;
+      // a group of D / 4 threads for about every part of an item
+      int32_t threads = 128;
+      while (threads < kMostJoinThreads && threads < (int64_t)n.units / n.items * (c.D / 4)) threads *= 2;
+      if (int rc = launch_after(paged_join_kernel, grid, threads, s, a)) return rc;
     }
     if (p.weights) {
       const int32_t blocks = kb_cdiv_i32(n.most_rows, 256), fill = kb_max_i32(1, kSms * 16 / (c.B * c.H_kv));

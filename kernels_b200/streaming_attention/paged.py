@@ -29,37 +29,50 @@ from .kernel import _clamp_i32
 
 
 def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
-    """The checked cache as the C ABI's structure."""
+    """The checked cache as the C ABI's structure, and its device's index.  (A few microseconds of calls that take about twelve: every
+    property of a tensor is asked for once, devices by their index.)"""
     if not (k_pages.is_cuda and v_pages.is_cuda):
         raise RuntimeError(f"{what}: the tensors must live on a CUDA device (there is no CPU path)")
-    device, f8 = k_pages.device, k_pages.dtype == torch.float8_e4m3fn
-    assert k_pages.ndim == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype, "k_pages and v_pages are [P, H_kv, page, D]"
-    assert v_pages.device == page_table.device == lens.device == device
-    P, H_kv, page, D = k_pages.shape
-    assert page >= 1 and (k_pages.numel() == 0 or (k_pages.stride(3) == 1 and v_pages.stride(3) == 1)), "rows of the pages are dense"
-    assert page_table.ndim == 2 and page_table.dtype == torch.int32 and lens.ndim == 1 and lens.dtype == torch.int32
-    assert page_table.shape[0] == lens.shape[0], "one table row and one length per sequence"
+    index, shape, dtype = k_pages.get_device(), k_pages.shape, k_pages.dtype
+    assert len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype, "k_pages and v_pages are [P, H_kv, page, D]"
+    assert v_pages.get_device() == page_table.get_device() == lens.get_device() == index
+    P, H_kv, page, D = shape
+    ks, vs = k_pages.stride(), v_pages.stride()
+    assert page >= 1 and (ks[3] == vs[3] == 1 or 0 in shape), "rows of the pages are dense"
+    table_shape, lens_shape = page_table.shape, lens.shape
+    assert len(table_shape) == 2 and len(lens_shape) == 1 and page_table.dtype == lens.dtype == torch.int32
+    B, M = table_shape
+    assert lens_shape[0] == B, "one table row and one length per sequence"
+    f8 = dtype == torch.float8_e4m3fn
     assert (k_scale is not None) == (v_scale is not None) == f8, "8-bit pages, and only those, come with scales"
     c = _lib.PagedCache()
     c.k, c.v = k_pages.data_ptr(), v_pages.data_ptr()
-    c.k_stride[:], c.v_stride[:] = k_pages.stride()[:3], v_pages.stride()[:3]
+    c.k_stride[:], c.v_stride[:] = ks[:3], vs[:3]
     if f8:
-        assert k_scale.shape == v_scale.shape == (P, H_kv, page) and k_scale.dtype == v_scale.dtype == torch.float32
-        assert k_scale.device == v_scale.device == device
+        assert k_scale.shape == v_scale.shape == shape[:3] and k_scale.dtype == v_scale.dtype == torch.float32
+        assert k_scale.get_device() == v_scale.get_device() == index
         c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
         c.k_scale_stride[:], c.v_scale_stride[:] = k_scale.stride(), v_scale.stride()
     c.page_table, c.lens, c.lens_stride = page_table.data_ptr(), lens.data_ptr(), lens.stride(0)
     c.table_stride[:] = page_table.stride()
-    c.B, c.H_kv, c.D, c.P, c.M, c.page = lens.shape[0], H_kv, D, P, page_table.shape[1], page
-    c.dtype = _lib.KB_E4M3 if f8 else _lib.dtype_code(k_pages.dtype)
-    return c
+    c.B, c.H_kv, c.D, c.P, c.M, c.page = B, H_kv, D, P, M, page
+    c.dtype = _lib.KB_E4M3 if f8 else _lib.dtype_code(dtype)
+    return c, index
 
 
-def _per_row(name, x, dtype, c, device):
+def _per_row(name, x, dtype, c, index):
     """Pointer and strides of ``weights`` or ``row_positions``."""
-    assert x.dtype == dtype and x.device == device and x.ndim == 3 and x.shape[:2] == (c.B, c.H_kv), f"{name} is [B, H_kv, M * page]"
-    assert x.shape[2] >= c.M * c.page and (x.stride(2) == 1 or x.shape[2] <= 1), f"{name} has an entry for every row, side by side"
-    return x.data_ptr(), x.stride()[:2]
+    shape, strides = x.shape, x.stride()
+    assert x.dtype == dtype and x.get_device() == index and len(shape) == 3 and shape[0] == c.B and shape[1] == c.H_kv, f"{name} is [B, H_kv, M * page]"
+    assert shape[2] >= c.M * c.page and (strides[2] == 1 or shape[2] <= 1), f"{name} has an entry for every row, side by side"
+    return x.data_ptr(), strides[:2]
+
+
+def _workspace(p, n, like):
+    """``n`` bytes on the device of ``like`` (int32); the caller holds them until the launch has been made."""
+    w = like.new_empty((n + 3) // 4)
+    p.workspace, p.workspace_bytes = w.data_ptr(), n
+    return w
 
 
 def paged_cache_write(
@@ -84,28 +97,28 @@ def paged_cache_write(
     0, those of ``row_positions`` the tokens' ``positions`` (int32 ``[B, T]``, None for the rows themselves).  Rows outside the table
     are dropped; two tokens of one call must not share a row of a page.
     """
-    c = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale)
-    device = k_pages.device
-    assert k.ndim == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device == device
-    T = k.shape[2]
-    assert k.shape[0] == c.B and k.shape[1] == c.H_kv and k.shape[3] == c.D, "k and v are [B, H_kv, T, D]"
-    assert c.dtype == _lib.KB_E4M3 or k.dtype == k_pages.dtype, "k and v have the pages' type"
+    c, index = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale)
+    shape, dtype = k.shape, k.dtype
+    assert len(shape) == 4 and v.shape == shape and v.dtype == dtype and k.get_device() == v.get_device() == index
+    B, H_kv, T, D = shape
+    assert B == c.B and H_kv == c.H_kv and D == c.D, "k and v are [B, H_kv, T, D]"
+    assert k_scale is not None or dtype == k_pages.dtype, "k and v have the pages' type"
     p = _lib.PagedWriteParams()
     p.cache = c
     p.k, p.v = _lib.tensor4(k), _lib.tensor4(v)
-    p.T, p.dtype = T, _lib.dtype_code(k.dtype)
+    p.T, p.dtype = T, _lib.dtype_code(dtype)
     if new_lens is not None:
-        assert new_lens.shape == lens.shape and new_lens.dtype == torch.int32 and new_lens.device == device
+        assert new_lens.shape == lens.shape and new_lens.dtype == torch.int32 and new_lens.get_device() == index
         p.new_lens, p.new_lens_stride = new_lens.data_ptr(), new_lens.stride(0)
     if positions is not None:
-        assert positions.shape == (c.B, T) and positions.dtype == torch.int32 and positions.device == device
+        assert positions.shape == (B, T) and positions.dtype == torch.int32 and positions.get_device() == index
         p.positions = positions.data_ptr()
         p.positions_stride[:] = positions.stride()
     if weights is not None:
-        p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, device)
+        p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, index)
     if row_positions is not None:
-        p.row_positions, p.row_positions_stride[:] = _per_row("row_positions", row_positions, torch.int32, c, device)
-    _lib.check(_lib.launch(_lib.load().kb_paged_write, p, device), "kb_paged_write")
+        p.row_positions, p.row_positions_stride[:] = _per_row("row_positions", row_positions, torch.int32, c, index)
+    _lib.check(_lib.launch(_lib.load().kb_paged_write, p, k_pages.device), "kb_paged_write")
 
 
 def paged_attention(
@@ -130,12 +143,13 @@ def paged_attention(
     no row.  With ``weights``, the softmax weight of every row that is seen, summed over the query heads of its key/value
     head, is added to ``weights`` in place.
     """
-    c = _pages("paged_attention", k_pages, v_pages, page_table, lens, k_scale, v_scale)
-    device = k_pages.device
-    assert q.ndim == 3 and q.shape[0] == c.B and q.shape[2] == c.D and q.device == device, "q is [B, H, D]"
-    B, H, D = q.shape
+    c, index = _pages("paged_attention", k_pages, v_pages, page_table, lens, k_scale, v_scale)
+    shape, dtype = q.shape, q.dtype
+    assert len(shape) == 3 and q.get_device() == index, "q is [B, H, D]"
+    B, H, D = shape
+    assert B == c.B and D == c.D, "q is [B, H, D]"
     assert c.H_kv >= 1 and H % c.H_kv == 0, "query heads share the key/value heads evenly"
-    assert c.dtype == _lib.KB_E4M3 or q.dtype == k_pages.dtype, "q has the pages' type"
+    assert k_scale is not None or dtype == k_pages.dtype, "q has the pages' type"
     assert context_size is None or context_size >= 1
     assert back_contexts >= 0
     strides = q.stride()
@@ -144,21 +158,22 @@ def paged_attention(
         strides = q.stride()
     p = _lib.PagedAttentionParams()
     p.cache = c
-    o = torch.empty((B, H, D), dtype=q.dtype, device=device)
-    lse = torch.empty((B, H), dtype=torch.float32, device=device) if return_lse or weights is not None else None
-    p.q, p.o, p.lse = q.data_ptr(), o.data_ptr(), lse.data_ptr() if lse is not None else None
+    o = q.new_empty(shape)
+    lse = lens.new_empty((B, H), dtype=torch.float32) if return_lse or weights is not None else None
+    p.q, p.o = q.data_ptr(), o.data_ptr()
     p.q_stride[:] = strides
+    if lse is not None:
+        p.lse = lse.data_ptr()
     if weights is not None:
-        p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, device)
-    p.H, p.dtype = H, _lib.dtype_code(q.dtype)
-    p.context_size, p.back_contexts = 0 if context_size is None else _clamp_i32(context_size), _clamp_i32(back_contexts)
+        p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, index)
+    p.H, p.dtype = H, _lib.dtype_code(dtype)
+    if context_size is not None:
+        p.context_size, p.back_contexts = _clamp_i32(context_size), _clamp_i32(back_contexts)
     p.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     lib = _lib.load()
-    p.workspace_bytes = lib.kb_paged_attention_workspace_bytes(p)
-    if p.workspace_bytes:
-        workspace = torch.empty(p.workspace_bytes, dtype=torch.uint8, device=device)
-        p.workspace = workspace.data_ptr()
-    _lib.check(_lib.launch(lib.kb_paged_attention, p, device), "kb_paged_attention")
+    workspace = _workspace(p, lib.kb_paged_attention_workspace_bytes(p), lens)
+    _lib.check(_lib.launch(lib.kb_paged_attention, p, k_pages.device), "kb_paged_attention")
+    del workspace
     return (o, lse) if return_lse else o
 
 
@@ -186,8 +201,7 @@ def paged_cache_evict(
     ``out``: a ``(lens, weights, row_positions)`` to be written instead, not overlapping the given ones (entries of
     the rows that remain; the pages change all the same).  Sequences that share pages need copies of their own first.
     """
-    c = _pages("paged_cache_evict", k_pages, v_pages, page_table, lens, k_scale, v_scale)
-    device = k_pages.device
+    c, index = _pages("paged_cache_evict", k_pages, v_pages, page_table, lens, k_scale, v_scale)
     assert budget >= 1 and recent >= 0, "at least one row stays"
     p = _lib.PagedEvictParams()
     p.cache = c
@@ -195,16 +209,14 @@ def paged_cache_evict(
     if out is None:
         out = (lens, weights, row_positions)
     else:
-        assert len(out) == 3 and out[0].shape == lens.shape and out[0].dtype == torch.int32 and out[0].device == device
+        assert len(out) == 3 and out[0].shape == lens.shape and out[0].dtype == torch.int32 and out[0].get_device() == index
     p.lens_out, p.lens_out_stride = out[0].data_ptr(), out[0].stride(0)
-    p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, device)
-    p.row_positions, p.row_positions_stride[:] = _per_row("row_positions", row_positions, torch.int32, c, device)
-    p.weights_out, p.weights_out_stride[:] = _per_row("out[1]", out[1], torch.float32, c, device)
-    p.row_positions_out, p.row_positions_out_stride[:] = _per_row("out[2]", out[2], torch.int32, c, device)
+    p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, index)
+    p.row_positions, p.row_positions_stride[:] = _per_row("row_positions", row_positions, torch.int32, c, index)
+    p.weights_out, p.weights_out_stride[:] = _per_row("out[1]", out[1], torch.float32, c, index)
+    p.row_positions_out, p.row_positions_out_stride[:] = _per_row("out[2]", out[2], torch.int32, c, index)
     lib = _lib.load()
-    p.workspace_bytes = lib.kb_paged_evict_workspace_bytes(p)
-    if p.workspace_bytes:
-        workspace = torch.empty(p.workspace_bytes, dtype=torch.uint8, device=device)
-        p.workspace = workspace.data_ptr()
-    _lib.check(_lib.launch(lib.kb_paged_evict, p, device), "kb_paged_evict")
+    workspace = _workspace(p, lib.kb_paged_evict_workspace_bytes(p), lens)
+    _lib.check(_lib.launch(lib.kb_paged_evict, p, k_pages.device), "kb_paged_evict")
+    del workspace
     return out

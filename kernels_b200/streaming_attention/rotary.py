@@ -19,20 +19,20 @@ from .. import _lib
 
 
 def _rotate(q, k, positions, inv_freq, ends, inverse):
-    B, H, T, D = q.shape
     p = _lib.RotaryParams()
-    q_out = torch.empty((B, H, T, D), dtype=q.dtype, device=q.device)
+    shape = q.shape
+    q_out, k_out = q.new_empty(shape), None
     p.q, p.q_out = _lib.tensor4(q), q_out.data_ptr()
-    k_out = None
+    p.B, p.H, p.T, p.D = shape
     if k is not None:
-        k_out = torch.empty((B, k.shape[1], T, D), dtype=q.dtype, device=q.device)
-        p.k, p.k_out, p.H_kv = _lib.tensor4(k), k_out.data_ptr(), k.shape[1]
-        if k.numel() == 0:
-            p.k.data = None
+        k_shape = k.shape
+        k_out = k.new_empty(k_shape)
+        if 0 not in k_shape:
+            p.k, p.k_out, p.H_kv = _lib.tensor4(k), k_out.data_ptr(), k_shape[1]
     p.positions, p.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
     strides = positions.stride()
     p.pos_stride[:] = strides if len(strides) == 3 else (strides[0], 0, strides[1])
-    p.B, p.H, p.T, p.D, p.R, p.axes = B, H, T, D, ends[-1], len(ends)
+    p.R, p.axes = ends[-1], len(ends)
     p.section_end[: len(ends)] = ends
     p.pos64 = positions.dtype == torch.int64
     p.dtype = _lib.dtype_code(q.dtype)
@@ -75,17 +75,24 @@ def rotary_embedding(
     """
     if not q.is_cuda:
         raise RuntimeError("rotary_embedding: the tensors must live on a CUDA device (there is no CPU path)")
-    assert q.ndim == 4 and positions.ndim in (2, 3) and inv_freq.ndim == 1
-    B, _, T, D = q.shape
+    shape, pos_shape, index, dtype = q.shape, positions.shape, q.get_device(), q.dtype
+    assert len(shape) == 4 and len(pos_shape) in (2, 3), "q is [B, H, T, D], positions are [A, T] or [A, B, T]"
+    B, _, T, D = shape
     if k is not None:
-        assert k.ndim == 4 and k.shape[0] == B and k.shape[2] == T and k.shape[3] == D and k.dtype == q.dtype and k.device == q.device
-    assert positions.dtype in (torch.int32, torch.int64) and positions.device == q.device
-    assert positions.shape[1:] == ((T,) if positions.ndim == 2 else (B, T)), "positions are [A, T] or [A, B, T]"
-    assert inv_freq.dtype == torch.float64 and inv_freq.device == q.device and 1 <= inv_freq.shape[0] <= D // 2
-    sections = (inv_freq.shape[0],) if sections is None else tuple(int(n) for n in sections)
-    assert 1 <= len(sections) <= 8 and len(sections) == positions.shape[0], "one section of frequencies per axis, at most 8"
-    assert min(sections) >= 0 and sum(sections) == inv_freq.shape[0], "the sections share out inv_freq"
-    ends = [sum(sections[: a + 1]) for a in range(len(sections))]
+        k_shape = k.shape
+        assert len(k_shape) == 4 and k_shape[0] == B and k_shape[2] == T and k_shape[3] == D and k.dtype == dtype and k.get_device() == index
+    assert positions.dtype in (torch.int32, torch.int64) and positions.get_device() == index
+    assert pos_shape[-1] == T and (len(pos_shape) == 2 or pos_shape[1] == B), "positions are [A, T] or [A, B, T]"
+    assert inv_freq.ndim == 1 and inv_freq.dtype == torch.float64 and inv_freq.get_device() == index
+    R = inv_freq.shape[0]
+    assert 1 <= R <= D // 2, "as many frequencies as there are pairs, at most"
+    sections = (R,) if sections is None else sections
+    ends, end = [], 0
+    for n in sections:
+        end += int(n)
+        ends.append(end)
+    assert 1 <= len(ends) <= 8 and len(ends) == pos_shape[0], "one section of frequencies per axis, at most 8"
+    assert end == R and min(sections) >= 0, "the sections share out inv_freq"
     inv_freq = inv_freq.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryEmbedding.apply(q, k, positions, inv_freq, ends, False)
