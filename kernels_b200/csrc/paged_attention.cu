@@ -44,6 +44,7 @@ struct AttendArgs {
   float2* part_ml;  // [2 units, heads]
   float* scores;    // [B, H, capacity], base-2 logits
   KbFastDiv fd_context;
+  uint32_t row16[3], scale_at[3];  // tensor-core kernel: page, head and row strides of keys and values in 16 bytes, of their scales in elements
 };
 
 // The rows that the token sees: [first, end).
@@ -98,6 +99,7 @@ __device__ __forceinline__ int64_t warp_sum(int64_t x) {
 struct Stretch {
   Place at;           // left 0: nothing to do
   int64_t begin, each;  // the unit's first tile, and tiles per unit
+  bool whole;           // instead of that: an item per unit
 };
 
 // Found by a whole warp.  `rows`: of a tile.
@@ -106,13 +108,28 @@ __device__ __forceinline__ Stretch find_stretch(const AttendArgs& a, int32_t uni
   const int64_t per_seq = (int64_t)a.H_kv * a.head_tiles;
   Place p{};
   int64_t total = 0;
+  int32_t longest = 0;
   for (p.b = lane; p.b < a.B; p.b += 32) {
     p.enter(a, rows);
     total += p.tiles;
+    longest = max(longest, p.tiles);
   }
   total = warp_sum(total) * per_seq;
+  longest = __reduce_max_sync(0xffffffffu, longest);
   Stretch s;
   s.each = total < (int64_t)a.units * a.least_tiles ? a.least_tiles : (total + a.units - 1) / a.units;
+  // Items of much the same length, one for a unit: taken whole they need no joining, which costs more than an uneven share.
+  // (64 sequences with windows of 513 to 640 rows, 16 heads: KB_ALIGNED us, and KB_SHARED us with shares of 16 tiles.)
+  s.whole = a.by_item && 4 * (int64_t)longest <= 5 * s.each;
+  if (s.whole) {
+    const bool there = unit < a.B * per_seq;
+    s.at = p;
+    s.at.b = there ? (int32_t)(unit / per_seq) : 0, s.at.hy = there ? (int32_t)(unit - s.at.b * per_seq) : 0, s.at.tile = 0;
+    s.at.enter(a, rows);
+    s.at.left = there ? s.at.tiles : 0;
+    s.begin = 0;
+    return s;
+  }
   s.begin = unit * s.each;
   p.left = s.begin >= total ? 0 : min(s.each, total - s.begin);
   if (p.left) {
@@ -324,11 +341,11 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
 
 // ---- tensor-core kernel ----------------------------------------------------------------------------------------------
 //
-// 16-bit and e4m3 caches of head dim 64 and 128.  A warp multiplies the 16 (or 8) query heads of a block with 16 keys at a time
-// (m16n8k16): the heads are the rows, so up to 16 heads cost what one does, and what the tensor cores have to do is a
-// small part of the time that the keys take to arrive.  That time is all there is to hide, and every warp hides it for itself: it
-// is a unit with a ring of kStages tiles of kR rows in shared memory, filled by 16-byte asynchronous copies that run on from one item
-// into the next, and it never waits for another warp.
+// 16-bit and e4m3 caches of head dim 64 and 128.  Sixteen keys are the rows of a product (m16n8k16) and eight query heads its
+// columns: S^T = K Q^T, then O^T += V^T P^T with the weights turned over in registers.  So up to eight heads cost what one does, and what
+// the tensor cores have to do is a small part of the time that the keys take to arrive.  That time is all there is to hide, and
+// every warp hides it for itself: it is a unit with a ring of kStages tiles of kR rows in shared memory, filled by 16-byte
+// asynchronous copies that run on from one item into the next, and it never waits for another warp.
 //
 // Rows are found one by one (a lane looks up a row), so pages of any size and order are read the same way; a row that is
 // masked is filled with zeros without being read, so that nothing in it can reach a sum.
@@ -355,54 +372,58 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
 __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-// c += a b, 16 x 8 x 16; with HALF the rows 8 .. 15 are not there
-template <bool BF16, bool HALF>
-__device__ __forceinline__ void mma16(float (&c)[HALF ? 2 : 4], const uint32_t (&a)[HALF ? 2 : 4], uint32_t b0, uint32_t b1) {
-  float x2, x3;
-  if constexpr (HALF) {
-    if constexpr (BF16)
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %8, %5, %8}, {%6, %7}, {%0, %1, %9, %9};"
-          : "+f"(c[0]), "+f"(c[1]), "=f"(x2), "=f"(x3) : "r"(a[0]), "r"(a[1]), "r"(b0), "r"(b1), "r"(0), "f"(0.f));
-    else
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %8, %5, %8}, {%6, %7}, {%0, %1, %9, %9};"
-          : "+f"(c[0]), "+f"(c[1]), "=f"(x2), "=f"(x3) : "r"(a[0]), "r"(a[1]), "r"(b0), "r"(b1), "r"(0), "f"(0.f));
-  } else {
-    if constexpr (BF16)
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
+__device__ __forceinline__ void lds4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t at) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+// an 8 x 8 matrix of 16-bit elements, a row per four lanes, turned over
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// c += a b, 16 x 8 x 16
+template <bool BF16>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 // four e4m3 to two pairs of f16
 __device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t four, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 
-// kF8: e4m3 cache (products in f16); kBf16: products in bf16, otherwise in f16; kHalf: at most eight query heads per item
-template <bool kF8, bool kBf16, int kD, bool kHalf>
+// kF8: e4m3 cache (products in f16); kBf16: products in bf16, otherwise in f16; kN: eights of query heads per item
+template <bool kF8, bool kBf16, int kD, int kN>
 struct MmaTile {
   static constexpr int kRowBytes = kF8 ? kD : 2 * kD, kChunks = kRowBytes / 16;
-  static constexpr int kR = kRowBytes == 256 ? 16 : 32;        // rows of a tile
-  static constexpr int kStages = kRowBytes == 256 ? 2 : kRowBytes == 64 ? 4 : 3;
+  static constexpr int kR = kRowBytes == 256 ? 16 : 32;  // rows of a tile
+  static constexpr int kStages = kRowBytes == 256 ? 2 : kRowBytes == 128 ? 3 : 4;
   static constexpr int kScaleBytes = kF8 ? 2 * kR * 4 : 0;
   static constexpr int kStageBytes = 2 * kR * kRowBytes + kScaleBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
-  static constexpr int kHeads = kHalf ? 8 : 16, kS = kHalf ? 1 : 2;  // kS: heads per thread
+  static constexpr int kHeads = 8 * kN;
   static constexpr int kSmem = kWarps * kWarpBytes;
-  static constexpr int kBlocks = kRowBytes == 256 && kHalf ? 3 : 2;      // per SM
+  static constexpr int kBlocks = kRowBytes == 256 && kN == 1 ? 3 : 2;  // per SM: what shared memory and registers allow
   static_assert(kStageBytes % 128 == 0, "matrix loads address a tile by exclusive or");
   // Where chunk c of row r lies: at c ^ swizzle(r).  The eight rows of a matrix load hit different banks, and so do the two rows
   // and four chunks of a 16-byte load of e4m3 keys.
   static __device__ __forceinline__ int swizzle(int r) { return !kF8 ? r & 7 : kD == 128 ? ((r & 1) << 2) | ((r >> 1) & 3) : (r >> 1) & 3; }
 };
 
-template <bool kF8, bool kBf16, int kD, bool kHalf>
-__global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlocks) paged_attend_mma_kernel(const AttendArgs a) {
-  using Tile = MmaTile<kF8, kBf16, kD, kHalf>;
-  constexpr int kR = Tile::kR, kStages = Tile::kStages, kChunks = Tile::kChunks, kRowBytes = Tile::kRowBytes, kHeads = Tile::kHeads, kS = Tile::kS;
-  constexpr int kSteps = kD / 16, kNt = kR / 8, kDt = kD / 8, kA = 2 * kS;
+template <bool kF8, bool kBf16, int kD, int kN>
+__global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks) paged_attend_mma_kernel(const AttendArgs a) {
+  using Tile = MmaTile<kF8, kBf16, kD, kN>;
+  constexpr int kR = Tile::kR, kStages = Tile::kStages, kChunks = Tile::kChunks, kRowBytes = Tile::kRowBytes, kHeads = Tile::kHeads;
+  constexpr int kSteps = kD / 16, kU = kR / 16, kDt = kD / 16;
   constexpr float kOffset = kBf16 ? 0.f : 7.f, kSlack = 8.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, oct = lane >> 2;
@@ -413,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
   const uint32_t ring = sm100::smem_u32(smem) + warp * Tile::kWarpBytes;
 
   // ---- copies: lane r looks up row r of a tile, a tile ahead of its copy
-  constexpr int kElem = kF8 ? 1 : 2, kRowsAtOnce = 32 / kChunks;
+  constexpr int kRowsAtOnce = 32 / kChunks;
   const int chunk = lane % kChunks, sub = lane / kChunks;
   const char *kfrom = a.c.k + chunk * 16, *vfrom = a.c.v + chunk * 16;
   const uint32_t place = sub * kRowBytes + ((chunk ^ Tile::swizzle(sub)) * 16);
@@ -429,9 +450,9 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
   };
   uint32_t live_bits[kStages - 1];  // of the tiles in the ring, oldest first
   auto issue = [&](int stage) -> uint32_t {
-    const int32_t page = next_page, at = next_at, head = next_head;
-    const uint32_t row16 = page >= 0 ? (uint32_t)((uint64_t)((page * a.c.k_page + head * a.c.k_head + at * a.c.k_row) * kElem) >> 4) : 0;
-    const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
+    const bool have = next_page >= 0;
+    const uint32_t row16 = have ? next_page * a.row16[0] + next_head * a.row16[1] + next_at * a.row16[2] : 0u;
+    const uint32_t live = __ballot_sync(0xffffffffu, have);
     const uint32_t to = ring + stage * Tile::kStageBytes;
 #pragma unroll
     for (int i = 0; i < kR / kRowsAtOnce; ++i) {
@@ -442,10 +463,10 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
       cp_async16(there + kR * kRowBytes, vfrom + off, ok);
     }
     if constexpr (kF8) {
-      const int64_t so = page >= 0 ? page * a.c.ks_page + head * a.c.ks_head + at * a.c.ks_row : 0;
+      const uint32_t at = have ? next_page * a.scale_at[0] + next_head * a.scale_at[1] + next_at * a.scale_at[2] : 0u;
       if (lane < kR) {
-        cp_async4(to + 2 * kR * kRowBytes + lane * 4, a.c.k_scale + so, page >= 0);
-        cp_async4(to + 2 * kR * kRowBytes + kR * 4 + lane * 4, a.c.v_scale + so, page >= 0);
+        cp_async4(to + 2 * kR * kRowBytes + lane * 4, a.c.k_scale + at, have);
+        cp_async4(to + 2 * kR * kRowBytes + kR * 4 + lane * 4, a.c.v_scale + at, have);
       }
     }
     look_up();
@@ -460,9 +481,9 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
   }
 
   // where this lane's matrix loads start in a tile; chunks and keys further on are an exclusive or and an offset away
-  const int kkey = kF8 ? oct : (lane & 7) + (lane >> 4) * 8, vkey = lane & 15;
-  const uint32_t kplace = kkey * kRowBytes + (((kF8 ? quad : (lane >> 3) & 1) ^ Tile::swizzle(kkey)) * 16);
-  const uint32_t vplace = (kR + vkey) * kRowBytes + (((lane >> 4) ^ Tile::swizzle(vkey)) * 16);
+  const int kkey = kF8 ? oct : lane & 15, vkey = kF8 ? lane & 15 : (lane & 7) + (lane >> 4) * 8;
+  const uint32_t kplace = kkey * kRowBytes + (((kF8 ? quad : lane >> 4) ^ Tile::swizzle(kkey)) * 16);
+  const uint32_t vplace = (kR + vkey) * kRowBytes + (((kF8 ? lane >> 4 : (lane >> 3) & 1) ^ Tile::swizzle(vkey)) * 16);
   int stage = 0;
   Place now = stretch.at;
   for (int64_t seen = 0; now.left > 0;) {
@@ -474,52 +495,60 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
     now.advance(a, kR, n);
     seen += n;
 
-    // ---- q as the products' left operand; with an e4m3 cache a lane's elements are the ones its 16-byte key loads hold
-    uint32_t q[kSteps][kA];
-    float back_scale[kS];
+    // ---- q as the products' right operand: lane (oct, quad) has elements of head oct; with an e4m3 cache the ones that its 16-byte key loads hold
+    uint32_t q[kSteps][kN][2];
+    float back_scale[kF8 ? kN : 1][2];  // of heads 2 quad and 2 quad + 1, as the scores lie
 #pragma unroll
-    for (int s = 0; s < kS; ++s) {
-      const int g = oct + 8 * s;
+    for (int e = 0; e < kN; ++e) {
+      const int g = oct + 8 * e;
       const uint16_t* from = static_cast<const uint16_t*>(a.q) + b * a.q_b + (int64_t)(h0 + (g < heads ? g : 0)) * a.q_h;
-      back_scale[s] = a.scale_log2;
 #pragma unroll
       for (int t = 0; t < kSteps; ++t)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int d = kF8 ? t / 4 * 64 + quad * 16 + t % 4 * 4 + 2 * p : t * 16 + 8 * p + quad * 2;
-          q[t][p * kS + s] = g < heads ? __ldg(reinterpret_cast<const uint32_t*>(from + d)) : 0u;
+          q[t][e][p] = g < heads ? __ldg(reinterpret_cast<const uint32_t*>(from + d)) : 0u;
         }
-      if (kF8 && a.dtype == KB_BF16) {
-        // (bf16 magnitudes without their signs order like whole numbers; what is not a number stays above)
-        uint32_t most = 0;
+      if constexpr (kF8) {
+        float down = a.scale_log2;
+        if (a.dtype == KB_BF16) {
+          // (bf16 magnitudes without their signs order like whole numbers; what is not a number stays above)
+          uint32_t most = 0;
 #pragma unroll
-        for (int t = 0; t < kSteps; ++t)
+          for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-          for (int p = 0; p < 2; ++p) most = __vmaxu2(most, q[t][p * kS + s] & 0x7fff7fffu);
-        most = max(most & 0xffffu, most >> 16);
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int e = (int)(most >> 7) - 127;  // the largest lies in [2^e, 2^(e + 1))
-        const int by = most == 0 || e == 128 ? 0 : max(-100, min(100, 14 - e));
-        const float up = __uint_as_float((uint32_t)(by + 127) << 23);
-        back_scale[s] *= __uint_as_float((uint32_t)(127 - by) << 23);
+            for (int p = 0; p < 2; ++p) most = __vmaxu2(most, q[t][e][p] & 0x7fff7fffu);
+          most = max(most & 0xffffu, most >> 16);
+          most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          const int x = (int)(most >> 7) - 127;  // the largest lies in [2^x, 2^(x + 1))
+          const int by = most == 0 || x == 128 ? 0 : max(-100, min(100, 14 - x));
+          const float up = __uint_as_float((uint32_t)(by + 127) << 23);
+          down *= __uint_as_float((uint32_t)(127 - by) << 23);
 #pragma unroll
-        for (int t = 0; t < kSteps; ++t)
+          for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const uint32_t w = q[t][p * kS + s];
-            q[t][p * kS + s] = sm100::pack_f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
-          }
+            for (int p = 0; p < 2; ++p) {
+              const uint32_t w = q[t][e][p];
+              q[t][e][p] = sm100::pack_f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) back_scale[e][i] = __shfl_sync(0xffffffffu, down, (quad * 2 + i) * 4);
       }
     }
 
-    float o[kDt][kA], m[kS], l[kS];
+    // element (2 r + i) of a product's lane: key (or element of the head) oct + 8 r, query head 2 quad + i
+    float o[kDt][kN][4], m[kN][2], l[kN][2];
 #pragma unroll
-    for (int s = 0; s < kS; ++s) m[s] = -INFINITY, l[s] = 0.f;
+    for (int e = 0; e < kN; ++e) {
 #pragma unroll
-    for (int j = 0; j < kDt; ++j)
+      for (int i = 0; i < 2; ++i) m[e][i] = -INFINITY, l[e][i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < kA; ++i) o[j][i] = 0.f;
+      for (int j = 0; j < kDt; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[j][e][i] = 0.f;
+    }
 
     for (int32_t i_tile = 0; i_tile < n; ++i_tile, r0 += kR) {
       cp_async_wait<kStages - 2>();
@@ -533,140 +562,143 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
       cp_async_commit();
 
       // scores
-      float sc[kNt][kA];
+      float sc[kU][kN][4];
 #pragma unroll
-      for (int j = 0; j < kNt; ++j)
+      for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int i = 0; i < kA; ++i) sc[j][i] = 0.f;
+        for (int e = 0; e < kN; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[u][e][i] = 0.f;
       if constexpr (!kF8) {
 #pragma unroll
         for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-          for (int j = 0; j < kNt; j += 2) {
+          for (int u = 0; u < kU; ++u) {
             uint32_t r[4];
-            ldsm4(r, (kat ^ (t * 32)) + j * 8 * kRowBytes);
-            mma16<kBf16, kHalf>(sc[j], q[t], r[0], r[1]);
-            mma16<kBf16, kHalf>(sc[j + 1], q[t], r[2], r[3]);
+            ldsm4(r, (kat ^ (t * 32)) + u * 16 * kRowBytes);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) mma16<kBf16>(sc[u][e], r, q[t][e]);
           }
       } else {
 #pragma unroll
         for (int t4 = 0; t4 < kSteps / 4; ++t4)
 #pragma unroll
-          for (int j = 0; j < kNt; ++j) {
-            uint32_t r[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                         : "r"((kat ^ (t4 * 64)) + j * 8 * kRowBytes) : "memory");
+          for (int u = 0; u < kU; ++u) {
+            uint32_t x[4], y[4];
+            lds4(x, (kat ^ (t4 * 64)) + u * 16 * kRowBytes);
+            lds4(y, (kat ^ (t4 * 64)) + (u * 16 + 8) * kRowBytes);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-              uint32_t b0, b1;
-              e4m3x4_to_f16x2(r[t], b0, b1);
-              mma16<kBf16, kHalf>(sc[j], q[t4 * 4 + t], b0, b1);
+              uint32_t r[4];
+              e4m3x4_to_f16x2(x[t], r[0], r[2]);
+              e4m3x4_to_f16x2(y[t], r[1], r[3]);
+#pragma unroll
+              for (int e = 0; e < kN; ++e) mma16<kBf16>(sc[u][e], r, q[t4 * 4 + t][e]);
             }
           }
       }
       // base-2 logits; what a row's value scale adds to the maximum
-      float top[kS];
+      float top[kN][2], vs[kF8 ? kU : 1][2];
 #pragma unroll
-      for (int s = 0; s < kS; ++s) top[s] = -INFINITY;
-      float vs[kF8 ? kNt : 1][2];
+      for (int e = 0; e < kN; ++e) top[e][0] = top[e][1] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < kNt; ++j) {
-        float ks[2] = {1.f, 1.f}, lift[2] = {0.f, 0.f};
-        if constexpr (kF8) {
-          const uint32_t sa = at + 2 * kR * kRowBytes + (j * 8 + quad * 2) * 4;
-          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[0]), "=f"(ks[1]) : "r"(sa) : "memory");
-          asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(vs[j][0]), "=f"(vs[j][1]) : "r"(sa + kR * 4) : "memory");
+      for (int u = 0; u < kU; ++u)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) lift[i] = __log2f(fmaxf(fabsf(vs[j][i]), 7.9e-31f));  // 2^-100: no lower, or the sum of the weights leaves fp32
-        }
-#pragma unroll
-        for (int s = 0; s < kS; ++s)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float x = sc[j][2 * s + i] * back_scale[s];
-            if (kF8) x *= ks[i];
-            sc[j][2 * s + i] = x;
+        for (int r = 0; r < 2; ++r) {
+          const int key = u * 16 + r * 8 + oct;
+          float ks = 1.f, lift = 0.f;
+          if constexpr (kF8) {
+            ks = lds_f32(at + 2 * kR * kRowBytes + key * 4);
+            vs[u][r] = lds_f32(at + 2 * kR * kRowBytes + kR * 4 + key * 4);
+            lift = __log2f(fmaxf(fabsf(vs[u][r]), 7.9e-31f));  // 2^-100: no lower, or the sum of the weights leaves fp32
           }
-        if (live != 0xffffffffu) {
+          const bool there = (live >> key) & 1;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (!((live >> (j * 8 + quad * 2 + i)) & 1)) {
+          for (int e = 0; e < kN; ++e)
 #pragma unroll
-              for (int s = 0; s < kS; ++s) sc[j][2 * s + i] = -INFINITY;
+            for (int i = 0; i < 2; ++i) {
+              float x = sc[u][e][2 * r + i] * (kF8 ? back_scale[e][i] * ks : a.scale_log2);
+              x = there ? x : -INFINITY;
+              sc[u][e][2 * r + i] = x;
+              top[e][i] = fmaxf(top[e][i], kF8 ? x + lift : x);
             }
         }
-#pragma unroll
-        for (int s = 0; s < kS; ++s)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) top[s] = fmaxf(top[s], kF8 ? sc[j][2 * s + i] + lift[i] : sc[j][2 * s + i]);
-      }
       if (a.scores) {
 #pragma unroll
-        for (int s = 0; s < kS; ++s)
-          if (oct + 8 * s < heads) {
-            float* out = a.scores + ((int64_t)b * a.H + h0 + oct + 8 * s) * a.c.capacity + r0 + quad * 2;
+        for (int e = 0; e < kN; ++e)
 #pragma unroll
-            for (int j = 0; j < kNt; ++j)
+          for (int i = 0; i < 2; ++i) {
+            const int g = 8 * e + 2 * quad + i;
+            if (g >= heads) continue;
+            float* out = a.scores + ((int64_t)b * a.H + h0 + g) * a.c.capacity + r0 + oct;
 #pragma unroll
-              for (int i = 0; i < 2; ++i)
-                if (r0 + j * 8 + quad * 2 + i < end) out[j * 8 + i] = sc[j][2 * s + i];
+            for (int u = 0; u < kU; ++u)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+                if (r0 + u * 16 + r * 8 + oct < end) out[u * 16 + r * 8] = sc[u][e][2 * r + i];
           }
       }
       bool raise = false;
 #pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 1));
-        top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], 2));
-        raise = raise || top[s] > m[s] + kSlack;
-      }
+      for (int e = 0; e < kN; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top[e][i] = fmaxf(top[e][i], __shfl_xor_sync(0xffffffffu, top[e][i], x));
+          raise = raise || top[e][i] > m[e][i] + kSlack;
+        }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int s = 0; s < kS; ++s) {
-          const float to = fmaxf(m[s], top[s]);
-          const float keep = to == -INFINITY ? 0.f : sm100::ex2_approx(m[s] - to);
-          m[s] = to;
-          l[s] *= keep;
+        for (int e = 0; e < kN; ++e)
 #pragma unroll
-          for (int j = 0; j < kDt; ++j) o[j][2 * s] *= keep, o[j][2 * s + 1] *= keep;
-        }
+          for (int i = 0; i < 2; ++i) {
+            const float to = fmaxf(m[e][i], top[e][i]);
+            const float keep = to == -INFINITY ? 0.f : sm100::ex2_approx(m[e][i] - to);
+            m[e][i] = to;
+            l[e][i] *= keep;
+#pragma unroll
+            for (int j = 0; j < kDt; ++j) o[j][e][i] *= keep, o[j][e][2 + i] *= keep;
+          }
       }
-      float base[kS];
+      float base[kN][2];
 #pragma unroll
-      for (int s = 0; s < kS; ++s) base[s] = m[s] == -INFINITY ? 0.f : m[s] - kOffset;
+      for (int e = 0; e < kN; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) base[e][i] = m[e][i] == -INFINITY ? 0.f : m[e][i] - kOffset;
       // weights and their products with V, 16 keys at a time
 #pragma unroll
-      for (int j = 0; j < kNt; j += 2) {
-        uint32_t p[kA];
+      for (int u = 0; u < kU; ++u) {
+        uint32_t p[kN][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int e = 0; e < kN; ++e)
 #pragma unroll
-          for (int s = 0; s < kS; ++s) {
-            float x = sm100::ex2_approx(sc[j + u][2 * s] - base[s]), y = sm100::ex2_approx(sc[j + u][2 * s + 1] - base[s]);
-            l[s] += x + y;
-            if constexpr (kF8) x *= vs[j + u][0], y *= vs[j + u][1];
-            p[u * kS + s] = sm100::pack16x2<kBf16>(x, y);
+          for (int r = 0; r < 2; ++r) {
+            float x = sm100::ex2_approx(sc[u][e][2 * r] - base[e][0]), y = sm100::ex2_approx(sc[u][e][2 * r + 1] - base[e][1]);
+            l[e][0] += x, l[e][1] += y;
+            if constexpr (kF8) x *= vs[u][r], y *= vs[u][r];
+            p[e][r] = transpose8x8(sm100::pack16x2<kBf16>(x, y));
           }
         if constexpr (!kF8) {
 #pragma unroll
-          for (int d = 0; d < kDt; d += 2) {
+          for (int j = 0; j < kDt; ++j) {
             uint32_t r[4];
-            ldsm4_t(r, (vat ^ (d * 16)) + j * 8 * kRowBytes);
-            mma16<kBf16, kHalf>(o[d], p, r[0], r[1]);
-            mma16<kBf16, kHalf>(o[d + 1], p, r[2], r[3]);
+            ldsm4_t(r, (vat ^ (j * 32)) + u * 16 * kRowBytes);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) mma16<kBf16>(o[j][e], r, p[e]);
           }
         } else {
-          // a 16-bit column of the transposed load is a pair of neighbouring elements; they go to products of their own
+          // a 16-bit column of the transposed load is a pair of neighbouring elements: rows oct and oct + 8 of a product
 #pragma unroll
-          for (int d = 0; d < kDt; d += 4) {
-            uint32_t r[4];
-            ldsm4_t(r, (vat ^ (d * 8)) + j * 8 * kRowBytes);
+          for (int j = 0; j < kDt; j += 2) {
+            uint32_t w[4];
+            ldsm4_t(w, (vat ^ (j * 16)) + u * 16 * kRowBytes);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              uint32_t lo0, lo1, hi0, hi1;  // (keys 2 quad and 2 quad + 1 of one element side by side, then of its neighbour)
-              e4m3x4_to_f16x2(__byte_perm(r[2 * c], 0, 0x3120), lo0, lo1);
-              e4m3x4_to_f16x2(__byte_perm(r[2 * c + 1], 0, 0x3120), hi0, hi1);
-              mma16<kBf16, kHalf>(o[d + 2 * c], p, lo0, hi0);
-              mma16<kBf16, kHalf>(o[d + 2 * c + 1], p, lo1, hi1);
+              uint32_t r[4];  // (keys 2 quad and 2 quad + 1 of one element side by side, then of its neighbour)
+              e4m3x4_to_f16x2(__byte_perm(w[2 * c], 0, 0x3120), r[0], r[1]);
+              e4m3x4_to_f16x2(__byte_perm(w[2 * c + 1], 0, 0x3120), r[2], r[3]);
+#pragma unroll
+              for (int e = 0; e < kN; ++e) mma16<kBf16>(o[j + c][e], r, p[e]);
             }
           }
         }
@@ -674,41 +706,36 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kHalf>::kBlo
       stage = stage == kStages - 1 ? 0 : stage + 1;
     }
 
-    // ---- what the item, or this part of it, comes to: a lane's elements lie in pairs, with an e4m3 cache in fours
+    // ---- what the item, or this part of it, comes to
 #pragma unroll
-    for (int s = 0; s < kS; ++s) {
-      l[s] += __shfl_xor_sync(0xffffffffu, l[s], 1);
-      l[s] += __shfl_xor_sync(0xffffffffu, l[s], 2);
-      const int g = oct + 8 * s;
-      if (g >= heads) continue;
-      const int64_t bh = (int64_t)b * a.H + h0 + g, part = (int64_t)slot * kHeads + g;
-      const float by = slot >= 0 ? 1.f : l[s] == 0.f ? 0.f : 1.f / l[s];
-      if (quad == 0) {
-        if (slot >= 0) a.part_ml[part] = make_float2(m[s] - kOffset, l[s]);
-        else if (a.lse) a.lse[bh] = l[s] == 0.f ? 0.f : m[s] - kOffset + log2f(l[s]);
-      }
+    for (int e = 0; e < kN; ++e)
 #pragma unroll
-      for (int j = 0; j < kDt; j += kF8 ? 2 : 1) {
-        const int d = kF8 ? j * 8 + quad * 4 : j * 8 + quad * 2;
-        constexpr int kN = kF8 ? 4 : 2;
-        float x[kN];
-        if constexpr (kF8) x[0] = o[j][2 * s], x[1] = o[j + 1][2 * s], x[2] = o[j][2 * s + 1], x[3] = o[j + 1][2 * s + 1];
-        else x[0] = o[j][2 * s], x[1] = o[j][2 * s + 1];
+      for (int i = 0; i < 2; ++i) {
+        float sum = l[e][i];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        const int g = 8 * e + 2 * quad + i;
+        if (g >= heads) continue;
+        const int64_t bh = (int64_t)b * a.H + h0 + g, part = (int64_t)slot * kHeads + g;
         // (a head without weights is 0 even where what it would be divided by is not: 0 * 0)
+        const bool none = sum == 0.f;
+        const float by = slot >= 0 ? 1.f : 1.f / sum;
+        if (oct == 0) {
+          if (slot >= 0) a.part_ml[part] = make_float2(m[e][i] - kOffset, sum);
+          else if (a.lse) a.lse[bh] = none ? 0.f : m[e][i] - kOffset + log2f(sum);
+        }
 #pragma unroll
-        for (int i = 0; i < kN; ++i) x[i] = l[s] == 0.f ? 0.f : x[i] * by;
-        if (slot >= 0) {
-          float* to = a.part_o + part * kD + d;
-          if constexpr (kF8) *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
-          else *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
-        } else {
-          uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + bh * kD + d);
-#pragma unroll
-          for (int i = 0; i < kN; i += 2)
-            to[i / 2] = (kF8 ? a.dtype == KB_BF16 : kBf16) ? sm100::pack_bf16x2(x[i], x[i + 1]) : sm100::pack_f16x2(x[i], x[i + 1]);
+        for (int j = 0; j < kDt; ++j) {
+          const float x = none ? 0.f : o[j][e][i] * by, y = none ? 0.f : o[j][e][2 + i] * by;
+          const int d = kF8 ? j * 16 + 2 * oct : j * 16 + oct, d2 = kF8 ? d + 1 : d + 8;
+          if (slot >= 0) {
+            a.part_o[part * kD + d] = x, a.part_o[part * kD + d2] = y;
+          } else {
+            const int32_t type = kF8 ? a.dtype : kBf16 ? KB_BF16 : KB_F16;
+            store_any(a.o, bh * kD + d, type, x), store_any(a.o, bh * kD + d2, type, y);
+          }
         }
       }
-    }
   }
   cp_async_wait<0>();
 }
@@ -765,54 +792,66 @@ __global__ void __launch_bounds__(kMostJoinThreads) paged_join_kernel(const Atte
 
 // ---- rows' weights -------------------------------------------------------------------------------------------------------
 
+// A block takes rows of one sequence and key/value head; the group's log-sum-exps are the same for all of them.
 __global__ void __launch_bounds__(256) paged_weigh_kernel(const AttendArgs a) {
+  constexpr int kAtOnce = 8;
   const int32_t hk = blockIdx.y, b = blockIdx.z;
-  wait_for_launch_before();
+  const int64_t bh = (int64_t)b * a.H + hk * a.group;
   int32_t first, end;
   seen_rows(a, b, first, end);
+  wait_for_launch_before();
   for (int64_t r = (int64_t)first + blockIdx.x * 256 + threadIdx.x; r < end; r += (int64_t)gridDim.x * 256) {
+    const float* s = a.scores + bh * a.c.capacity + r;
+    float* to = a.weights + b * a.w_b + hk * a.w_h + r;
     float w = 0.f;
-    for (int g = 0; g < a.group; ++g) {
-      const int64_t bh = (int64_t)b * a.H + hk * a.group + g;
-      w += exp2f(a.scores[bh * a.c.capacity + r] - a.lse[bh]);
+    const float old = *to;
+    for (int g0 = 0; g0 < a.group; g0 += kAtOnce) {
+      float x[kAtOnce];
+#pragma unroll
+      for (int g = 0; g < kAtOnce; ++g) x[g] = g0 + g < a.group ? __ldcs(s + (int64_t)(g0 + g) * a.c.capacity) : 0.f;
+#pragma unroll
+      for (int g = 0; g < kAtOnce; ++g)
+        if (g0 + g < a.group) w += exp2f(x[g] - a.lse[bh + g0 + g]);
     }
-    a.weights[b * a.w_b + hk * a.w_h + r] += w;
+    *to = old + w;
   }
 }
 
 // Whether the tensor-core kernel takes the call: a 16-bit q of head dim 64 or 128 with dense heads; keys and values of one layout, with rows on
-// 16-byte boundaries, within 2^32 such units.
+// 16-byte boundaries, within 2^32 such units; their scales of one layout, within 2^32 elements.
 bool takes_mma(const kb_paged_attention_params& p) {
   const kb_paged_cache& c = p.cache;
   const int e = dtype_size(c.dtype);
   if (p.dtype == KB_F32 || (c.D != 64 && c.D != 128) || !paged_rows_aligned(c, e)) return false;
-  if (p.q_stride[2] != 1 || p.q_stride[0] % 2 || p.q_stride[1] % 2 || reinterpret_cast<uintptr_t>(p.q) % 4 || reinterpret_cast<uintptr_t>(p.o) % 4) return false;
-  int64_t last = 0;
+  if (p.q_stride[2] != 1 || p.q_stride[0] % 2 || p.q_stride[1] % 2 || reinterpret_cast<uintptr_t>(p.q) % 4) return false;
   const int32_t extent[3] = {c.P, c.H_kv, c.page};
-  for (int i = 0; i < 3; ++i) {
-    if (c.k_stride[i] != c.v_stride[i] || c.k_stride[i] < 0 || c.k_stride[i] > (int64_t)1 << 40) return false;
-    if (c.dtype == KB_E4M3 && c.k_scale_stride[i] != c.v_scale_stride[i]) return false;
-    if (c.k_stride[i] > 0 && extent[i] > 1 && c.k_stride[i] > ((int64_t)1 << 40) / extent[i]) return false;
-    last += c.k_stride[i] * kb_max_i32(extent[i] - 1, 0);
-  }
-  return last * e / 16 < 0xffffffff - 64;
+  const auto within = [&](const int64_t (&x)[3], const int64_t (&y)[3], int64_t unit) {
+    uint64_t last = 0;
+    for (int i = 0; i < 3; ++i) {
+      if (x[i] != y[i] || x[i] < 0 || x[i] >= (int64_t)1 << 36) return false;
+      last += (uint64_t)x[i] * (extent[i] > 1 ? extent[i] - 1 : 0) / unit;  // (below 2^36 * 2^31)
+      if (last >= 0xffffff00u) return false;
+    }
+    return true;
+  };
+  return within(c.k_stride, c.v_stride, 16 / e) && (c.dtype != KB_E4M3 || within(c.k_scale_stride, c.v_scale_stride, 1));
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------------
 
 constexpr int kSms = 148;
 
-template <bool kF8, bool kBf16, int kD, bool kHalf>
+template <bool kF8, bool kBf16, int kD, int kN>
 struct MmaKernel {
-  using Tile = MmaTile<kF8, kBf16, kD, kHalf>;
+  using Tile = MmaTile<kF8, kBf16, kD, kN>;
   static constexpr int kHeads = Tile::kHeads, kRows = Tile::kR, kUnits = kSms * Tile::kBlocks * kWarps;
   static constexpr int kLeast = 64 / kRows;  // tiles: short stretches leave parts that cost more to join than they save
   static int launch(const AttendArgs& a, bool, cudaStream_t s) {
     static std::atomic<bool> done[kMaxDevices];
     int dev = 0, n_sm = 0;
     if (!device_sm_count(&dev, &n_sm)) return KB_ERR_LAUNCH;
-    KB_CUDA_TRY(opt_in_smem_once(paged_attend_mma_kernel<kF8, kBf16, kD, kHalf>, Tile::kSmem, dev, done));
-    paged_attend_mma_kernel<kF8, kBf16, kD, kHalf><<<kb_cdiv_i32(a.units, kWarps), kThreads, Tile::kSmem, s>>>(a);
+    KB_CUDA_TRY(opt_in_smem_once(paged_attend_mma_kernel<kF8, kBf16, kD, kN>, Tile::kSmem, dev, done));
+    paged_attend_mma_kernel<kF8, kBf16, kD, kN><<<kb_cdiv_i32(a.units, kWarps), kThreads, Tile::kSmem, s>>>(a);
     KB_LAUNCH_CHECK("paged_attend_mma_kernel");
     return KB_OK;
   }
@@ -830,9 +869,9 @@ struct GenericKernel {
 // f(a kernel): the one for the call
 template <bool kF8, bool kBf16, typename F>
 auto with_mma(const kb_paged_attention_params& p, F f) {
-  const bool half = p.H / p.cache.H_kv <= 8;
-  if (p.cache.D == 64) return half ? f(MmaKernel<kF8, kBf16, 64, true>()) : f(MmaKernel<kF8, kBf16, 64, false>());
-  return half ? f(MmaKernel<kF8, kBf16, 128, true>()) : f(MmaKernel<kF8, kBf16, 128, false>());
+  const bool eight = p.H / p.cache.H_kv <= 8;
+  if (p.cache.D == 64) return eight ? f(MmaKernel<kF8, kBf16, 64, 1>()) : f(MmaKernel<kF8, kBf16, 64, 2>());
+  return eight ? f(MmaKernel<kF8, kBf16, 128, 1>()) : f(MmaKernel<kF8, kBf16, 128, 2>());
 }
 template <typename T, int D, typename F>
 auto with_group(const kb_paged_attention_params& p, F f) {
@@ -913,6 +952,7 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
     a.fd_context = kb_fastdiv_make(a.context);
   }
   a.scale_log2 = p.sm_scale * kLog2e;
+  for (int i = 0; i < 3; ++i) a.row16[i] = (uint32_t)(c.k_stride[i] * dtype_size(c.dtype) / 16), a.scale_at[i] = (uint32_t)c.k_scale_stride[i];
   return with_kernel(p, [&](auto kernel) {
     const Plan n = make_plan<decltype(kernel)>(p);
     a.heads = n.heads, a.head_tiles = n.head_tiles, a.units = n.units, a.least_tiles = n.least, a.by_item = n.by_item;

@@ -65,21 +65,46 @@ __device__ __forceinline__ void store8(T* out, const Eight<T>& e) {
   }
 }
 
-// The row's elements as its 8-bit form holds them, x / scale correctly rounded.
+// The largest magnitude's bits.  Bits without the sign: numbers keep their order, and a NaN is above them all, so that it reaches the scale.
+__device__ __forceinline__ uint32_t largest_bits(const Eight<float>& e) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) m = max(m, __float_as_uint(e.v[i]) & 0x7fffffffu);
+  return m;
+}
 template <typename T>
-__device__ __forceinline__ Eight<uint8_t> quantize8(const Eight<T>& e, float scale) {
+__device__ __forceinline__ uint32_t largest_bits(const Eight<T>& e) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&e);
+  const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+  const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+  return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&h)));
+}
+
+// The row's elements as its 8-bit form holds them: x / scale correctly rounded (div_by, two at a time), then rounded to e4m3.
+template <typename T>
+__device__ __forceinline__ Eight<uint8_t> quantize8(const Eight<T>& e, float scale, float r) {
   float f[kPerThread];
   if (scale <= 1e37f) {
-    const float r = 1.f / scale;
+    const uint64_t r2 = sm100::f2_pack(r, r), down = sm100::f2_pack(-scale, -scale);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) f[i] = div_by(to_f32(e.v[i]), scale, r);
+    for (int i = 0; i < kPerThread; i += 2) {
+      const uint64_t x = sm100::f2_pack(to_f32(e.v[i]), to_f32(e.v[i + 1])), q = sm100::f2_mul(x, r2);
+      sm100::f2_unpack(sm100::f2_fma(sm100::f2_fma(q, down, x), r2, q), f[i], f[i + 1]);
+    }
   } else {  // an infinity or a NaN in the row
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) f[i] = to_f32(e.v[i]) / scale;
   }
   Eight<uint8_t> out;
-  reinterpret_cast<uint32_t*>(&out)[0] = sm100::pack_e4m3x4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<uint32_t*>(&out)[1] = sm100::pack_e4m3x4(f[4], f[5], f[6], f[7]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    // the signs as they come: the correction above turns -0 into 0
+    uint32_t sign;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&e) + i * sizeof(T);
+    if constexpr (sizeof(T) == 2) sign = __byte_perm(w[0], w[1], 0x7531);
+    else sign = __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
+    reinterpret_cast<uint32_t*>(&out)[i] = sm100::pack_e4m3x4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]) | (sign & 0x80808080u);
+  }
   return out;
 }
 
@@ -136,10 +161,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteA
         const int32_t h = h2 + u;
         const bool write = live && h < h1;
         if constexpr (kF8) {
-          // as bits without the sign: numbers keep their order, and a NaN is above them all, so that it reaches the scale
-          uint32_t m = 0;
-#pragma unroll
-          for (int i = 0; i < kPerThread; ++i) m = max(m, __float_as_uint(to_f32(e[w][u].v[i])) & 0x7fffffffu);
+          uint32_t m = largest_bits(e[w][u]);
           for (int s = lanes / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
           float scale = __fmul_rn(__uint_as_float(m), 1.f / 448.f);
           if (scale < 1e-12f) scale = 1e-12f;  // (a NaN stays)
@@ -148,7 +170,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteA
               if (w) a.c.v_scale[page * a.c.vs_page + h * a.c.vs_head + at * a.c.vs_row] = scale;
               else a.c.k_scale[page * a.c.ks_page + h * a.c.ks_head + at * a.c.ks_row] = scale;
             }
-            store8<uint8_t, kAligned>(reinterpret_cast<uint8_t*>(base[w]) + to[w] + h * head[w], quantize8(e[w][u], scale));
+            store8<uint8_t, kAligned>(reinterpret_cast<uint8_t*>(base[w]) + to[w] + h * head[w], quantize8(e[w][u], scale, 1.f / scale));
           }
         } else if (write) {
           store8<T, kAligned>(reinterpret_cast<T*>(base[w]) + to[w] + h * head[w], e[w][u]);
