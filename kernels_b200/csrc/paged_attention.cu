@@ -794,27 +794,30 @@ __global__ void __launch_bounds__(kMostJoinThreads) paged_join_kernel(const Atte
 
 // A block takes rows of one sequence and key/value head; the group's log-sum-exps are the same for all of them.
 __global__ void __launch_bounds__(256) paged_weigh_kernel(const AttendArgs a) {
-  constexpr int kAtOnce = 8;
+  constexpr int kAtOnce = 4;
   const int32_t hk = blockIdx.y, b = blockIdx.z;
   const int64_t bh = (int64_t)b * a.H + hk * a.group;
   int32_t first, end;
   seen_rows(a, b, first, end);
   wait_for_launch_before();
-  for (int64_t r = (int64_t)first + blockIdx.x * 256 + threadIdx.x; r < end; r += (int64_t)gridDim.x * 256) {
-    const float* s = a.scores + bh * a.c.capacity + r;
-    float* to = a.weights + b * a.w_b + hk * a.w_h + r;
-    float w = 0.f;
-    const float old = *to;
-    for (int g0 = 0; g0 < a.group; g0 += kAtOnce) {
-      float x[kAtOnce];
+  const int32_t r = first + blockIdx.x * 256 + threadIdx.x;
+  if (r >= end) return;
+  const float *s = a.scores + bh * a.c.capacity + r, *lse = a.lse + bh;
+  float* to = a.weights + b * a.w_b + hk * a.w_h + r;
+  const float old = *to;
+  float w = 0.f;
+  for (int g0 = 0; g0 < a.group; g0 += kAtOnce) {
+    float x[kAtOnce], y[kAtOnce];
 #pragma unroll
-      for (int g = 0; g < kAtOnce; ++g) x[g] = g0 + g < a.group ? __ldcs(s + (int64_t)(g0 + g) * a.c.capacity) : 0.f;
-#pragma unroll
-      for (int g = 0; g < kAtOnce; ++g)
-        if (g0 + g < a.group) w += exp2f(x[g] - a.lse[bh + g0 + g]);
+    for (int g = 0; g < kAtOnce; ++g) {
+      const bool there = g0 + g < a.group;
+      x[g] = there ? __ldcs(s + (int64_t)(g0 + g) * a.c.capacity) : -INFINITY;
+      y[g] = there ? lse[g0 + g] : 0.f;
     }
-    *to = old + w;
+#pragma unroll
+    for (int g = 0; g < kAtOnce; ++g) w += exp2f(x[g] - y[g]);
   }
+  *to = old + w;
 }
 
 // Whether the tensor-core kernel takes the call: a 16-bit q of head dim 64 or 128 with dense heads; keys and values of one layout, with rows on
@@ -970,8 +973,7 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
       if (int rc = launch_after(paged_join_kernel, grid, threads, s, a)) return rc;
     }
     if (p.weights) {
-      const int32_t blocks = kb_cdiv_i32(n.most_rows, 256), fill = kb_max_i32(1, kSms * 16 / (c.B * c.H_kv));
-      const dim3 grid(kb_max_i32(1, kb_min_i32(blocks, fill)), c.H_kv, c.B);
+      const dim3 grid(kb_max_i32(1, kb_cdiv_i32(n.most_rows, 256)), c.H_kv, c.B);
       if (int rc = launch_after(paged_weigh_kernel, grid, 256, s, a)) return rc;
     }
     return (int)KB_OK;

@@ -268,94 +268,179 @@ struct Team {
   }
 };
 
-// A team (a block, or a cluster of them) per sequence and head; warp w of it has the rows [w S, (w + 1) S), 32 at a time so that ranks
-// within it are ballots.  kHeld: S = kWarpRows and the keys stay in registers; otherwise the rows are as many as there are, and
-// the keys are formed again from memory whenever they are needed.
-template <bool kHeld>
+// A team (a block, or a cluster of them) per sequence and head.
+struct SelectHead {
+  const float* w;
+  const int32_t* pos;
+  float* wo;
+  int32_t* po;
+  int32_t* count;
+  int64_t list;  // where its moves go
+  int32_t n;
+
+  __device__ __forceinline__ SelectHead(const EvictArgs& a, int32_t b, int32_t h) {
+    n = a.c.rows(b);
+    w = a.weights + b * a.w_b + h * a.w_h;
+    pos = a.positions + b * a.p_b + h * a.p_h;
+    wo = a.weights_out + b * a.wo_b + h * a.wo_h;
+    po = a.positions_out + b * a.po_b + h * a.po_h;
+    count = a.counts + (int64_t)b * a.H_kv + h;
+    list = ((int64_t)b * a.H_kv + h) * a.most_moves;
+  }
+};
+
+// Keys in registers.  Warp w of the team has the rows [w kWarpRows, (w + 1) kWarpRows), 32 at a time so that ranks within it are ballots.
+// The threshold, the least key that stays, is found bit by bit from the top: a count of the keys that reach it with the bit set.  A
+// dozen bits leave few keys between what surely stays and what surely goes; once they fit, one per thread, only they are counted.
 __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
   __shared__ int red[2][32], of_rank[2][8];
+  __shared__ uint32_t few[1024];
+  __shared__ int few_n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   Team team{red, of_rank, a.cluster, (int)blockIdx.x % a.cluster, 0};
-  const int32_t h = blockIdx.x / a.cluster, b = blockIdx.y;
-  const int32_t n = a.c.rows(b);
-  const float* w = a.weights + b * a.w_b + h * a.w_h;
-  const int32_t* pos = a.positions + b * a.p_b + h * a.p_h;
-  float* wo = a.weights_out + b * a.wo_b + h * a.wo_h;
-  int32_t* po = a.positions_out + b * a.po_b + h * a.po_h;
-  int32_t* count = a.counts + (int64_t)b * a.H_kv + h;
-  const int per_warp = kHeld ? kWarpRows : kb_cdiv_i32(kb_max_i32(n, 1), warps * 32) * 32;
-  const int begin = kb_min_i32((team.rank * warps + warp) * per_warp, n), end = kb_min_i32(begin + per_warp, n);
-  const uint32_t below = (1u << lane) - 1;
-
+  const SelectHead s(a, blockIdx.y, blockIdx.x / a.cluster);
+  const int32_t n = s.n, row0 = (team.rank * warps + warp) * kWarpRows + lane;
+  if (threadIdx.x == 0) few_n = 0;
   if (a.cluster > 1) sm100::cluster_sync_all();  // (a block's shared memory may be written once the block has started)
-  uint32_t held[kHeld ? kKeys : 1];
-  int32_t newest = INT32_MIN;
-  if constexpr (kHeld) {
+
+  uint32_t key[kKeys];
+  {
     float x[kKeys];
     int32_t y[kKeys];
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
-      const int i = begin + j * 32 + lane;
-      x[j] = i < end ? w[i] : 0.f;
-      y[j] = i < end ? pos[i] : INT32_MIN;
+      const int i = row0 + j * 32;
+      x[j] = i < n ? s.w[i] : 0.f;
+      y[j] = i < n ? s.pos[i] : INT32_MIN;
     }
+    int32_t newest = INT32_MIN;
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
-      const int i = begin + j * 32 + lane;
-      if (!a.in_place && i < end && i < a.budget) wo[i] = x[j], po[i] = y[j];
+      const int i = row0 + j * 32;
+      if (!a.in_place && i < n && i < a.budget) s.wo[i] = x[j], s.po[i] = y[j];
       newest = max(newest, y[j]);
     }
     if (n <= a.budget) {
-      if (threadIdx.x == 0 && team.rank == 0) *count = 0;
+      if (threadIdx.x == 0 && team.rank == 0) *s.count = 0;
       return;
     }
     newest = team.max(__reduce_max_sync(0xffffffffu, newest));
     const int64_t from = (int64_t)newest - a.recent;  // positions above it are among the newest
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) held[j] = begin + j * 32 + lane < end ? rank_key(x[j], y[j] > from) : 0u;
-  } else {
-    for (int i = begin + lane; i < end; i += 32) {
-      if (!a.in_place && i < a.budget) wo[i] = w[i], po[i] = pos[i];
-      newest = max(newest, pos[i]);
-    }
-    if (n <= a.budget) {
-      if (threadIdx.x == 0) *count = 0;
-      return;
-    }
-    newest = team.max(__reduce_max_sync(0xffffffffu, newest));
+    for (int j = 0; j < kKeys; ++j) key[j] = row0 + j * 32 < n ? rank_key(x[j], y[j] > from) : 0u;  // (0: does not count below)
   }
+  uint32_t least = 0, bit = 0x80000000u;
+  int reached = n, over = 0;  // keys that reach `least`, and those above what the bits to come can make of it
+  for (; bit && reached != a.budget && reached - over > (int)blockDim.x; bit >>= 1) {
+    int reach = 0;
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) reach += key[j] >= (least | bit);
+    reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
+    if (reach >= a.budget) least |= bit, reached = reach;
+    else over = reach;
+  }
+  if (bit && reached != a.budget) {
+    const uint32_t most = least + (bit - 1) + bit;  // (no more than 2^32 - 1)
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j)
+      if (key[j] >= least && key[j] <= most && row0 + j * 32 < n) few[atomicAdd(&few_n, 1)] = key[j];  // (in any order: they are counted)
+    __syncthreads();
+    const bool here = threadIdx.x < few_n;
+    const uint32_t mine = here ? few[threadIdx.x] : 0u;
+    const int others = over;
+    for (; bit && reached != a.budget; bit >>= 1) {
+      int reach = __syncthreads_count(here && mine >= (least | bit));
+      if (a.cluster > 1) reach = team.sum(warp == 0 ? reach : 0);
+      reach += others;
+      if (reach >= a.budget) least |= bit, reached = reach;
+      else over = reach;
+    }
+  }
+  let_next_launch_start();
+  // which rows stay; of those that equal the threshold, where there are too many, the lowest
+  uint32_t keep = 0;
+#pragma unroll
+  for (int j = 0; j < kKeys; ++j) keep |= (uint32_t)(key[j] >= least && row0 + j * 32 < n) << j;
+  if (reached != a.budget) {
+    int equal = 0, before;
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) equal += key[j] == least && row0 + j * 32 < n;
+    team.sum(__reduce_add_sync(0xffffffffu, equal), &before);
+    const int ties = a.budget - over;
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) {
+      const bool tie = key[j] == least && row0 + j * 32 < n;
+      const uint32_t eq = __ballot_sync(0xffffffffu, tie);
+      if (tie && before + __popc(eq & ((1u << lane) - 1)) >= ties) keep &= ~(1u << j);
+      before += __popc(eq);
+    }
+  }
+  uint32_t hole = 0, mover = 0;
+#pragma unroll
+  for (int j = 0; j < kKeys; ++j) {
+    const int i = row0 + j * 32;
+    const bool stays = (keep >> j) & 1;
+    hole |= (uint32_t)(i < a.budget && i < n && !stays) << j;
+    mover |= (uint32_t)(i >= a.budget && stays) << j;
+  }
+  int hole_at, mover_at;
+  team.sum(__reduce_add_sync(0xffffffffu, __popc(hole)), &hole_at);
+  const int moves = team.sum(__reduce_add_sync(0xffffffffu, __popc(mover)), &mover_at);
+  if (threadIdx.x == 0 && team.rank == 0) *s.count = moves;
+  const uint32_t below = (1u << lane) - 1;
+#pragma unroll
+  for (int j = 0; j < kKeys; ++j) {
+    const uint32_t hb = __ballot_sync(0xffffffffu, (hole >> j) & 1), mb = __ballot_sync(0xffffffffu, (mover >> j) & 1);
+    if ((hole >> j) & 1) a.dst[s.list + hole_at + __popc(hb & below)] = row0 + j * 32;
+    if ((mover >> j) & 1) a.src[s.list + mover_at + __popc(mb & below)] = row0 + j * 32;
+    hole_at += __popc(hb), mover_at += __popc(mb);
+  }
+}
+
+// The same for more rows than a cluster's registers hold: keys are formed again from memory whenever they are needed.
+__global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs a) {
+  __shared__ int red[2][32], of_rank[2][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  Team team{red, of_rank, 1, 0, 0};
+  const SelectHead s(a, blockIdx.y, blockIdx.x);
+  const int per_warp = kb_cdiv_i32(kb_max_i32(s.n, 1), warps * 32) * 32;
+  const int begin = kb_min_i32(warp * per_warp, s.n), end = kb_min_i32(begin + per_warp, s.n);
+  const uint32_t below = (1u << lane) - 1;
+  int32_t newest = INT32_MIN;
+  for (int i = begin + lane; i < end; i += 32) {
+    if (!a.in_place && i < a.budget) s.wo[i] = s.w[i], s.po[i] = s.pos[i];
+    newest = max(newest, s.pos[i]);
+  }
+  if (s.n <= a.budget) {
+    if (threadIdx.x == 0) *s.count = 0;
+    return;
+  }
+  newest = team.max(__reduce_max_sync(0xffffffffu, newest));
   const int64_t from = (int64_t)newest - a.recent;
   // f(key, row, whether there is such a row) for the warp's rows, all lanes together
   auto each = [&](auto f) {
-    if constexpr (kHeld) {
-#pragma unroll
-      for (int j = 0; j < kKeys; ++j)
-        if (begin + j * 32 < end) f(held[j], begin + j * 32 + lane, begin + j * 32 + lane < end);
-    } else {
-      for (int i0 = begin; i0 < end; i0 += 32) {
-        const int i = i0 + lane;
-        f(i < end ? rank_key(w[i], pos[i] > from) : 0u, i, i < end);
-      }
+    for (int i0 = begin; i0 < end; i0 += 32) {
+      const int i = i0 + lane;
+      f(i < end ? rank_key(s.w[i], s.pos[i] > from) : 0u, i, i < end);
     }
   };
-  // the largest threshold that at least `budget` keys reach, bit by bit; done where exactly so many reach it
   uint32_t least = 0;
-  int reached = n;
+  int reached = s.n, over = 0;
   for (uint32_t bit = 0x80000000u; bit && reached != a.budget; bit >>= 1) {
     int reach = 0;
-    each([&](uint32_t k, int, bool) { reach += k >= (least | bit); });  // (a row that is not there has key 0)
+    each([&](uint32_t k, int, bool) { reach += k >= (least | bit); });
     reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
     if (reach >= a.budget) least |= bit, reached = reach;
+    else over = reach;
   }
-  int above = 0, equal = 0, equal_before;
-  each([&](uint32_t k, int, bool in) {
-    above += __popc(__ballot_sync(0xffffffffu, in && k > least));
-    equal += __popc(__ballot_sync(0xffffffffu, in && k == least));
-  });
-  team.sum(equal, &equal_before);
-  const int ties = a.budget - team.sum(above);  // so many of the equal keys stay, the lowest rows
+  int ties = INT32_MAX, equal_before = 0;
+  if (reached != a.budget) {
+    int equal = 0;
+    each([&](uint32_t k, int, bool in) { equal += in && k == least; });
+    team.sum(__reduce_add_sync(0xffffffffu, equal), &equal_before);
+    ties = a.budget - over;
+  }
   let_next_launch_start();
-  const int64_t list = ((int64_t)b * a.H_kv + h) * a.most_moves;
   int holes = 0, movers = 0, hole_at = 0, mover_at = 0;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
@@ -367,8 +452,8 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
       const bool hole = in && !keep && i < a.budget, mover = keep && i >= a.budget;
       const uint32_t hb = __ballot_sync(0xffffffffu, hole), mb = __ballot_sync(0xffffffffu, mover);
       if (pass) {
-        if (hole) a.dst[list + hole_at + __popc(hb & below)] = i;
-        if (mover) a.src[list + mover_at + __popc(mb & below)] = i;
+        if (hole) a.dst[s.list + hole_at + __popc(hb & below)] = i;
+        if (mover) a.src[s.list + mover_at + __popc(mb & below)] = i;
         hole_at += __popc(hb), mover_at += __popc(mb);
       } else {
         holes += __popc(hb), movers += __popc(mb);
@@ -377,7 +462,7 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
     if (pass == 0) {
       team.sum(holes, &hole_at);
       const int moves = team.sum(movers, &mover_at);
-      if (threadIdx.x == 0 && team.rank == 0) *count = moves;
+      if (threadIdx.x == 0) *s.count = moves;
     }
   }
 }
@@ -461,7 +546,7 @@ int launch_select(const EvictArgs& in, int32_t heads, int32_t B, cudaStream_t s)
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = a.cluster, at.val.clusterDim.y = at.val.clusterDim.z = 1;
   c.attrs = &at, c.numAttrs = a.cluster > 1 ? 1 : 0;
-  KB_CUDA_TRY(held ? cudaLaunchKernelEx(&c, paged_select_kernel<true>, a) : cudaLaunchKernelEx(&c, paged_select_kernel<false>, a));
+  KB_CUDA_TRY(cudaLaunchKernelEx(&c, held ? paged_select_kernel : paged_select_long_kernel, a));
   count_launch();
   return KB_OK;
 }

@@ -6,8 +6,8 @@
 // turns exactly, and at position p the angle is off by at most p * 2^-54 turns (the frequency comes with 53 bits),
 // where a product in fp32 would be off by p * 2^-24.
 //
-// HBM-bound: every element is read and written once.  A thread owns one vector of pairs of one token, computes their
-// cosines and sines once and walks over heads with them.
+// HBM-bound: every element is read and written once.  A block takes a few tokens and forms the cosines and sines of their pairs
+// once, in shared memory; then its threads, each with one vector of pairs of one token, walk over the heads, several of them side by side.
 #include "common.cuh"
 
 namespace kb {
@@ -25,9 +25,9 @@ struct RotaryArgs {
   const double* inv_freq;
   int32_t B, T, D, R, axes, pos64, inverse;
   int32_t section_end[kMaxAxes];
-  int32_t vecs;            // vectors of pairs per token
+  int32_t vecs, tokens;    // vectors of pairs per token, tokens per block: both powers of two
   int32_t heads_per_cta;
-  KbFastDiv fd_vecs, fd_T;
+  KbFastDiv fd_T, fd_R;
 };
 
 template <typename T, int E> struct Elems { T v[E]; };
@@ -51,39 +51,57 @@ __device__ __forceinline__ void store_elems(T* p, const Elems<T, E>& e) {
   }
 }
 
+constexpr int kMostPairs = 512;  // of a block's tokens
+
+// cos and sin of the angle of pair d of a token
+__device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int32_t b, int32_t t, int32_t d) {
+  int32_t axis = 0;
+  while (axis < a.axes - 1 && d >= a.section_end[axis]) ++axis;
+  const int64_t at = axis * a.pos_axis + b * a.pos_b + t * a.pos_t;
+  const int64_t pos = a.pos64 ? static_cast<const int64_t*>(a.positions)[at] : static_cast<const int32_t*>(a.positions)[at];
+  const double turns = a.inv_freq[d] * 0.15915494309189535;  // 1 / (2 pi)
+  const uint64_t frac = (uint64_t)((turns - floor(turns)) * 18446744073709551616.0);
+  const int64_t angle = (int64_t)((uint64_t)pos * frac);  // [-1/2, 1/2) turns
+  float2 r;
+  sincospif((float)angle * 1.0842021724855044e-19f, &r.y, &r.x);  // 2^-63: half turns
+  if (a.inverse) r.y = -r.y;
+  return r;
+}
+
 // E: pairs per thread.  Vectors [0, R / E) hold pairs, the ones behind them what of a head is not rotated, cut in two halves.
 template <typename T, int E>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
-  const int64_t idx = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (idx >= (int64_t)a.B * a.T * a.vecs) return;
-  const int32_t bt = (int32_t)(idx / a.vecs), vec = (int32_t)(idx - (int64_t)bt * a.vecs);
-  const int32_t b = bt / a.T, t = bt - b * a.T;
+  __shared__ __align__(16) float2 turns[kMostPairs];
+  const int64_t token0 = (int64_t)blockIdx.x * a.tokens, all_tokens = (int64_t)a.B * a.T;
+  for (int i = threadIdx.x; i < a.tokens * a.R; i += kThreads) {
+    const int32_t k = kb_fastdiv(i, a.fd_R), d = i - k * a.R;
+    if (token0 + k < all_tokens) {
+      const int32_t b = kb_fastdiv((int32_t)(token0 + k), a.fd_T);
+      turns[i] = turn_of(a, b, (int32_t)(token0 + k) - b * a.T, d);
+    }
+  }
+  __syncthreads();
+  const int vec = threadIdx.x & (a.vecs - 1), rest_of = threadIdx.x / a.vecs, k = rest_of & (a.tokens - 1), head = rest_of / a.tokens;
+  const int head_lanes = kThreads / (a.vecs * a.tokens);
+  if (token0 + k >= all_tokens) return;
+  const int32_t b = kb_fastdiv((int32_t)(token0 + k), a.fd_T), t = (int32_t)(token0 + k) - b * a.T;
   const int32_t rot_vecs = a.R / E;
   const bool turned = vec < rot_vecs;
   const int32_t rest = a.D / 2 - a.R;  // half of what is not rotated
   const int32_t d0 = turned ? vec * E : 2 * a.R + (vec - rot_vecs) * E;
   const int32_t d1 = d0 + (turned ? a.R : rest);
-
   float c[E], s[E];
   if (turned) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int32_t d = d0 + e;
-      int32_t axis = 0;
-      while (axis < a.axes - 1 && d >= a.section_end[axis]) ++axis;
-      const int64_t at = axis * a.pos_axis + b * a.pos_b + t * a.pos_t;
-      const int64_t pos = a.pos64 ? static_cast<const int64_t*>(a.positions)[at] : static_cast<const int32_t*>(a.positions)[at];
-      const double turns = a.inv_freq[d] * 0.15915494309189535;  // 1 / (2 pi)
-      const uint64_t frac = (uint64_t)((turns - floor(turns)) * 18446744073709551616.0);
-      const int64_t angle = (int64_t)((uint64_t)pos * frac);  // [-1/2, 1/2) turns
-      sincospif((float)angle * 1.0842021724855044e-19f, &s[e], &c[e]);  // 2^-63: half turns
-      if (a.inverse) s[e] = -s[e];
+      const float2 r = turns[k * a.R + d0 + e];
+      c[e] = r.x, s[e] = r.y;
     }
   }
   const int32_t all = a.heads[0] + a.heads[1];
   const int32_t h0 = blockIdx.y * a.heads_per_cta, h1 = min(h0 + a.heads_per_cta, all);
 #pragma unroll 4
-  for (int32_t hh = h0; hh < h1; ++hh) {
+  for (int32_t hh = h0 + head; hh < h1; hh += head_lanes) {
     const int which = hh >= a.heads[0];
     const int32_t h = which ? hh - a.heads[0] : hh;
     const T* x = static_cast<const T*>(a.x[which]) + b * a.sb[which] + h * a.sh[which] + t * a.st[which];
@@ -114,13 +132,17 @@ template <typename T, int E>
 int launch(const RotaryArgs& in, cudaStream_t s) {
   RotaryArgs a = in;
   a.vecs = a.D / 2 / E;
-  const int64_t ctas = ((int64_t)a.B * a.T * a.vecs + kThreads - 1) / kThreads;
-  const int32_t all = a.heads[0] + a.heads[1];
-  if (ctas > 0x7fffffff) return KB_ERR_TOO_LARGE;
-  // few tokens: the heads go to CTAs of their own, at the price of the angles computed again in each
-  int32_t groups = (int32_t)(ctas >= 148 * 8 ? 1 : (148 * 8 + ctas - 1) / ctas);
-  groups = groups > all ? all : groups;
-  a.heads_per_cta = (all + groups - 1) / groups;
+  // a quarter of the block's threads for a head (of 128 pairs at most), so that four heads or more are under way
+  a.tokens = a.vecs >= kThreads / 4 ? 1 : kThreads / 4 / a.vecs;
+  while (a.tokens * a.R > kMostPairs) a.tokens /= 2;
+  a.fd_T = kb_fastdiv_make(a.T), a.fd_R = kb_fastdiv_make(a.R);
+  const int64_t ctas = ((int64_t)a.B * a.T + a.tokens - 1) / a.tokens;
+  const int32_t all = a.heads[0] + a.heads[1], lanes = kThreads / (a.vecs * a.tokens);
+  // few tokens: the heads go to blocks of their own, at the price of the angles formed again in each
+  int32_t groups = (int32_t)(ctas >= 148 * 4 ? 1 : (148 * 4 + ctas - 1) / ctas);
+  const int32_t most = (all + lanes - 1) / lanes;
+  groups = groups > most ? most : groups;
+  a.heads_per_cta = ((all + groups - 1) / groups + lanes - 1) / lanes * lanes;
   groups = (all + a.heads_per_cta - 1) / a.heads_per_cta;
   rotary_kernel<T, E><<<dim3((unsigned)ctas, (unsigned)groups), kThreads, 0, s>>>(a);
   KB_LAUNCH_CHECK("rotary_kernel");
