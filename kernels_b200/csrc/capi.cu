@@ -452,7 +452,7 @@ int kb_paged_attention(const kb_paged_attention_params* p, void* stream) {
   if (!kb::dtype_ok(p->dtype) || (p->cache.dtype != KB_E4M3 && p->cache.dtype != p->dtype)) return KB_ERR_UNSUPPORTED;
   if (kb::empty(p->cache.B, 1, p->H)) return KB_OK;
   if (p->cache.H_kv < 1 || p->H % p->cache.H_kv || !p->q || !p->o || (p->weights && !p->lse)) return KB_ERR_BAD_ARGUMENT;
-  if (p->H > 65535) return KB_ERR_TOO_LARGE;
+  if (p->H > 65535 || (int64_t)p->cache.B * p->H > (int64_t)1 << 30) return KB_ERR_TOO_LARGE;
   const uint64_t need = kb::paged_attention_workspace_bytes(*p);
   if (need && (!p->workspace || p->workspace_bytes < need || reinterpret_cast<uintptr_t>(p->workspace) % 16)) return KB_ERR_BAD_ARGUMENT;
   return kb::paged_attention(*p, static_cast<cudaStream_t>(stream));

@@ -22,7 +22,7 @@ namespace {
 
 // ---- write -----------------------------------------------------------------------------------------------------------
 
-constexpr int kWriteThreads = 256, kPerThread = 8, kHeadsAtOnce = 4;
+constexpr int kWriteThreads = 256, kPerThread = 8;
 
 struct WriteArgs {
   PagedView c;
@@ -135,46 +135,55 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteA
   }
   live = live && page >= 0;
   if (!__any_sync(0xffffffffu, live)) return;
+  // One head's keys and values in flight per thread leave room for more threads: 8 prompts of 4096-8192 tokens into 8-bit pages take 62 us
+  // with one, 65 with two, 68 with four.
+  constexpr int kHeadsAtOnce = kF8 ? 1 : 2;
+  using Out = typename std::conditional<kF8, uint8_t, T>::type;
   const T* from[2];
+  Out* to[2];
+  float* scale_to[2];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) from[w] = static_cast<const T*>(a.x[w]) + b * a.sb[w] + t * a.st[w] + d * a.sd[w];
-  const int64_t to[2] = {page * a.c.k_page + at * a.c.k_row + d, page * a.c.v_page + at * a.c.v_row + d};
-  const int64_t head[2] = {a.c.k_head, a.c.v_head};
-  char* base[2] = {a.c.k, a.c.v};
+  for (int w = 0; w < 2; ++w) from[w] = static_cast<const T*>(a.x[w]) + b * a.sb[w] + t * a.st[w] + d * a.sd[w] + h0 * a.sh[w];
+  to[0] = reinterpret_cast<Out*>(a.c.k) + page * a.c.k_page + at * a.c.k_row + h0 * a.c.k_head + d;
+  to[1] = reinterpret_cast<Out*>(a.c.v) + page * a.c.v_page + at * a.c.v_row + h0 * a.c.v_head + d;
+  if constexpr (kF8) {
+    scale_to[0] = a.c.k_scale + page * a.c.ks_page + at * a.c.ks_row + h0 * a.c.ks_head;
+    scale_to[1] = a.c.v_scale + page * a.c.vs_page + at * a.c.vs_row + h0 * a.c.vs_head;
+  }
+  const int64_t head[2] = {a.c.k_head, a.c.v_head}, scale_head[2] = {a.c.ks_head, a.c.vs_head};
   for (int32_t h2 = h0; h2 < h1; h2 += kHeadsAtOnce) {
-    Eight<T> e[2][kHeadsAtOnce];
+    Eight<T> e[kHeadsAtOnce][2];
 #pragma unroll
     for (int u = 0; u < kHeadsAtOnce; ++u)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         if (live && h2 + u < h1) {
-          load8<T, kAligned>(e[w][u], from[w] + (h2 + u) * a.sh[w], a.sd[w]);
+          load8<T, kAligned>(e[u][w], from[w], a.sd[w]);
         } else {
 #pragma unroll
-          for (int i = 0; i < kPerThread; ++i) e[w][u].v[i] = from_f32<T>(0.f);
+          for (int i = 0; i < kPerThread; ++i) e[u][w].v[i] = from_f32<T>(0.f);
         }
+        from[w] += a.sh[w];
       }
 #pragma unroll
     for (int u = 0; u < kHeadsAtOnce; ++u)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const int32_t h = h2 + u;
-        const bool write = live && h < h1;
+        const bool write = live && h2 + u < h1;
         if constexpr (kF8) {
-          uint32_t m = largest_bits(e[w][u]);
+          uint32_t m = largest_bits(e[u][w]);
           for (int s = lanes / 2; s > 0; s >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
           float scale = __fmul_rn(__uint_as_float(m), 1.f / 448.f);
           if (scale < 1e-12f) scale = 1e-12f;  // (a NaN stays)
           if (write) {
-            if (lane == 0) {
-              if (w) a.c.v_scale[page * a.c.vs_page + h * a.c.vs_head + at * a.c.vs_row] = scale;
-              else a.c.k_scale[page * a.c.ks_page + h * a.c.ks_head + at * a.c.ks_row] = scale;
-            }
-            store8<uint8_t, kAligned>(reinterpret_cast<uint8_t*>(base[w]) + to[w] + h * head[w], quantize8(e[w][u], scale, 1.f / scale));
+            if (lane == 0) *scale_to[w] = scale;
+            store8<uint8_t, kAligned>(to[w], quantize8(e[u][w], scale, 1.f / scale));
           }
+          scale_to[w] += scale_head[w];
         } else if (write) {
-          store8<T, kAligned>(reinterpret_cast<T*>(base[w]) + to[w] + h * head[w], e[w][u]);
+          store8<T, kAligned>(to[w], e[u][w]);
         }
+        to[w] += head[w];
       }
   }
 }
@@ -184,7 +193,7 @@ int launch_write(const WriteArgs& in, bool f8, bool aligned, cudaStream_t s) {
   WriteArgs a = in;
   const int64_t tokens = (int64_t)a.B * a.T, each = kWriteThreads / (a.D / kPerThread), ctas = (tokens + each - 1) / each;
   // few tokens: the heads go to blocks of their own
-  a.heads_per_cta = ctas >= 148 * 4 ? a.H_kv : kHeadsAtOnce;
+  a.heads_per_cta = ctas >= 148 * 4 ? a.H_kv : kb_min_i32(2, a.H_kv);
   const dim3 grid((unsigned)ctas, (unsigned)kb_cdiv_i32(a.H_kv, a.heads_per_cta));
   if (f8) {
     if (aligned) paged_write_kernel<T, true, true><<<grid, kWriteThreads, 0, s>>>(a);

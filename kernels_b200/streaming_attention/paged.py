@@ -65,6 +65,7 @@ def _per_row(name, x, dtype, c, index):
     shape, strides = x.shape, x.stride()
     assert x.dtype == dtype and x.get_device() == index and len(shape) == 3 and shape[0] == c.B and shape[1] == c.H_kv, f"{name} is [B, H_kv, M * page]"
     assert shape[2] >= c.M * c.page and (strides[2] == 1 or shape[2] <= 1), f"{name} has an entry for every row, side by side"
+    assert (strides[0] or shape[0] <= 1) and (strides[1] or shape[1] <= 1), f"{name} is written: every sequence and head has entries of its own"
     return x.data_ptr(), strides[:2]
 
 
@@ -158,7 +159,7 @@ def paged_attention(
         strides = q.stride()
     p = _lib.PagedAttentionParams()
     p.cache = c
-    o = q.new_empty(shape)
+    o = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     lse = lens.new_empty((B, H), dtype=torch.float32) if return_lse or weights is not None else None
     p.q, p.o = q.data_ptr(), o.data_ptr()
     p.q_stride[:] = strides

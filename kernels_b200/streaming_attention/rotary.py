@@ -21,12 +21,12 @@ from .. import _lib
 def _rotate(q, k, positions, inv_freq, ends, inverse):
     p = _lib.RotaryParams()
     shape = q.shape
-    q_out, k_out = q.new_empty(shape), None
+    q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), None
     p.q, p.q_out = _lib.tensor4(q), q_out.data_ptr()
     p.B, p.H, p.T, p.D = shape
     if k is not None:
         k_shape = k.shape
-        k_out = k.new_empty(k_shape)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         if 0 not in k_shape:
             p.k, p.k_out, p.H_kv = _lib.tensor4(k), k_out.data_ptr(), k_shape[1]
     p.positions, p.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
@@ -46,14 +46,18 @@ class _RotaryEmbedding(torch.autograd.Function):
     def forward(ctx, q, k, positions, inv_freq, ends, inverse):
         ctx.save_for_backward(positions, inv_freq)
         ctx.ends, ctx.inverse = ends, inverse
-        ctx.shapes = q.shape, None if k is None else k.shape
         return _rotate(q, k, positions, inv_freq, ends, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         # (turned by the same function, so that gradients have gradients)
-        dq, dk = _RotaryEmbedding.apply(dq, dk, positions, inv_freq, ctx.ends, not ctx.inverse)
+        turn = lambda q, k: _RotaryEmbedding.apply(q, k, positions, inv_freq, ctx.ends, not ctx.inverse)  # noqa: E731
+        need_q, need_k = ctx.needs_input_grad[:2]
+        if need_q:
+            dq, dk = turn(dq, dk if need_k else None)
+        else:
+            dq, dk = None, turn(dk, None)[0]
         return dq, dk, None, None, None, None
 
 

@@ -598,7 +598,7 @@ def test_refusals():
     calls = [
         (paged_attention, dict(q=q), [dict(q=q[:1]), dict(q=q[:, :3]), dict(q=q.float()), dict(q=q[..., :32]), dict(q=q[0]), dict(q=q.cpu()), dict(context_size=0),
                                       dict(back_contexts=-1), dict(weights=w[:, :1]), dict(weights=w[..., 1:]), dict(weights=w.double()),
-                                      dict(weights=w.transpose(1, 2)), dict(weights=w.cpu())]),
+                                      dict(weights=w.transpose(1, 2)), dict(weights=w.cpu()), dict(weights=w[:1].expand(2, 2, L))]),
         (paged_cache_write, dict(k=k, v=k), [dict(k=k[:1], v=k[:1]), dict(v=k[:, :1]), dict(k=k.float(), v=k.float()), dict(k=k[..., :32], v=k[..., :32]),
                                              dict(new_lens=g["lens"].long()), dict(new_lens=g["lens"][:1]), dict(positions=g["lens"]), dict(weights=w[..., 1:]),
                                              dict(positions=torch.zeros(2, 3, device="cuda")), dict(row_positions=w), dict(v=k.cpu())]),

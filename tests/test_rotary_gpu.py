@@ -154,6 +154,16 @@ def test_rotary_second_gradients_and_unused_outputs():
     assert torch.allclose(dq, q, atol=1e-5)  # a rotation's transpose undoes it
     (again,) = torch.autograd.grad(dq.square().sum() / 2, q)
     assert torch.allclose(again, q, atol=1e-5)
+    # the keys alone, the queries alone, gradients that come expanded
+    for grads in ((False, True), (True, False)):
+        x, y = q.detach().requires_grad_(grads[0]), k.detach().requires_grad_(grads[1])
+        out = rotary_embedding(x, y, positions, inv_freq)
+        leaf, got = (x, out[0]) if grads[0] else (y, out[1])
+        (d,) = torch.autograd.grad((out[0] + out[1]).sum(), leaf)
+        ref = PO.rotary(torch.ones_like(leaf.cpu().detach()), -positions.cpu(), inv_freq.cpu(), sections)
+        assert torch.allclose(d.cpu().double(), ref, atol=1e-5) and got.requires_grad
+    (d,) = torch.autograd.grad(rotary_embedding(q, None, positions, inv_freq)[0].sum(), q)
+    assert d.shape == q.shape
 
 
 def test_rotary_in_a_graph_and_on_another_stream():
