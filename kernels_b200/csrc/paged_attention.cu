@@ -2,7 +2,7 @@
 // token sees, its log-sum-exp, and on request every row's weight added to a running sum.
 //
 // HBM-bound: two FLOPs per byte and query head; all that counts is to read every cached row once, at full rate.  The query
-// heads that share a key/value head are therefore worked on together (an item: a sequence and up to 16 query heads), and the rows
+// heads that share a key/value head are therefore worked on together (an item: a sequence and up to 24 query heads), and the rows
 // of all items, cut into tiles, form one line that is shared out evenly: every unit (a warp of the tensor-core
 // kernel, a block of the generic one) walks over a stretch of it, whatever the lengths are, and as many units are
 // launched as the GPU holds.  A unit keeps, per head, the running maximum, the sum and the unnormalised output (fp32).  An item that lies
@@ -23,7 +23,6 @@ namespace kb {
 namespace {
 
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-constexpr int kMostHeads = 16;  // of an item
 
 struct AttendArgs {
   PagedView c;
@@ -341,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
 
 // ---- tensor-core kernel ----------------------------------------------------------------------------------------------
 //
-// 16-bit and e4m3 caches of head dim 64 and 128.  Sixteen keys are the rows of a product (m16n8k16) and eight query heads its
+// Caches of head dim 64 and 128.  Sixteen keys are the rows of a product (m16n8k16, m16n8k8 for fp32) and eight query heads its
 // columns: S^T = K Q^T, then O^T += V^T P^T with the weights turned over in registers.  So up to eight heads cost what one does, and what
 // the tensor cores have to do is a small part of the time that the keys take to arrive.  That time is all there is to hide, and
 // every warp hides it for itself: it is a unit with a ring of kStages tiles of kR rows in shared memory, filled by 16-byte
@@ -355,6 +354,10 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
 // multiplied are p * v_scale, so the running maximum is taken over score + log2(v_scale), which keeps them within f16.
 // f16 weights start at 2^7 and may grow to 2^15 before sums are rescaled: seven bits more for the small ones.
 // Weights are rounded to 16 bits for the product with V (as in the operator's forward kernel); their sum is taken before that.
+//
+// fp32 is cut in two: x = hi + lo, hi the 11 leading bits (tf32), lo the next 11, and a product is hi hi + lo hi + hi lo, which leaves out
+// some 2^-23 of it (and makes NaN of what fp32 has infinities for).  The tensor cores cut sums off where an addition rounds, so what they add to a long sum goes in by an addition.  (On CUDA cores a row costs 4 D flops per query head and the sums over lanes besides: 16 sequences of 4096 rows,
+// 32 / 8 heads of 128, took 434 us, five times what the rows take to be read.)
 
 __device__ __forceinline__ void cp_async16(uint32_t to, const void* from, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
@@ -396,35 +399,56 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], con
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
+// c += a b, 16 x 8 x 8, in tf32
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// hi: to nearest, so that lo, which is cut off, has either sign.  (A NaN stays one, in hi or in lo; so does an infinity, as a NaN.)
+template <int N>
+__device__ __forceinline__ void split_tf32(const uint32_t (&x)[N], uint32_t (&hi)[N], uint32_t (&lo)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    hi[i] = (x[i] + 0x1000u) & 0xffffe000u;
+    lo[i] = __float_as_uint(__uint_as_float(x[i]) - __uint_as_float(hi[i])) & 0xffffe000u;
+  }
+}
 // four e4m3 to two pairs of f16
 __device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t four, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 
-// kF8: e4m3 cache (products in f16); kBf16: products in bf16, otherwise in f16; kN: eights of query heads per item
-template <bool kF8, bool kBf16, int kD, int kN>
+// kType: of the cache; products are in f16 for e4m3.  kN: eights of query heads per item
+template <int kType, int kD, int kN>
 struct MmaTile {
-  static constexpr int kRowBytes = kF8 ? kD : 2 * kD, kChunks = kRowBytes / 16;
-  static constexpr int kR = kRowBytes == 256 ? 16 : 32;  // rows of a tile
-  static constexpr int kStages = kRowBytes == 256 ? 2 : kRowBytes == 128 ? 3 : 4;
-  static constexpr int kScaleBytes = kF8 ? 2 * kR * 4 : 0;
+  static constexpr int kElem = kType == KB_F32 ? 4 : kType == KB_E4M3 ? 1 : 2;
+  static constexpr int kRowBytes = kD * kElem, kChunks = kRowBytes / 16;
+  static constexpr int kR = kRowBytes >= 256 ? 16 : 32;  // rows of a tile
+  static constexpr int kStages = kRowBytes >= 256 ? 2 : kRowBytes == 128 ? 3 : 4;
+  static constexpr int kScaleBytes = kType == KB_E4M3 ? 2 * kR * 4 : 0;
   static constexpr int kStageBytes = 2 * kR * kRowBytes + kScaleBytes;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kHeads = 8 * kN;
   static constexpr int kSmem = kWarps * kWarpBytes;
-  static constexpr int kBlocks = kRowBytes == 256 && kN == 1 ? 3 : 2;  // per SM: what shared memory and registers allow
+  // per SM: what shared memory and registers allow
+  static constexpr int kBlocks = kRowBytes == 512 ? 1 : kRowBytes == 256 && kN == 1 ? 3 : 2;
   static_assert(kStageBytes % 128 == 0, "matrix loads address a tile by exclusive or");
-  // Where chunk c of row r lies: at c ^ swizzle(r).  The eight rows of a matrix load hit different banks, and so do the two rows
-  // and four chunks of a 16-byte load of e4m3 keys.
-  static __device__ __forceinline__ int swizzle(int r) { return !kF8 ? r & 7 : kD == 128 ? ((r & 1) << 2) | ((r >> 1) & 3) : (r >> 1) & 3; }
+  // Where chunk c of row r lies: at c ^ swizzle(r), so that what a matrix load (eight rows of a chunk) or a quarter of a 16-byte
+  // load takes (two keys by four chunks; in fp32 also four rows by two chunks) lies in different banks.
+  static __device__ __forceinline__ int swizzle(int r) {
+    if (kType == KB_F32) return ((r & 1) << 2) | (r & 2);
+    if (kType == KB_E4M3) return kD == 128 ? ((r & 1) << 2) | ((r >> 1) & 3) : (r >> 1) & 3;
+    return r & 7;
+  }
 };
 
-template <bool kF8, bool kBf16, int kD, int kN>
-__global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks) paged_attend_mma_kernel(const AttendArgs a) {
-  using Tile = MmaTile<kF8, kBf16, kD, kN>;
+template <int kType, int kD, int kN>
+__global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) paged_attend_mma_kernel(const AttendArgs a) {
+  using Tile = MmaTile<kType, kD, kN>;
+  constexpr bool kF8 = kType == KB_E4M3, kBf16 = kType == KB_BF16, kF32 = kType == KB_F32;
   constexpr int kR = Tile::kR, kStages = Tile::kStages, kChunks = Tile::kChunks, kRowBytes = Tile::kRowBytes, kHeads = Tile::kHeads;
   constexpr int kSteps = kD / 16, kU = kR / 16, kDt = kD / 16;
-  constexpr float kOffset = kBf16 ? 0.f : 7.f, kSlack = 8.f;
+  constexpr float kOffset = kF8 || kType == KB_F16 ? 7.f : 0.f, kSlack = 8.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, oct = lane >> 2;
   const int32_t unit = blockIdx.x * kWarps + warp;
@@ -481,9 +505,10 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks
   }
 
   // where this lane's matrix loads start in a tile; chunks and keys further on are an exclusive or and an offset away
-  const int kkey = kF8 ? oct : lane & 15, vkey = kF8 ? lane & 15 : (lane & 7) + (lane >> 4) * 8;
-  const uint32_t kplace = kkey * kRowBytes + (((kF8 ? quad : lane >> 4) ^ Tile::swizzle(kkey)) * 16);
-  const uint32_t vplace = (kR + vkey) * kRowBytes + (((kF8 ? lane >> 4 : (lane >> 3) & 1) ^ Tile::swizzle(vkey)) * 16);
+  const int kkey = kF8 || kF32 ? oct : lane & 15, kchunk = kF8 || kF32 ? quad : lane >> 4;
+  const int vkey = kF32 ? quad : kF8 ? lane & 15 : (lane & 7) + (lane >> 4) * 8, vchunk = kF32 ? oct : kF8 ? lane >> 4 : (lane >> 3) & 1;
+  const uint32_t kplace = kkey * kRowBytes + ((kchunk ^ Tile::swizzle(kkey)) * 16);
+  const uint32_t vplace = (kR + vkey) * kRowBytes + ((vchunk ^ Tile::swizzle(vkey)) * 16);
   int stage = 0;
   Place now = stretch.at;
   for (int64_t seen = 0; now.left > 0;) {
@@ -495,15 +520,22 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks
     now.advance(a, kR, n);
     seen += n;
 
-    // ---- q as the products' right operand: lane (oct, quad) has elements of head oct; with an e4m3 cache the ones that its 16-byte key loads hold
-    uint32_t q[kSteps][kN][2];
+    // ---- q as the products' right operand: lane (oct, quad) has elements of head oct, with e4m3 and fp32 caches the ones that its 16-byte key loads hold
+    uint32_t q[kSteps][kN][kF32 ? 4 : 2];
     float back_scale[kF8 ? kN : 1][2];  // of heads 2 quad and 2 quad + 1, as the scores lie
 #pragma unroll
     for (int e = 0; e < kN; ++e) {
       const int g = oct + 8 * e;
-      const uint16_t* from = static_cast<const uint16_t*>(a.q) + b * a.q_b + (int64_t)(h0 + (g < heads ? g : 0)) * a.q_h;
+      const int64_t head = b * a.q_b + (int64_t)(h0 + (g < heads ? g : 0)) * a.q_h;
+      if constexpr (kF32) {
 #pragma unroll
-      for (int t = 0; t < kSteps; ++t)
+        for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) q[t][e][p] = g < heads ? __ldg(static_cast<const uint32_t*>(a.q) + head + t * 16 + quad * 4 + p) : 0u;
+      }
+      const uint16_t* from = static_cast<const uint16_t*>(a.q) + head;
+#pragma unroll
+      for (int t = 0; t < (kF32 ? 0 : kSteps); ++t)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int d = kF8 ? t / 4 * 64 + quad * 16 + t % 4 * 4 + 2 * p : t * 16 + 8 * p + quad * 2;
@@ -569,7 +601,37 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks
         for (int e = 0; e < kN; ++e)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[u][e][i] = 0.f;
-      if constexpr (!kF8) {
+      if constexpr (kF32) {
+        float small[kN][4] = {};
+#pragma unroll
+        for (int t = 0; t < kSteps; ++t) {
+          uint32_t x[4], y[4];
+          lds4(x, kat ^ (t * 64));
+          lds4(y, (kat ^ (t * 64)) + 8 * kRowBytes);
+#pragma unroll
+          for (int p = 0; p < 4; p += 2) {
+            const uint32_t r[4] = {x[p], y[p], x[p + 1], y[p + 1]};
+            uint32_t hi[4], lo[4];
+            split_tf32(r, hi, lo);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+              const uint32_t w[2] = {q[t][e][p], q[t][e][p + 1]};
+              uint32_t qhi[2], qlo[2];
+              split_tf32(w, qhi, qlo);
+              mma8(small[e], lo, qhi);
+              mma8(small[e], hi, qlo);
+              float step[4] = {0.f, 0.f, 0.f, 0.f};
+              mma8(step, hi, qhi);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sc[0][e][i] += step[i];
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kN; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[0][e][i] += small[e][i];
+      } else if constexpr (!kF8) {
 #pragma unroll
         for (int t = 0; t < kSteps; ++t)
 #pragma unroll
@@ -669,6 +731,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         uint32_t p[kN][2];
+        float pf[kF32 ? kN : 1][4];
 #pragma unroll
         for (int e = 0; e < kN; ++e)
 #pragma unroll
@@ -676,9 +739,46 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks
             float x = sm100::ex2_approx(sc[u][e][2 * r] - base[e][0]), y = sm100::ex2_approx(sc[u][e][2 * r + 1] - base[e][1]);
             l[e][0] += x, l[e][1] += y;
             if constexpr (kF8) x *= vs[u][r], y *= vs[u][r];
-            p[e][r] = transpose8x8(sm100::pack16x2<kBf16>(x, y));
+            if constexpr (kF32) pf[e][2 * r] = x, pf[e][2 * r + 1] = y;
+            else p[e][r] = transpose8x8(sm100::pack16x2<kBf16>(x, y));
           }
-        if constexpr (!kF8) {
+        if constexpr (kF32) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // eight keys: 8 h + quad and 8 h + quad + 4
+            uint32_t phi[kN][2], plo[kN][2];
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {  // turned over: from key oct, heads 2 quad and 2 quad + 1 to key quad + 4 k, head oct
+                const int from = (quad + 4 * k) * 4 + (oct >> 1);
+                const float x = __shfl_sync(0xffffffffu, pf[e][2 * h], from), y = __shfl_sync(0xffffffffu, pf[e][2 * h + 1], from);
+                p[e][k] = __float_as_uint(oct & 1 ? y : x);
+              }
+              split_tf32(p[e], phi[e], plo[e]);
+            }
+#pragma unroll
+            for (int j = 0; j < kDt; j += 2) {
+              uint32_t x[4], y[4];
+              lds4(x, (vat ^ (j * 64)) + 8 * h * kRowBytes);
+              lds4(y, (vat ^ (j * 64)) + (8 * h + 4) * kRowBytes);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const uint32_t r[4] = {x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1]};
+                uint32_t hi[4], lo[4];
+                split_tf32(r, hi, lo);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) {
+                  float step[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma8(step, lo, phi[e]);
+                  mma8(step, hi, plo[e]);
+                  mma8(step, hi, phi[e]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) o[j + c][e][i] += step[i];
+                }
+              }
+            }
+          }
+        } else if constexpr (!kF8) {
 #pragma unroll
           for (int j = 0; j < kDt; ++j) {
             uint32_t r[4];
@@ -727,11 +827,11 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kF8, kBf16, kD, kN>::kBlocks
 #pragma unroll
         for (int j = 0; j < kDt; ++j) {
           const float x = none ? 0.f : o[j][e][i] * by, y = none ? 0.f : o[j][e][2 + i] * by;
-          const int d = kF8 ? j * 16 + 2 * oct : j * 16 + oct, d2 = kF8 ? d + 1 : d + 8;
+          const int d = kF32 ? j / 2 * 32 + oct * 4 + j % 2 * 2 : kF8 ? j * 16 + 2 * oct : j * 16 + oct, d2 = kF8 || kF32 ? d + 1 : d + 8;
           if (slot >= 0) {
             a.part_o[part * kD + d] = x, a.part_o[part * kD + d2] = y;
           } else {
-            const int32_t type = kF8 ? a.dtype : kBf16 ? KB_BF16 : KB_F16;
+            const int32_t type = kF8 ? a.dtype : kType;
             store_any(a.o, bh * kD + d, type, x), store_any(a.o, bh * kD + d2, type, y);
           }
         }
@@ -820,13 +920,14 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const AttendArgs a) {
   *to = old + w;
 }
 
-// Whether the tensor-core kernel takes the call: a 16-bit q of head dim 64 or 128 with dense heads; keys and values of one layout, with rows on
-// 16-byte boundaries, within 2^32 such units; their scales of one layout, within 2^32 elements.
+// Whether the tensor-core kernel takes the call: head dim 64 or 128; dense heads of q, which has 16 bits where the cache has 8; keys and values of
+// one layout, with rows on 16-byte boundaries, within 2^32 such units; their scales of one layout, within 2^32 elements.
 bool takes_mma(const kb_paged_attention_params& p) {
   const kb_paged_cache& c = p.cache;
   const int e = dtype_size(c.dtype);
-  if (p.dtype == KB_F32 || (c.D != 64 && c.D != 128) || !paged_rows_aligned(c, e)) return false;
-  if (p.q_stride[2] != 1 || p.q_stride[0] % 2 || p.q_stride[1] % 2 || reinterpret_cast<uintptr_t>(p.q) % 4) return false;
+  if ((p.dtype == KB_F32 && c.dtype != KB_F32) || (c.D != 64 && c.D != 128) || !paged_rows_aligned(c, e)) return false;
+  if (p.q_stride[2] != 1) return false;
+  if (p.dtype != KB_F32 && (p.q_stride[0] % 2 || p.q_stride[1] % 2 || reinterpret_cast<uintptr_t>(p.q) % 4)) return false;
   const int32_t extent[3] = {c.P, c.H_kv, c.page};
   const auto within = [&](const int64_t (&x)[3], const int64_t (&y)[3], int64_t unit) {
     uint64_t last = 0;
@@ -844,17 +945,17 @@ bool takes_mma(const kb_paged_attention_params& p) {
 
 constexpr int kSms = 148;
 
-template <bool kF8, bool kBf16, int kD, int kN>
+template <int kType, int kD, int kN>
 struct MmaKernel {
-  using Tile = MmaTile<kF8, kBf16, kD, kN>;
+  using Tile = MmaTile<kType, kD, kN>;
   static constexpr int kHeads = Tile::kHeads, kRows = Tile::kR, kUnits = kSms * Tile::kBlocks * kWarps;
   static constexpr int kLeast = 64 / kRows;  // tiles: short stretches leave parts that cost more to join than they save
   static int launch(const AttendArgs& a, bool, cudaStream_t s) {
     static std::atomic<bool> done[kMaxDevices];
     int dev = 0, n_sm = 0;
     if (!device_sm_count(&dev, &n_sm)) return KB_ERR_LAUNCH;
-    KB_CUDA_TRY(opt_in_smem_once(paged_attend_mma_kernel<kF8, kBf16, kD, kN>, Tile::kSmem, dev, done));
-    paged_attend_mma_kernel<kF8, kBf16, kD, kN><<<kb_cdiv_i32(a.units, kWarps), kThreads, Tile::kSmem, s>>>(a);
+    KB_CUDA_TRY(opt_in_smem_once(paged_attend_mma_kernel<kType, kD, kN>, Tile::kSmem, dev, done));
+    paged_attend_mma_kernel<kType, kD, kN><<<kb_cdiv_i32(a.units, kWarps), kThreads, Tile::kSmem, s>>>(a);
     KB_LAUNCH_CHECK("paged_attend_mma_kernel");
     return KB_OK;
   }
@@ -870,11 +971,19 @@ struct GenericKernel {
 };
 
 // f(a kernel): the one for the call
-template <bool kF8, bool kBf16, typename F>
+template <int kType, int kD, typename F>
+auto with_eights(const kb_paged_attention_params& p, F f) {
+  // as few items as three eights of heads each allow (two in fp32: registers), and those alike
+  const int32_t eights = kb_cdiv_i32(p.H / p.cache.H_kv, 8), most = kType == KB_F32 ? 2 : 3, n = kb_cdiv_i32(eights, kb_cdiv_i32(eights, most));
+  if (n == 1) return f(MmaKernel<kType, kD, 1>());
+  if constexpr (kType != KB_F32) {
+    if (n == 3) return f(MmaKernel<kType, kD, 3>());
+  }
+  return f(MmaKernel<kType, kD, 2>());
+}
+template <int kType, typename F>
 auto with_mma(const kb_paged_attention_params& p, F f) {
-  const bool eight = p.H / p.cache.H_kv <= 8;
-  if (p.cache.D == 64) return eight ? f(MmaKernel<kF8, kBf16, 64, 1>()) : f(MmaKernel<kF8, kBf16, 64, 2>());
-  return eight ? f(MmaKernel<kF8, kBf16, 128, 1>()) : f(MmaKernel<kF8, kBf16, 128, 2>());
+  return p.cache.D == 64 ? with_eights<kType, 64>(p, f) : with_eights<kType, 128>(p, f);
 }
 template <typename T, int D, typename F>
 auto with_group(const kb_paged_attention_params& p, F f) {
@@ -893,7 +1002,14 @@ auto with_generic(const kb_paged_attention_params& p, F f) {
 template <typename F>
 auto with_kernel(const kb_paged_attention_params& p, F f) {
   const int32_t dtype = p.cache.dtype;
-  if (takes_mma(p)) return dtype == KB_E4M3 ? with_mma<true, false>(p, f) : dtype == KB_BF16 ? with_mma<false, true>(p, f) : with_mma<false, false>(p, f);
+  if (takes_mma(p)) {
+    switch (dtype) {
+      case KB_F32: return with_mma<KB_F32>(p, f);
+      case KB_F16: return with_mma<KB_F16>(p, f);
+      case KB_BF16: return with_mma<KB_BF16>(p, f);
+      default: return with_mma<KB_E4M3>(p, f);
+    }
+  }
   switch (dtype) {
     case KB_F32: return with_generic<float>(p, f);
     case KB_F16: return with_generic<__half>(p, f);
