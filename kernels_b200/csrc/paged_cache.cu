@@ -242,6 +242,18 @@ struct Team {
   int (*of_rank)[8];    // [2][ranks]
   int size, rank, turn; // of the cluster
 
+  // `x` into `to`, a variable of every block's shared memory
+  __device__ __forceinline__ void tell(uint32_t* to, uint32_t x) const {
+    if (size == 1) {
+      *to = x;
+      return;
+    }
+    for (int r = 0; r < size; ++r) {
+      uint32_t there;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(sm100::smem_u32(to)), "r"(r));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(x) : "memory");
+    }
+  }
   // op over the team's warps of `x` (the same in a warp's lanes); `before`: over the warps before this one only
   template <typename Op>
   __device__ __forceinline__ int all(int x, int none, Op op, int* before = nullptr) {
@@ -304,12 +316,10 @@ struct SelectHead {
 __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
   __shared__ int red[2][32], of_rank[2][8];
   __shared__ uint32_t few[1024];
-  __shared__ int few_n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   Team team{red, of_rank, a.cluster, (int)blockIdx.x % a.cluster, 0};
   const SelectHead s(a, blockIdx.y, blockIdx.x / a.cluster);
   const int32_t n = s.n, row0 = (team.rank * warps + warp) * kWarpRows + lane;
-  if (threadIdx.x == 0) few_n = 0;
   if (a.cluster > 1) sm100::cluster_sync_all();  // (a block's shared memory may be written once the block has started)
 
   uint32_t key[kKeys];
@@ -349,18 +359,29 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
     else over = reach;
   }
   if (bit && reached != a.budget) {
+    // every block of the team gets all of them and goes on by itself
     const uint32_t most = least + (bit - 1) + bit;  // (no more than 2^32 - 1)
+    const int many = reached - over, others = over;
+    uint32_t picked = 0;
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) picked |= (uint32_t)(key[j] >= least && key[j] <= most && row0 + j * 32 < n) << j;
+    int at = __popc(picked), before;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, at, x);
+      if (lane >= x) at += y;
+    }
+    team.sum(__shfl_sync(0xffffffffu, at, 31), &before);
+    at += before - __popc(picked);
 #pragma unroll
     for (int j = 0; j < kKeys; ++j)
-      if (key[j] >= least && key[j] <= most && row0 + j * 32 < n) few[atomicAdd(&few_n, 1)] = key[j];  // (in any order: they are counted)
-    __syncthreads();
-    const bool here = threadIdx.x < few_n;
+      if ((picked >> j) & 1) team.tell(&few[at++], key[j]);
+    if (team.size > 1) sm100::cluster_sync_all();
+    else __syncthreads();
+    const bool here = threadIdx.x < many;
     const uint32_t mine = here ? few[threadIdx.x] : 0u;
-    const int others = over;
     for (; bit && reached != a.budget; bit >>= 1) {
-      int reach = __syncthreads_count(here && mine >= (least | bit));
-      if (a.cluster > 1) reach = team.sum(warp == 0 ? reach : 0);
-      reach += others;
+      const int reach = others + __syncthreads_count(here && mine >= (least | bit));
       if (reach >= a.budget) least |= bit, reached = reach;
       else over = reach;
     }

@@ -53,6 +53,12 @@ def write(k, v, k_pages, v_pages, table, lens, new_lens=None, positions=None, we
                     pages[at[0], :, at[1]] = x[b, :, t]
 
 
+def _rows(pages, page, head, row):
+    if pages.dtype == torch.float8_e4m3fn:  # (indexing does not take 8-bit floats)
+        return pages.view(torch.uint8)[page, head, row].view(torch.float8_e4m3fn).double()
+    return pages[page, head, row].double()
+
+
 def attend(q, k_pages, v_pages, table, lens, context_size=None, back=0, sm_scale=None, k_scale=None, v_scale=None):
     """``(o [B, H, D], lse [B, H], weights [B, H, capacity], spread)`` in fp64.  ``spread``: for tolerances, per head the largest
     ``sum |q_d k_d|`` of a row, and per output element the sum of ``p |v|``."""
@@ -74,9 +80,9 @@ def attend(q, k_pages, v_pages, table, lens, context_size=None, back=0, sm_scale
         pg, ro = (torch.tensor([at[i] for _, at in rows]) for i in (0, 1))
         for h in range(H):
             g = h // (H // H_kv)
-            k, v = k_pages.double()[pg, g, ro], v_pages.double()[pg, g, ro]
+            k, v = _rows(k_pages, pg, g, ro), _rows(v_pages, pg, g, ro)
             if k_scale is not None:
-                k, v = k * k_scale.double()[pg, g, ro][:, None], v * v_scale.double()[pg, g, ro][:, None]
+                k, v = k * k_scale[pg, g, ro].double()[:, None], v * v_scale[pg, g, ro].double()[:, None]
             s = (k @ q[b, h].double()) * sm_scale
             p = s.softmax(0)
             o[b, h], lse[b, h], w[b, h, idx] = p @ v, s.logsumexp(0) / math.log(2), p

@@ -112,6 +112,14 @@ def check_attend(c, q, context_size=None, back=0, sm_scale=None, weights=None, o
     (4, 1, 256, 8, [77], F16, F8),
     (16, 16, 64, 32, [513, 512, 511], F16, F16),                    # every head with keys of its own
     (40, 2, 128, 64, [400, 100], BF16, F8),                         # groups of twenty
+    (20, 1, 64, 16, [333, 40], BF16, F8),
+    (24, 1, 128, 32, [257, 90], F16, F16),
+    (17, 1, 64, 16, [257, 90, 0], BF16, BF16),
+    (50, 2, 64, 16, [100, 33], F16, F16),                           # more heads than an item takes, unevenly
+    (9, 1, 64, 16, [200, 17], F32, F32),
+    (24, 2, 128, 48, [200, 17, 1], F32, F32),
+    (20, 1, 128, 16, [300], F32, F32),
+    (3, 3, 128, 64, [700, 64], F32, F32),
 ])
 @pytest.mark.parametrize("weigh", [False, True])
 def test_attention_matches_definition(H, H_kv, D, page, lens, q_dtype, dtype, weigh):
@@ -138,6 +146,26 @@ def test_attention_splits_long_rows(dtype):
         c = make_cache(len(lens), 2, 128, 64, lens, dtype)
         q = torch.randn(len(lens), 8, 128, generator=torch.Generator().manual_seed(9)).to(F32 if dtype == F32 else BF16)
         check_attend(c, q, weights=torch.zeros(len(lens), 2, c["page_table"].shape[1] * 64))
+
+
+@pytest.mark.parametrize("dtype,D,H_kv,B", [(BF16, 128, 8, 260), (F16, 64, 16, 90), (F8, 128, 8, 170), (F32, 64, 8, 260), (F32, 128, 4, 180), (BF16, 32, 8, 90)])
+def test_attention_of_many_sequences(dtype, D, H_kv, B):
+    """More sequences and heads than there are warps (or blocks) to work on them: several to a warp, some cut in two, one very long, some empty."""
+    g = torch.Generator().manual_seed(5)
+    lens = torch.randint(0, 90, (B,), generator=g).tolist()
+    lens[3], lens[17], lens[B - 1] = 2500, 700, 333
+    c = make_cache(B, H_kv, D, 16, lens, dtype)
+    q = torch.randn(B, H_kv, D, generator=g).to(F32 if dtype == F32 else F16 if dtype == F16 else BF16)
+    check_attend(c, q, weights=torch.zeros(B, H_kv, c["page_table"].shape[1] * 16))
+
+
+@pytest.mark.parametrize("dtype,D,H_kv,B", [(BF16, 128, 16, 110), (F16, 64, 16, 74), (F8, 64, 16, 73), (F32, 128, 4, 148), (BF16, 256, 8, 70)])
+def test_attention_of_sequences_of_one_length(dtype, D, H_kv, B):
+    """About as many sequences and heads as there are warps, and much the same lengths: none is cut in two.  Then one that is longer."""
+    q = torch.randn(B, H_kv, D, generator=torch.Generator().manual_seed(6)).to(F32 if dtype == F32 else F16 if dtype == F16 else BF16)
+    for longest in (70, 300):
+        c = make_cache(B, H_kv, D, 16, [60 + b % 11 for b in range(B - 1)] + [longest], dtype, M=20)
+        check_attend(c, q, weights=torch.zeros(B, H_kv, 320))
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, F8])
@@ -215,6 +243,7 @@ def test_attention_takes_any_layout(dtype):
         if dtype == F8:
             changed |= dict(k_scale=other(g["k_scale"]), v_scale=g["v_scale"].transpose(0, 2).contiguous().transpose(0, 2))
         check_attend(c, q, on_gpu=changed)
+    check_attend(c, q, on_gpu=dict(g, v_pages=other(g["v_pages"])))  # keys and values of different layouts
     del scale, ref
     for qs in (q.cuda().transpose(0, 1).contiguous().transpose(0, 1), q.cuda().transpose(1, 2).contiguous().transpose(1, 2)):
         a = paged_attention(qs, g["k_pages"], g["v_pages"], g["page_table"], g["lens"], k_scale=g.get("k_scale"), v_scale=g.get("v_scale"))
