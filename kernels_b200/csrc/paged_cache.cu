@@ -2,8 +2,8 @@
 // weight that they have received.
 //
 // WRITE.  Token t < n_b of sequence b goes to row len_b - n_b + t.  HBM-bound: every element is read once and written
-// once.  A row of one head is eight elements per thread, D / 8 neighbouring threads: its largest magnitude, which sets
-// the scale of an 8-bit row, is a few shuffles away, and rows stay independent of one another.
+// once.  A row of one head is eight or sixteen elements per thread, a few neighbouring threads: its largest magnitude, which sets
+// the scale of an 8-bit row, is a few shuffles away.  The threads look up a token's place once and walk over its heads.
 //
 // EVICT.  Rows rank by (position among the newest `recent`, then weight, then the lower row); the first `budget` stay.
 // The kept rows below the budget stay where they are, and the i-th kept row behind it moves to the i-th place that came
@@ -22,7 +22,7 @@ namespace {
 
 // ---- write -----------------------------------------------------------------------------------------------------------
 
-constexpr int kWriteThreads = 256, kPerThread = 8;
+constexpr int kWriteThreads = 256;
 
 struct WriteArgs {
   PagedView c;
@@ -39,65 +39,65 @@ struct WriteArgs {
   KbFastDiv fd_T;
 };
 
-template <typename T>
-struct Eight { T v[kPerThread]; };
+template <typename T, int N>
+struct Several { T v[N]; };
 
-template <typename T, bool kAligned>
-__device__ __forceinline__ void load8(Eight<T>& e, const T* x, int64_t sd) {
+template <typename T, int N, bool kAligned>
+__device__ __forceinline__ void load_several(Several<T, N>& e, const T* x, int64_t sd) {
   if constexpr (kAligned) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(&e)[i] = __ldcs(reinterpret_cast<const uint4*>(x) + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) e.v[i] = x[i * sd];
+    for (int i = 0; i < N; ++i) e.v[i] = x[i * sd];
   }
 }
-template <typename T, bool kAligned>
-__device__ __forceinline__ void store8(T* out, const Eight<T>& e) {
-  if constexpr (kAligned && sizeof(T) == 1) {
-    *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(&e);
-  } else if constexpr (kAligned) {
+template <typename T, int N, bool kAligned>
+__device__ __forceinline__ void store_several(T* out, const Several<T, N>& e) {
+  if constexpr (kAligned) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(e) / 16; ++i) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(&e)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) out[i] = e.v[i];
+    for (int i = 0; i < N; ++i) out[i] = e.v[i];
   }
 }
 
 // The largest magnitude's bits.  Bits without the sign: numbers keep their order, and a NaN is above them all, so that it reaches the scale.
-__device__ __forceinline__ uint32_t largest_bits(const Eight<float>& e) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) m = max(m, __float_as_uint(e.v[i]) & 0x7fffffffu);
-  return m;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t largest_bits(const Eight<T>& e) {
+template <typename T, int N>
+__device__ __forceinline__ uint32_t largest_bits(const Several<T, N>& e) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(&e);
-  const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
-  const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
-  return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&h)));
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, w[i] & 0x7fffffffu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&h)));
+  }
 }
 
 // The row's elements as its 8-bit form holds them: x / scale correctly rounded (div_by, two at a time), then rounded to e4m3.
-template <typename T>
-__device__ __forceinline__ Eight<uint8_t> quantize8(const Eight<T>& e, float scale, float r) {
-  float f[kPerThread];
+template <typename T, int N>
+__device__ __forceinline__ Several<uint8_t, N> quantize(const Several<T, N>& e, float scale, float r) {
+  float f[N];
   if (scale <= 1e37f) {
     const uint64_t r2 = sm100::f2_pack(r, r), down = sm100::f2_pack(-scale, -scale);
 #pragma unroll
-    for (int i = 0; i < kPerThread; i += 2) {
+    for (int i = 0; i < N; i += 2) {
       const uint64_t x = sm100::f2_pack(to_f32(e.v[i]), to_f32(e.v[i + 1])), q = sm100::f2_mul(x, r2);
       sm100::f2_unpack(sm100::f2_fma(sm100::f2_fma(q, down, x), r2, q), f[i], f[i + 1]);
     }
   } else {  // an infinity or a NaN in the row
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) f[i] = to_f32(e.v[i]) / scale;
+    for (int i = 0; i < N; ++i) f[i] = to_f32(e.v[i]) / scale;
   }
-  Eight<uint8_t> out;
+  Several<uint8_t, N> out;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < N / 4; ++i) {
     // the signs as they come: the correction above turns -0 into 0
     uint32_t sign;
     const uint32_t* w = reinterpret_cast<const uint32_t*>(&e) + i * sizeof(T);
@@ -108,10 +108,15 @@ __device__ __forceinline__ Eight<uint8_t> quantize8(const Eight<T>& e, float sca
   return out;
 }
 
+// 8-bit rows: sixteen, so that a row's largest magnitude is three exchanges away instead of four (head dim 128).
+template <typename T, bool kF8>
+constexpr __host__ __device__ int elements_per_thread() { return kF8 ? 16 : 8; }
+
 // T: the tokens' type; kF8: the cache holds e4m3, otherwise T
 template <typename T, bool kF8, bool kAligned>
 __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteArgs a) {
-  const int lanes = a.D / kPerThread;  // 2, 4, 8, 16 or 32 threads per row
+  constexpr int kPerThread = elements_per_thread<T, kF8>();
+  const int lanes = a.D / kPerThread;  // a power of two up to 32
   const int lane = threadIdx.x & (lanes - 1), d = lane * kPerThread;
   const int64_t token = (int64_t)blockIdx.x * (kWriteThreads / lanes) + threadIdx.x / lanes;
   const int32_t h0 = blockIdx.y * a.heads_per_cta, h1 = kb_min_i32(h0 + a.heads_per_cta, a.H_kv);
@@ -135,8 +140,8 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteA
   }
   live = live && page >= 0;
   if (!__any_sync(0xffffffffu, live)) return;
-  // One head's keys and values in flight per thread leave room for more threads: 8 prompts of 4096-8192 tokens into 8-bit pages take 62 us
-  // with one, 65 with two, 68 with four.
+  // One head's keys and values in flight per thread leave room for more threads.  8 prompts of 4096-8192 tokens into 8-bit pages take 62 us with one,
+  // 65 with two, 68 with four (eight elements per thread; sixteen: 53 us, 6.0 TB/s).
   constexpr int kHeadsAtOnce = kF8 ? 1 : 2;
   using Out = typename std::conditional<kF8, uint8_t, T>::type;
   const T* from[2];
@@ -152,13 +157,13 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteA
   }
   const int64_t head[2] = {a.c.k_head, a.c.v_head}, scale_head[2] = {a.c.ks_head, a.c.vs_head};
   for (int32_t h2 = h0; h2 < h1; h2 += kHeadsAtOnce) {
-    Eight<T> e[kHeadsAtOnce][2];
+    Several<T, kPerThread> e[kHeadsAtOnce][2];
 #pragma unroll
     for (int u = 0; u < kHeadsAtOnce; ++u)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         if (live && h2 + u < h1) {
-          load8<T, kAligned>(e[u][w], from[w], a.sd[w]);
+          load_several<T, kPerThread, kAligned>(e[u][w], from[w], a.sd[w]);
         } else {
 #pragma unroll
           for (int i = 0; i < kPerThread; ++i) e[u][w].v[i] = from_f32<T>(0.f);
@@ -177,11 +182,11 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteA
           if (scale < 1e-12f) scale = 1e-12f;  // (a NaN stays)
           if (write) {
             if (lane == 0) *scale_to[w] = scale;
-            store8<uint8_t, kAligned>(to[w], quantize8(e[u][w], scale, 1.f / scale));
+            store_several<uint8_t, kPerThread, kAligned>(to[w], quantize(e[u][w], scale, 1.f / scale));
           }
           scale_to[w] += scale_head[w];
         } else if (write) {
-          store8<T, kAligned>(to[w], e[u][w]);
+          store_several<T, kPerThread, kAligned>(to[w], e[u][w]);
         }
         to[w] += head[w];
       }
@@ -191,7 +196,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteA
 template <typename T>
 int launch_write(const WriteArgs& in, bool f8, bool aligned, cudaStream_t s) {
   WriteArgs a = in;
-  const int64_t tokens = (int64_t)a.B * a.T, each = kWriteThreads / (a.D / kPerThread), ctas = (tokens + each - 1) / each;
+  const int64_t tokens = (int64_t)a.B * a.T, each = kWriteThreads / (a.D / (f8 ? elements_per_thread<T, true>() : elements_per_thread<T, false>())), ctas = (tokens + each - 1) / each;
   // few tokens: the heads go to blocks of their own
   a.heads_per_cta = ctas >= 148 * 4 ? a.H_kv : kb_min_i32(2, a.H_kv);
   const dim3 grid((unsigned)ctas, (unsigned)kb_cdiv_i32(a.H_kv, a.heads_per_cta));
