@@ -892,32 +892,33 @@ __global__ void __launch_bounds__(kMostJoinThreads) paged_join_kernel(const Atte
 
 // ---- rows' weights -------------------------------------------------------------------------------------------------------
 
+constexpr int kWeighRows = 1024;  // of a block, four per thread
+
 // A block takes rows of one sequence and key/value head; the group's log-sum-exps are the same for all of them.
 __global__ void __launch_bounds__(256) paged_weigh_kernel(const AttendArgs a) {
-  constexpr int kAtOnce = 4;
+  constexpr int kEach = kWeighRows / 256;
   const int32_t hk = blockIdx.y, b = blockIdx.z;
   const int64_t bh = (int64_t)b * a.H + hk * a.group;
   int32_t first, end;
   seen_rows(a, b, first, end);
   wait_for_launch_before();
-  const int32_t r = first + blockIdx.x * 256 + threadIdx.x;
-  if (r >= end) return;
-  const float *s = a.scores + bh * a.c.capacity + r, *lse = a.lse + bh;
-  float* to = a.weights + b * a.w_b + hk * a.w_h + r;
-  const float old = *to;
-  float w = 0.f;
-  for (int g0 = 0; g0 < a.group; g0 += kAtOnce) {
-    float x[kAtOnce], y[kAtOnce];
+  const int32_t r0 = first + blockIdx.x * kWeighRows + threadIdx.x;
+  if (r0 >= end) return;
+  const float *scores = a.scores + bh * a.c.capacity + r0, *lse = a.lse + bh;
+  float* to = a.weights + b * a.w_b + hk * a.w_h + r0;
+  float w[kEach], x[kEach];
 #pragma unroll
-    for (int g = 0; g < kAtOnce; ++g) {
-      const bool there = g0 + g < a.group;
-      x[g] = there ? __ldcs(s + (int64_t)(g0 + g) * a.c.capacity) : -INFINITY;
-      y[g] = there ? lse[g0 + g] : 0.f;
-    }
+  for (int i = 0; i < kEach; ++i) w[i] = 0.f;
+  for (int g = 0; g < a.group; ++g, scores += a.c.capacity) {
+    const float base = lse[g];
 #pragma unroll
-    for (int g = 0; g < kAtOnce; ++g) w += exp2f(x[g] - y[g]);
+    for (int i = 0; i < kEach; ++i) x[i] = r0 + i * 256 < end ? __ldcs(scores + i * 256) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) w[i] += sm100::ex2_approx(x[i] - base);
   }
-  *to = old + w;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (r0 + i * 256 < end) to[i * 256] += w[i];
 }
 
 // Whether the tensor-core kernel takes the call: head dim 64 or 128; dense heads of q, which has 16 bits where the cache has 8; keys and values of
@@ -1085,13 +1086,13 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
     if (int rc = kernel.launch(a, paged_rows_aligned(c, dtype_size(c.dtype)), s)) return rc;
     if (n.joins) {
       const dim3 grid((unsigned)(n.join_bytes / sizeof(int4)), kb_min_i32(n.heads, a.group));
-      // a group of D / 4 threads for about every part of an item
+      // a group of D / 4 threads for every second part of an item or so
       int32_t threads = 128;
-      while (threads < kMostJoinThreads && threads < (int64_t)n.units / n.items * (c.D / 4)) threads *= 2;
+      while (threads < kMostJoinThreads && threads < (int64_t)n.units / n.items * (c.D / 8)) threads *= 2;
       if (int rc = launch_after(paged_join_kernel, grid, threads, s, a)) return rc;
     }
     if (p.weights) {
-      const dim3 grid(kb_max_i32(1, kb_cdiv_i32(n.most_rows, 256)), c.H_kv, c.B);
+      const dim3 grid(kb_max_i32(1, kb_cdiv_i32(n.most_rows, kWeighRows)), c.H_kv, c.B);
       if (int rc = launch_after(paged_weigh_kernel, grid, 256, s, a)) return rc;
     }
     return (int)KB_OK;
