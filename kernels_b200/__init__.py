@@ -3,7 +3,8 @@
 
 Sub-packages mirror the reference's importable packages:
 
-* ``kernels_b200.streaming_attention`` — ``streaming_attention``, ``streaming_attention_reference``
+* ``kernels_b200.streaming_attention`` — ``streaming_attention``, ``streaming_attention_reference``, and beside them packed
+  batches, the streaming step, 8-bit inputs, the projections, rotary positions and the paged key/value cache
 * ``kernels_b200.self_attention`` — ``self_attention`` and its two torch references
 * ``kernels_b200.softmax`` — ``softmax``
 

@@ -143,6 +143,9 @@ def paged_attention(
     Returns ``o`` ``[B, H, D]`` and, on request, the base-2 log-sum-exp ``[B, H]``; both are 0 for a sequence that sees
     no row.  With ``weights``, the softmax weight of every row that is seen, summed over the query heads of its key/value
     head, is added to ``weights`` in place.
+
+    Sums are held in fp32.  16-bit and e4m3 caches: weights are rounded to 16 bits before they are multiplied with ``v``.  fp32 caches of head dim 64
+    and 128 are multiplied on the tensor cores in three parts, as exactly as in fp32; an infinity in a row counts as a NaN there.
     """
     c, index = _pages("paged_attention", k_pages, v_pages, page_table, lens, k_scale, v_scale)
     shape, dtype = q.shape, q.dtype
