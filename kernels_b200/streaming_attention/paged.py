@@ -20,6 +20,7 @@ workspace with torch on the current stream.  Forward only (inference).  There is
 from __future__ import annotations
 
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -28,9 +29,15 @@ from .. import _lib
 from .kernel import _clamp_i32
 
 
+_pack_write = _lib.packer(_lib.PagedWriteParams).pack
+_pack_attention = _lib.packer(_lib.PagedAttentionParams).pack
+_pack_evict = _lib.packer(_lib.PagedEvictParams).pack
+_NO_SCALES = (0,) * 8
+
+
 def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
-    """The checked cache as the C ABI's structure, and its device's index.  (A few microseconds of calls that take about twelve: every
-    property of a tensor is asked for once, devices by their index.)"""
+    """The checked cache: the numbers of the C ABI's ``kb_paged_cache``, the device's index and the rows that a table names.  (A few microseconds
+    of calls that take about ten: every property of a tensor is asked for once, devices by their index.)"""
     if not (k_pages.is_cuda and v_pages.is_cuda):
         raise RuntimeError(f"{what}: the tensors must live on a CUDA device (there is no CPU path)")
     index, shape, dtype = k_pages.get_device(), k_pages.shape, k_pages.dtype
@@ -45,35 +52,40 @@ def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
     assert lens_shape[0] == B, "one table row and one length per sequence"
     f8 = dtype == torch.float8_e4m3fn
     assert (k_scale is not None) == (v_scale is not None) == f8, "8-bit pages, and only those, come with scales"
-    c = _lib.PagedCache()
-    c.k, c.v = k_pages.data_ptr(), v_pages.data_ptr()
-    c.k_stride[:], c.v_stride[:] = ks[:3], vs[:3]
+    scales, code = _NO_SCALES, _lib.KB_E4M3
     if f8:
         assert k_scale.shape == v_scale.shape == shape[:3] and k_scale.dtype == v_scale.dtype == torch.float32
         assert k_scale.get_device() == v_scale.get_device() == index
-        c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        c.k_scale_stride[:], c.v_scale_stride[:] = k_scale.stride(), v_scale.stride()
-    c.page_table, c.lens, c.lens_stride = page_table.data_ptr(), lens.data_ptr(), lens.stride(0)
-    c.table_stride[:] = page_table.stride()
-    c.B, c.H_kv, c.D, c.P, c.M, c.page = B, H_kv, D, P, M, page
-    c.dtype = _lib.KB_E4M3 if f8 else _lib.dtype_code(dtype)
-    return c, index
+        scales = k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride()
+    else:
+        code = _lib.dtype_code(dtype)
+    cache = (k_pages.data_ptr(), v_pages.data_ptr(), *ks[:3], *vs[:3], *scales, page_table.data_ptr(), *page_table.stride(), lens.data_ptr(), lens.stride(0),
+             B, H_kv, D, P, M, page, code)
+    return cache, index, M * page
 
 
-def _per_row(name, x, dtype, c, index):
+def _per_row(name, x, dtype, B, H_kv, rows, index):
     """Pointer and strides of ``weights`` or ``row_positions``."""
     shape, strides = x.shape, x.stride()
-    assert x.dtype == dtype and x.get_device() == index and len(shape) == 3 and shape[0] == c.B and shape[1] == c.H_kv, f"{name} is [B, H_kv, M * page]"
-    assert shape[2] >= c.M * c.page and (strides[2] == 1 or shape[2] <= 1), f"{name} has an entry for every row, side by side"
-    assert (strides[0] or shape[0] <= 1) and (strides[1] or shape[1] <= 1), f"{name} is written: every sequence and head has entries of its own"
-    return x.data_ptr(), strides[:2]
+    assert x.dtype == dtype and x.get_device() == index and len(shape) == 3 and shape[0] == B and shape[1] == H_kv, f"{name} is [B, H_kv, M * page]"
+    assert shape[2] >= rows and (strides[2] == 1 or shape[2] <= 1), f"{name} has an entry for every row, side by side"
+    assert (strides[0] or B <= 1) and (strides[1] or H_kv <= 1), f"{name} is written: every sequence and head has entries of its own"
+    return x.data_ptr(), strides[0], strides[1]
 
 
-def _workspace(p, n, like):
-    """``n`` bytes on the device of ``like`` (int32); the caller holds them until the launch has been made."""
-    w = like.new_empty((n + 3) // 4)
-    p.workspace, p.workspace_bytes = w.data_ptr(), n
-    return w
+def _launch(entry, sizes, block, at, like):
+    """Launch with a workspace of the bytes that ``sizes`` asks for, on the device of ``like`` (int32); its address and size go to ``at`` of the
+    packed ``block``."""
+    lib = _lib.load()
+    n = getattr(lib, sizes)(block)
+    if n:
+        workspace = like.new_empty((n + 3) // 4)
+        block = block[:at] + _POINTER_AND_SIZE.pack(workspace.data_ptr(), n) + block[at + 16:]
+    _lib.check(_lib.launch_packed(getattr(lib, entry), block, like.device), entry)
+
+
+_POINTER_AND_SIZE = struct.Struct("=QQ")
+_NONE3 = (0, 0, 0)
 
 
 def paged_cache_write(
@@ -98,28 +110,26 @@ def paged_cache_write(
     0, those of ``row_positions`` the tokens' ``positions`` (int32 ``[B, T]``, None for the rows themselves).  Rows outside the table
     are dropped; two tokens of one call must not share a row of a page.
     """
-    c, index = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale)
+    cache, index, rows = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale)
     shape, dtype = k.shape, k.dtype
     assert len(shape) == 4 and v.shape == shape and v.dtype == dtype and k.get_device() == v.get_device() == index
     B, H_kv, T, D = shape
-    assert B == c.B and H_kv == c.H_kv and D == c.D, "k and v are [B, H_kv, T, D]"
+    pages_shape, lens_shape = k_pages.shape, lens.shape
+    assert B == lens_shape[0] and H_kv == pages_shape[1] and D == pages_shape[3], "k and v are [B, H_kv, T, D]"
     assert k_scale is not None or dtype == k_pages.dtype, "k and v have the pages' type"
-    p = _lib.PagedWriteParams()
-    p.cache = c
-    p.k, p.v = _lib.tensor4(k), _lib.tensor4(v)
-    p.T, p.dtype = T, _lib.dtype_code(dtype)
+    new = at = (0, 0, 0)
     if new_lens is not None:
-        assert new_lens.shape == lens.shape and new_lens.dtype == torch.int32 and new_lens.get_device() == index
-        p.new_lens, p.new_lens_stride = new_lens.data_ptr(), new_lens.stride(0)
+        assert new_lens.shape == lens_shape and new_lens.dtype == torch.int32 and new_lens.get_device() == index
+        new = new_lens.data_ptr(), new_lens.stride(0)
     if positions is not None:
         assert positions.shape == (B, T) and positions.dtype == torch.int32 and positions.get_device() == index
-        p.positions = positions.data_ptr()
-        p.positions_stride[:] = positions.stride()
-    if weights is not None:
-        p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, index)
-    if row_positions is not None:
-        p.row_positions, p.row_positions_stride[:] = _per_row("row_positions", row_positions, torch.int32, c, index)
-    _lib.check(_lib.launch(_lib.load().kb_paged_write, p, k_pages.device), "kb_paged_write")
+        at = positions.data_ptr(), *positions.stride()
+    block = _pack_write(
+        *cache, k.data_ptr(), *k.stride(), v.data_ptr(), *v.stride(), new[0], new[1], *at,
+        *(_NONE3 if weights is None else _per_row("weights", weights, torch.float32, B, H_kv, rows, index)),
+        *(_NONE3 if row_positions is None else _per_row("row_positions", row_positions, torch.int32, B, H_kv, rows, index)),
+        T, _lib.dtype_code(dtype))
+    _lib.check(_lib.launch_packed(_lib.load().kb_paged_write, block, k_pages.device), "kb_paged_write")
 
 
 def paged_attention(
@@ -147,12 +157,13 @@ def paged_attention(
     Sums are held in fp32.  16-bit and e4m3 caches: weights are rounded to 16 bits before they are multiplied with ``v``.  fp32 caches of head dim 64
     and 128 are multiplied on the tensor cores in three parts, as exactly as in fp32; an infinity in a row counts as a NaN there.
     """
-    c, index = _pages("paged_attention", k_pages, v_pages, page_table, lens, k_scale, v_scale)
-    shape, dtype = q.shape, q.dtype
+    cache, index, rows = _pages("paged_attention", k_pages, v_pages, page_table, lens, k_scale, v_scale)
+    shape, dtype, pages_shape = q.shape, q.dtype, k_pages.shape
     assert len(shape) == 3 and q.get_device() == index, "q is [B, H, D]"
     B, H, D = shape
-    assert B == c.B and D == c.D, "q is [B, H, D]"
-    assert c.H_kv >= 1 and H % c.H_kv == 0, "query heads share the key/value heads evenly"
+    H_kv = pages_shape[1]
+    assert B == lens.shape[0] and D == pages_shape[3], "q is [B, H, D]"
+    assert H_kv >= 1 and H % H_kv == 0, "query heads share the key/value heads evenly"
     assert k_scale is not None or dtype == k_pages.dtype, "q has the pages' type"
     assert context_size is None or context_size >= 1
     assert back_contexts >= 0
@@ -160,24 +171,14 @@ def paged_attention(
     if strides[2] != 1 or strides[0] % 2 or strides[1] % 2 or q.data_ptr() % 4:
         q = q.contiguous()  # (the tensor-core kernel takes pairs of elements)
         strides = q.stride()
-    p = _lib.PagedAttentionParams()
-    p.cache = c
     o = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     lse = lens.new_empty((B, H), dtype=torch.float32) if return_lse or weights is not None else None
-    p.q, p.o = q.data_ptr(), o.data_ptr()
-    p.q_stride[:] = strides
-    if lse is not None:
-        p.lse = lse.data_ptr()
-    if weights is not None:
-        p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, index)
-    p.H, p.dtype = H, _lib.dtype_code(dtype)
-    if context_size is not None:
-        p.context_size, p.back_contexts = _clamp_i32(context_size), _clamp_i32(back_contexts)
-    p.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-    lib = _lib.load()
-    workspace = _workspace(p, lib.kb_paged_attention_workspace_bytes(p), lens)
-    _lib.check(_lib.launch(lib.kb_paged_attention, p, k_pages.device), "kb_paged_attention")
-    del workspace
+    block = _pack_attention(
+        *cache, q.data_ptr(), *strides, o.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        *(_NONE3 if weights is None else _per_row("weights", weights, torch.float32, B, H_kv, rows, index)), 0, 0,
+        H, _lib.dtype_code(dtype), 0 if context_size is None else _clamp_i32(context_size), 0 if context_size is None else _clamp_i32(back_contexts),
+        1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale))
+    _launch("kb_paged_attention", "kb_paged_attention_workspace_bytes", block, _lib.PagedAttentionParams.workspace.offset, lens)
     return (o, lse) if return_lse else o
 
 
@@ -205,22 +206,18 @@ def paged_cache_evict(
     ``out``: a ``(lens, weights, row_positions)`` to be written instead, not overlapping the given ones (entries of
     the rows that remain; the pages change all the same).  Sequences that share pages need copies of their own first.
     """
-    c, index = _pages("paged_cache_evict", k_pages, v_pages, page_table, lens, k_scale, v_scale)
+    cache, index, rows = _pages("paged_cache_evict", k_pages, v_pages, page_table, lens, k_scale, v_scale)
     assert budget >= 1 and recent >= 0, "at least one row stays"
-    p = _lib.PagedEvictParams()
-    p.cache = c
-    p.budget, p.recent = _clamp_i32(budget), _clamp_i32(recent)
+    B, H_kv = lens.shape[0], k_pages.shape[1]
+    w = _per_row("weights", weights, torch.float32, B, H_kv, rows, index)
+    p = _per_row("row_positions", row_positions, torch.int32, B, H_kv, rows, index)
     if out is None:
         out = (lens, weights, row_positions)
+        w_out, p_out = w, p
     else:
         assert len(out) == 3 and out[0].shape == lens.shape and out[0].dtype == torch.int32 and out[0].get_device() == index
-    p.lens_out, p.lens_out_stride = out[0].data_ptr(), out[0].stride(0)
-    p.weights, p.weights_stride[:] = _per_row("weights", weights, torch.float32, c, index)
-    p.row_positions, p.row_positions_stride[:] = _per_row("row_positions", row_positions, torch.int32, c, index)
-    p.weights_out, p.weights_out_stride[:] = _per_row("out[1]", out[1], torch.float32, c, index)
-    p.row_positions_out, p.row_positions_out_stride[:] = _per_row("out[2]", out[2], torch.int32, c, index)
-    lib = _lib.load()
-    workspace = _workspace(p, lib.kb_paged_evict_workspace_bytes(p), lens)
-    _lib.check(_lib.launch(lib.kb_paged_evict, p, k_pages.device), "kb_paged_evict")
-    del workspace
+        w_out = _per_row("out[1]", out[1], torch.float32, B, H_kv, rows, index)
+        p_out = _per_row("out[2]", out[2], torch.int32, B, H_kv, rows, index)
+    block = _pack_evict(*cache, *w, *p, *w_out, *p_out, out[0].data_ptr(), out[0].stride(0), 0, 0, _clamp_i32(budget), _clamp_i32(recent))
+    _launch("kb_paged_evict", "kb_paged_evict_workspace_bytes", block, _lib.PagedEvictParams.workspace.offset, lens)
     return out

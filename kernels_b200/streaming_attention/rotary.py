@@ -18,26 +18,26 @@ import torch
 from .. import _lib
 
 
+_pack = _lib.packer(_lib.RotaryParams).pack
+
+
 def _rotate(q, k, positions, inv_freq, ends, inverse):
-    p = _lib.RotaryParams()
     shape = q.shape
+    B, H, T, D = shape
     q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), None
-    p.q, p.q_out = _lib.tensor4(q), q_out.data_ptr()
-    p.B, p.H, p.T, p.D = shape
+    keys, keys_to, H_kv = (0, 0, 0, 0, 0), 0, 0
     if k is not None:
         k_shape = k.shape
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         if 0 not in k_shape:
-            p.k, p.k_out, p.H_kv = _lib.tensor4(k), k_out.data_ptr(), k_shape[1]
-    p.positions, p.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+            keys, keys_to, H_kv = (k.data_ptr(), *k.stride()), k_out.data_ptr(), k_shape[1]
     strides = positions.stride()
-    p.pos_stride[:] = strides if len(strides) == 3 else (strides[0], 0, strides[1])
-    p.R, p.axes = ends[-1], len(ends)
-    p.section_end[: len(ends)] = ends
-    p.pos64 = positions.dtype == torch.int64
-    p.dtype = _lib.dtype_code(q.dtype)
-    p.inverse = inverse
-    _lib.check(_lib.launch(_lib.load().kb_rotary, p, q.device), "kb_rotary")
+    if len(strides) == 2:
+        strides = strides[0], 0, strides[1]
+    block = _pack(q.data_ptr(), *q.stride(), *keys, q_out.data_ptr(), keys_to, positions.data_ptr(), *strides, inv_freq.data_ptr(),
+                  B, H, H_kv, T, D, ends[-1], len(ends), *ends, *(0,) * (8 - len(ends)),
+                  positions.dtype == torch.int64, _lib.dtype_code(q.dtype), inverse)
+    _lib.check(_lib.launch_packed(_lib.load().kb_rotary, block, q.device), "kb_rotary")
     return q_out, k_out
 
 

@@ -95,6 +95,28 @@ def test_call_refusals():
         assert lib.kb_rotary(C.byref(r), None) == status, change
 
 
+@pytest.mark.parametrize("cls", [_lib.PagedCache, _lib.RotaryParams, _lib.PagedWriteParams, _lib.PagedAttentionParams, _lib.PagedEvictParams, _lib.SaBwdParams])
+def test_packed_blocks_are_the_structures_bytes(cls):
+    """Every number of a block, nested structures and arrays included, lands where the C structure has it."""
+    def fill(x, numbers):
+        for name, kind in x._fields_:
+            if issubclass(kind, C.Structure):
+                fill(getattr(x, name), numbers)
+            elif issubclass(kind, C.Array):
+                for i in range(kind._length_):
+                    numbers.append(len(numbers) + 1)
+                    getattr(x, name)[i] = numbers[-1]
+            else:
+                numbers.append(len(numbers) + 1)
+                setattr(x, name, numbers[-1])
+        return numbers
+
+    block = cls()
+    numbers = fill(block, [])
+    packed = _lib.packer(cls)
+    assert packed.size == C.sizeof(cls) and packed.pack(*numbers) == bytes(block)
+
+
 def test_workspace_of_a_long_cache_passes_32_bits():
     lib = _lib.load()
     p = _lib.PagedAttentionParams()
