@@ -51,8 +51,9 @@ class _RotaryEmbedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
-        # (turned by the same function, so that gradients have gradients)
-        turn = lambda q, k: _RotaryEmbedding.apply(q, k, positions, inv_freq, ctx.ends, not ctx.inverse)  # noqa: E731
+        # (turned by the same function where gradients are to have gradients)
+        go = _RotaryEmbedding.apply if torch.is_grad_enabled() else _rotate
+        turn = lambda q, k: go(q, k, positions, inv_freq, ctx.ends, not ctx.inverse)  # noqa: E731
         need_q, need_k = ctx.needs_input_grad[:2]
         if need_q:
             dq, dk = turn(dq, dk if need_k else None)
