@@ -337,6 +337,16 @@ def plain_call(*tensors) -> bool:
     )
 
 
+def forward_ad_active() -> bool:
+    """Whether inputs may carry tangents (always assumed with a torch that does not say)."""
+    return not _can_tell_plain or _forward_ad._current_level >= 0
+
+
+def transforms_active() -> bool:
+    """Whether a functorch transform is under way."""
+    return _can_tell_plain and _transforms_active()
+
+
 def launch_count() -> int:
     return int(load().kb_launch_count())
 

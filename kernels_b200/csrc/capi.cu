@@ -427,7 +427,7 @@ int kb_rotary(const kb_rotary_params* p, void* stream) {
     if (p->section_end[i] < (i ? p->section_end[i - 1] : 0)) return KB_ERR_BAD_ARGUMENT;
   if (p->section_end[p->axes - 1] != p->R) return KB_ERR_BAD_ARGUMENT;
   if (kb::empty(p->B, p->H + (p->k.data ? p->H_kv : 0), p->T)) return KB_OK;
-  if (!p->q.data || !p->q_out || (p->k.data && !p->k_out) || !p->positions || !p->inv_freq) return KB_ERR_BAD_ARGUMENT;
+  if ((p->H > 0 && (!p->q.data || !p->q_out)) || (p->k.data && !p->k_out) || !p->positions || !p->inv_freq) return KB_ERR_BAD_ARGUMENT;
   if ((int64_t)p->B * p->T > (int64_t)1 << 30 || p->H > 65535 || p->H_kv > 65535) return KB_ERR_TOO_LARGE;
   return kb::rotary(*p, static_cast<cudaStream_t>(stream));
 }

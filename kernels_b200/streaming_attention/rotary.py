@@ -41,18 +41,28 @@ def _rotate(q, k, positions, inv_freq, ends, inverse):
     return q_out, k_out
 
 
+def _keep(ctx, inputs):
+    _, _, positions, inv_freq, ctx.ends, ctx.inverse = inputs
+    ctx.save_for_backward(positions, inv_freq)
+    ctx.save_for_forward(positions, inv_freq)
+
+
+def _turn(*inputs):
+    """:func:`_rotate` with gradients."""
+    return (_RotaryEmbeddingTransformed if _lib.transforms_active() else _RotaryEmbedding).apply(*inputs)
+
+
 class _RotaryEmbedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, ends, inverse):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.ends, ctx.inverse = ends, inverse
-        return _rotate(q, k, positions, inv_freq, ends, inverse)
+    def forward(ctx, *inputs):
+        _keep(ctx, inputs)
+        return _rotate(*inputs)
 
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         # (turned by the same function where gradients are to have gradients)
-        go = _RotaryEmbedding.apply if torch.is_grad_enabled() else _rotate
+        go = _turn if torch.is_grad_enabled() else _rotate
         turn = lambda q, k: go(q, k, positions, inv_freq, ctx.ends, not ctx.inverse)  # noqa: E731
         need_q, need_k = ctx.needs_input_grad[:2]
         if need_q:
@@ -60,6 +70,24 @@ class _RotaryEmbedding(torch.autograd.Function):
         else:
             dq, dk = None, turn(dk, None)[0]
         return dq, dk, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        positions, inv_freq = ctx.saved_tensors
+        turn = lambda x: None if x is None else _turn(x, None, positions, inv_freq, ctx.ends, ctx.inverse)[0]  # noqa: E731
+        return turn(tq), turn(tk)
+
+
+class _RotaryEmbeddingTransformed(_RotaryEmbedding):
+    """The form that functorch's transforms ask for (a call of it takes 20 microseconds more)."""
+
+    @staticmethod
+    def forward(q, k, positions, inv_freq, ends, inverse):
+        return _rotate(q, k, positions, inv_freq, ends, inverse)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _keep(ctx, inputs)
 
 
 def rotary_embedding(
@@ -90,6 +118,7 @@ def rotary_embedding(
     assert pos_shape[-1] == T and (len(pos_shape) == 2 or pos_shape[1] == B), "positions are [A, T] or [A, B, T]"
     assert inv_freq.ndim == 1 and inv_freq.dtype == torch.float64 and inv_freq.get_device() == index
     R = inv_freq.shape[0]
+    assert not inv_freq.requires_grad, "the frequencies have no gradient"
     assert 1 <= R <= D // 2, "as many frequencies as there are pairs, at most"
     sections = (R,) if sections is None else sections
     ends, end = [], 0
@@ -99,6 +128,6 @@ def rotary_embedding(
     assert 1 <= len(ends) <= 8 and len(ends) == pos_shape[0], "one section of frequencies per axis, at most 8"
     assert end == R and min(sections) >= 0, "the sections share out inv_freq"
     inv_freq = inv_freq.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryEmbedding.apply(q, k, positions, inv_freq, ends, False)
+    if _lib.forward_ad_active() or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+        return _turn(q, k, positions, inv_freq, ends, False)
     return _rotate(q, k, positions, inv_freq, ends, False)

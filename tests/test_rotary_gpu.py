@@ -107,6 +107,8 @@ def test_rotary_empty_calls():
     q, k = torch.randn(2, 2, 3, 16, device="cuda"), torch.randn(2, 0, 3, 16, device="cuda")
     y, z = rotary_embedding(q, k, torch.zeros(1, 2, 3, dtype=torch.int32, device="cuda"), f)
     assert torch.equal(y, q) and z.shape == k.shape
+    y, z = rotary_embedding(k, q, torch.zeros(1, 2, 3, dtype=torch.int32, device="cuda"), f)
+    assert torch.equal(z, q) and y.shape == k.shape
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -166,6 +168,29 @@ def test_rotary_second_gradients_and_unused_outputs():
     assert d.shape == q.shape
 
 
+def test_rotary_under_transforms():
+    """Forward-mode tangents and functorch gradients turn with the tensors; a compiled caller gets the eager result."""
+    import torch.autograd.forward_ad as fw
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    sections = (4, 12)
+    q, k, positions, inv_freq = (x.cuda() for x in _inputs(2, 2, 1, 9, 64, 16, sections, F32, 50))
+    t = torch.randn_like(q)
+    want = rotary_embedding(q, k, positions, inv_freq, sections)
+    with fw.dual_level():
+        y, z = rotary_embedding(fw.make_dual(q, t), k, positions, inv_freq, sections)
+        y, tangent = fw.unpack_dual(y)
+        z, none = fw.unpack_dual(z)
+        assert torch.equal(y, want[0]) and torch.equal(z, want[1]) and (none is None or (none == 0).all())
+        assert torch.equal(tangent, rotary_embedding(t, None, positions, inv_freq, sections)[0])
+    g = torch.func.grad(lambda x: (rotary_embedding(x, None, positions, inv_freq, sections)[0] * t).sum())(q)
+    x = q.clone().requires_grad_()
+    (ref,) = torch.autograd.grad(rotary_embedding(x, None, positions, inv_freq, sections)[0], x, t)
+    assert torch.equal(g, ref)
+    compiled = torch.compile(lambda x, y: rotary_embedding(x * 1, y, positions, inv_freq, sections))
+    assert all(torch.equal(a, b) for a, b in zip(compiled(q, k), want))
+
+
 def test_rotary_in_a_graph_and_on_another_stream():
     from kernels_b200.streaming_attention import rotary_embedding
 
@@ -194,7 +219,7 @@ def test_rotary_refusals():
         dict(positions=positions.float()), dict(positions=positions[:, :1]), dict(positions=positions[0, 0]), dict(inv_freq=inv_freq.float()),
         dict(sections=(16, 16)), dict(sections=(31,)), dict(sections=(33, -1), positions=positions.expand(2, 2, 17)), dict(k=k.half()),
         dict(k=k[:1]), dict(inv_freq=torch.ones(33, dtype=torch.float64, device="cuda")), dict(positions=positions.cpu()),
-        dict(positions=positions.expand(9, 2, 17), sections=(32,) + (0,) * 8),
+        dict(positions=positions.expand(9, 2, 17), sections=(32,) + (0,) * 8), dict(inv_freq=inv_freq.clone().requires_grad_()),
     ]
     for change in bad:
         args = dict(q=q, k=k, positions=positions, inv_freq=inv_freq) | change
