@@ -40,7 +40,7 @@ struct AttendArgs {
   float scale_log2;
   int4* join;       // [items] with by_item, otherwise by the unit that starts the item, [units]: {first part (-1: none), its unit, last unit, item}
   float* part_o;    // [2 units, heads, D]
-  float2* part_ml;  // [2 units, heads]
+  float4* part_ml;  // [2 units, heads]: maximum, sum of the weights, sum of what was multiplied with V (the weights as rounded), 0
   float* scores;    // [B, H, capacity], base-2 logits
   KbFastDiv fd_context;
   uint32_t row16[3], scale_at[3];  // tensor-core kernel: page, head and row strides of keys and values in 16 bytes, of their scales in elements
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
         if (a.lse && d == 0) a.lse[bh] = sum == 0.f ? 0.f : base + log2f(sum);
       } else {
         a.part_o[((int64_t)slot * G + g) * D + d] = x;
-        if (d == 0) a.part_ml[(int64_t)slot * G + g] = make_float2(top, sum);
+        if (d == 0) a.part_ml[(int64_t)slot * G + g] = make_float4(top, sum, sum, 0.f);
       }
     }
     __syncthreads();  // (q_s and o_s are the next item's)
@@ -353,7 +353,9 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
 // 2^14: what is lost lies 2^-38 below the largest).  A row's value scale belongs to its weight: the weights that are
 // multiplied are p * v_scale, so the running maximum is taken over score + log2(v_scale), which keeps them within f16.
 // f16 weights start at 2^7 and may grow to 2^15 before sums are rescaled: seven bits more for the small ones.
-// Weights are rounded to 16 bits for the product with V (as in the operator's forward kernel); their sum is taken before that.
+// Weights are rounded to 16 bits for the product with V (as in the operator's forward kernel).  A 16-bit cache's output is divided by the sum of
+// the rounded weights, so that what their roundings have in common cancels (one row that outweighs the others comes out exact); the
+// log-sum-exp is that of the weights as they were.
 //
 // fp32 is cut in two: x = hi + lo, hi the 11 leading bits (tf32), lo the next 11, and a product is hi hi + lo hi + hi lo, which leaves out
 // some 2^-23 of it (and makes NaN of what fp32 has infinities for).  The tensor cores cut sums off where an addition rounds, so what they add to a long sum goes in by an addition.  (On CUDA cores a row costs 4 D flops per query head and the sums over lanes besides: 16 sequences of 4096 rows,
@@ -383,6 +385,10 @@ __device__ __forceinline__ float lds_f32(uint32_t at) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
   return x;
 }
+template <bool BF16>
+__device__ __forceinline__ float low16(uint32_t two) { return BF16 ? __uint_as_float(two << 16) : __half2float(__ushort_as_half((unsigned short)two)); }
+template <bool BF16>
+__device__ __forceinline__ float high16(uint32_t two) { return BF16 ? __uint_as_float(two & 0xffff0000u) : __half2float(__ushort_as_half((unsigned short)(two >> 16))); }
 // an 8 x 8 matrix of 16-bit elements, a row per four lanes, turned over
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -445,7 +451,7 @@ struct MmaTile {
 template <int kType, int kD, int kN>
 __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) paged_attend_mma_kernel(const AttendArgs a) {
   using Tile = MmaTile<kType, kD, kN>;
-  constexpr bool kF8 = kType == KB_E4M3, kBf16 = kType == KB_BF16, kF32 = kType == KB_F32;
+  constexpr bool kF8 = kType == KB_E4M3, kBf16 = kType == KB_BF16, kF32 = kType == KB_F32, kRounded = !kF8 && !kF32;
   constexpr int kR = Tile::kR, kStages = Tile::kStages, kChunks = Tile::kChunks, kRowBytes = Tile::kRowBytes, kHeads = Tile::kHeads;
   constexpr int kSteps = kD / 16, kU = kR / 16, kDt = kD / 16;
   constexpr float kOffset = kF8 || kType == KB_F16 ? 7.f : 0.f, kSlack = 8.f;
@@ -571,11 +577,14 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
     }
 
     // element (2 r + i) of a product's lane: key (or element of the head) oct + 8 r, query head 2 quad + i
-    float o[kDt][kN][4], m[kN][2], l[kN][2];
+    float o[kDt][kN][4], m[kN][2], l[kN][2], z[kRounded ? kN : 1][2];
 #pragma unroll
     for (int e = 0; e < kN; ++e) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) m[e][i] = -INFINITY, l[e][i] = 0.f;
+      for (int i = 0; i < 2; ++i) {
+        m[e][i] = -INFINITY, l[e][i] = 0.f;
+        if constexpr (kRounded) z[e][i] = 0.f;
+      }
 #pragma unroll
       for (int j = 0; j < kDt; ++j)
 #pragma unroll
@@ -718,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
             const float keep = to == -INFINITY ? 0.f : sm100::ex2_approx(m[e][i] - to);
             m[e][i] = to;
             l[e][i] *= keep;
+            if constexpr (kRounded) z[e][i] *= keep;
 #pragma unroll
             for (int j = 0; j < kDt; ++j) o[j][e][i] *= keep, o[j][e][2 + i] *= keep;
           }
@@ -739,8 +749,13 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
             float x = sm100::ex2_approx(sc[u][e][2 * r] - base[e][0]), y = sm100::ex2_approx(sc[u][e][2 * r + 1] - base[e][1]);
             l[e][0] += x, l[e][1] += y;
             if constexpr (kF8) x *= vs[u][r], y *= vs[u][r];
-            if constexpr (kF32) pf[e][2 * r] = x, pf[e][2 * r + 1] = y;
-            else p[e][r] = transpose8x8(sm100::pack16x2<kBf16>(x, y));
+            if constexpr (kF32) {
+              pf[e][2 * r] = x, pf[e][2 * r + 1] = y;
+            } else {
+              const uint32_t both = sm100::pack16x2<kBf16>(x, y);
+              if constexpr (kRounded) z[e][0] += low16<kBf16>(both), z[e][1] += high16<kBf16>(both);
+              p[e][r] = transpose8x8(both);
+            }
           }
         if constexpr (kF32) {
 #pragma unroll
@@ -811,17 +826,21 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
     for (int e = 0; e < kN; ++e)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float sum = l[e][i];
+        float sum = l[e][i], by_sum = kRounded ? z[kRounded ? e : 0][i] : 0.f;
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        for (int x = 4; x < 32; x <<= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          if constexpr (kRounded) by_sum += __shfl_xor_sync(0xffffffffu, by_sum, x);
+        }
+        if constexpr (!kRounded) by_sum = sum;
         const int g = 8 * e + 2 * quad + i;
         if (g >= heads) continue;
         const int64_t bh = (int64_t)b * a.H + h0 + g, part = (int64_t)slot * kHeads + g;
         // (a head without weights is 0 even where what it would be divided by is not: 0 * 0)
         const bool none = sum == 0.f;
-        const float by = slot >= 0 ? 1.f : 1.f / sum;
+        const float by = slot >= 0 ? 1.f : 1.f / by_sum;
         if (oct == 0) {
-          if (slot >= 0) a.part_ml[part] = make_float2(m[e][i] - kOffset, sum);
+          if (slot >= 0) a.part_ml[part] = make_float4(m[e][i] - kOffset, sum, by_sum, 0.f);
           else if (a.lse) a.lse[bh] = none ? 0.f : m[e][i] - kOffset + log2f(sum);
         }
 #pragma unroll
@@ -846,7 +865,7 @@ constexpr int kMostJoinThreads = 1024;
 
 // A block per item and head.  Groups of D / 4 threads take every so many-th part, four elements per thread; the groups are added up in order.
 __global__ void __launch_bounds__(kMostJoinThreads) paged_join_kernel(const AttendArgs a) {
-  __shared__ float red[kMostJoinThreads / 32], sums[kMostJoinThreads / 4], o_s[kMostJoinThreads * 4];
+  __shared__ float red[kMostJoinThreads / 32], sums[kMostJoinThreads / 4][2], o_s[kMostJoinThreads * 4];
   const int threads = blockDim.x;
   let_next_launch_start();
   wait_for_launch_before();
@@ -868,24 +887,24 @@ __global__ void __launch_bounds__(kMostJoinThreads) paged_join_kernel(const Atte
   const float base = top == -INFINITY ? 0.f : top;
 
   const int width = a.D / 4, groups = threads / width, group = threadIdx.x / width, d = (threadIdx.x - group * width) * 4;
-  float sum = 0.f;
+  float sum = 0.f, by = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int i = group; i < n; i += groups) {
-    const float2 e = a.part_ml[part_at(i)];
+    const float4 e = a.part_ml[part_at(i)];
     const float4 y = *reinterpret_cast<const float4*>(a.part_o + part_at(i) * a.D + d);
     const float keep = exp2f(e.x - base);
-    sum = fmaf(e.y, keep, sum);
+    sum = fmaf(e.y, keep, sum), by = fmaf(e.z, keep, by);
     x.x = fmaf(y.x, keep, x.x), x.y = fmaf(y.y, keep, x.y), x.z = fmaf(y.z, keep, x.z), x.w = fmaf(y.w, keep, x.w);
   }
   *reinterpret_cast<float4*>(o_s + group * a.D + d) = x;
-  if (d == 0) sums[group] = sum;
+  if (d == 0) sums[group][0] = sum, sums[group][1] = by;
   __syncthreads();
   const int64_t bh = (int64_t)b * a.H + h;
   for (int i = threadIdx.x; i < a.D; i += threads) {
-    float s = 0.f, y = 0.f;
-    for (int k = 0; k < groups; ++k) s += sums[k], y += o_s[k * a.D + i];
-    store_any(a.o, bh * a.D + i, a.dtype, s == 0.f ? 0.f : y / s);
+    float s = 0.f, z = 0.f, y = 0.f;
+    for (int k = 0; k < groups; ++k) s += sums[k][0], z += sums[k][1], y += o_s[k * a.D + i];
+    store_any(a.o, bh * a.D + i, a.dtype, s == 0.f ? 0.f : y / z);
     if (a.lse && i == 0) a.lse[bh] = s == 0.f ? 0.f : base + log2f(s);
   }
 }
@@ -1046,7 +1065,7 @@ Plan make_plan(const kb_paged_attention_params& p) {
   const size_t entries = n.by_item ? items : n.units, parts = 2 * (size_t)n.units * n.heads;
   n.join_bytes = entries * sizeof(int4);
   n.part_bytes = parts * c.D * sizeof(float);
-  n.ml_bytes = parts * sizeof(float2);
+  n.ml_bytes = parts * sizeof(float4);
   n.score_bytes = p.weights ? (size_t)c.B * p.H * capacity * sizeof(float) : 0;
   return n;
 }
@@ -1081,7 +1100,7 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
     char* w = static_cast<char*>(p.workspace);
     a.join = reinterpret_cast<int4*>(w), w += n.join_bytes;
     a.part_o = reinterpret_cast<float*>(w), w += n.part_bytes;
-    a.part_ml = reinterpret_cast<float2*>(w), w += n.ml_bytes;
+    a.part_ml = reinterpret_cast<float4*>(w), w += n.ml_bytes;
     if (p.weights) a.scores = reinterpret_cast<float*>(w);
     if (int rc = kernel.launch(a, paged_rows_aligned(c, dtype_size(c.dtype)), s)) return rc;
     if (n.joins) {
