@@ -252,18 +252,34 @@ def test_attention_takes_any_layout(dtype):
         assert torch.equal(a, b)
 
 
-def test_attention_in_a_cache_past_32_bit_offsets():
-    """The last pages of a cache of 2^32 elements and more."""
+def test_a_cache_past_32_bit_offsets():
+    """The last pages of pools of 2^32 elements and more: attended with, written, evicted from."""
+    from kernels_b200.streaming_attention import paged_cache_evict, paged_cache_write
+
     P, page, D = 17000, 2048, 128
-    k = torch.zeros(P, 1, page, D, dtype=F16, device="cuda")
+    k, v = (torch.zeros(P, 1, page, D, dtype=F16, device="cuda") for _ in range(2))
     assert k.numel() > 2**32
     c = make_cache(1, 1, D, page, [3000], F16, spare=0)
-    small = c["k_pages"]
+    order = c["page_table"][0].long()
     table = torch.tensor([[P - 1, P - 2]], dtype=torch.int32)
-    k[P - 1], k[P - 2] = small[c["page_table"][0, 0]].cuda(), small[c["page_table"][0, 1]].cuda()
+    for pool, small in ((k, c["k_pages"]), (v, c["v_pages"])):
+        pool[P - 1], pool[P - 2] = small[order[0]].cuda(), small[order[1]].cuda()
     q = torch.randn(1, 2, D).half()
-    c["v_pages"] = c["k_pages"]
-    check_attend(c, q, on_gpu=dict(k_pages=k, v_pages=k, page_table=table.cuda(), lens=c["lens"].cuda()))
+    g = dict(k_pages=k, v_pages=v, page_table=table.cuda(), lens=c["lens"].cuda())
+    check_attend(c, q, on_gpu=g)
+    check_attend(c, q, on_gpu=dict(g, v_pages=v.view(P, page, 1, D).transpose(1, 2)))  # (another layout on paper: the generic kernel)
+    weights, positions = make_books(1, 1, 2 * page)
+    books = weights.cuda(), positions.cuda()
+    x, y = (torch.randn(1, 1, 5, D).half() for _ in range(2))
+    c["lens"] += 5
+    g["lens"] += 5
+    PO.write(x, y, c["k_pages"], c["v_pages"], c["page_table"], c["lens"], None, None, weights, positions)
+    paged_cache_write(x.cuda(), y.cuda(), *g.values(), weights=books[0], row_positions=books[1])
+    PO.evict(c["k_pages"], c["v_pages"], c["page_table"], c["lens"], weights, positions, 2500, 100)
+    paged_cache_evict(*g.values(), *books, 2500, 100)
+    for pool, small in ((k, c["k_pages"]), (v, c["v_pages"])):
+        assert torch.equal(pool[P - 1].cpu(), small[order[0]]) and torch.equal(pool[P - 2].cpu(), small[order[1]]) and not pool[: P - 2].any()
+    assert torch.equal(books[0].cpu(), weights) and torch.equal(books[1].cpu(), positions) and g["lens"].tolist() == [2500]
 
 
 def test_attention_same_inputs_same_bits():
