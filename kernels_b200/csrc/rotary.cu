@@ -6,10 +6,11 @@
 // turns exactly, and at position p the angle is off by at most p * 2^-54 turns (the frequency comes with 53 bits),
 // where a product in fp32 would be off by p * 2^-24.
 //
-// HBM-bound: every element is read and written once, past the caches' order of use (__ldcs, __stcs).  A block takes a few tokens and forms the cosines and sines of their pairs
-// once, in shared memory; then its threads, each with one vector of pairs of one token, walk over the heads, several of them side by side.
-// 4 x 8192 tokens, 32 + 8 heads of 128, bf16: 119 us, 5.6 TB/s (0.86 of the measured copy); 8 x 4095 tokens, 16 + 16 heads of 64, f16, forward and backward:
-// 121 us; 64 tokens: 3.5 us on the device.
+// HBM-bound: every element is read and written once, past the caches' order of use (__ldcs, __stcs).  A block takes a few tokens and
+// forms the cosines and sines of their pairs once, in shared memory; then its threads, each with one vector of pairs of one
+// token, walk over the heads, several of them side by side.
+// 4 x 8192 tokens, 32 + 8 heads of 128, bf16: 119 us, 5.6 TB/s (0.86 of the measured copy); 8 x 4095 tokens, 16 + 16 heads of 64, f16,
+// forward and backward: 121 us; 64 tokens: 3.5 us on the device.
 #include "common.cuh"
 
 namespace kb {

@@ -87,7 +87,8 @@ def test_call_refusals():
     r = _lib.RotaryParams()
     r.q.data = r.q_out = r.positions = r.inv_freq = 4096
     good = dict(B=1, H=1, T=1, D=64, R=32, axes=1, dtype=_lib.KB_F16)
-    for change, status in [(dict(B=-1), BAD), (dict(H=-1), BAD), (dict(T=-1), BAD), (dict(D=65), UNSUPPORTED), (dict(dtype=3), UNSUPPORTED), (dict(R=0), BAD), (dict(R=33), BAD),
+    for change, status in [(dict(B=-1), BAD), (dict(H=-1), BAD), (dict(T=-1), BAD), (dict(D=65), UNSUPPORTED), (dict(dtype=3), UNSUPPORTED), (dict(R=0), BAD),
+                           (dict(R=33), BAD),
                            (dict(axes=0), BAD), (dict(axes=9), BAD), (dict(axes=2), BAD), (dict(T=1 << 30, B=2), TOO_LARGE), (dict(q_out=None), BAD)]:
         for n, x in (good | dict(q_out=4096) | change).items():
             setattr(r, n, x)
