@@ -438,10 +438,11 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
 __global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs a) {
   __shared__ int red[2][32], of_rank[2][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  Team team{red, of_rank, 1, 0, 0};
-  const SelectHead s(a, blockIdx.y, blockIdx.x);
-  const int per_warp = kb_cdiv_i32(kb_max_i32(s.n, 1), warps * 32) * 32;
-  const int begin = kb_min_i32(warp * per_warp, s.n), end = kb_min_i32(begin + per_warp, s.n);
+  Team team{red, of_rank, a.cluster, (int)blockIdx.x % a.cluster, 0};
+  const SelectHead s(a, blockIdx.y, blockIdx.x / a.cluster);
+  if (a.cluster > 1) sm100::cluster_sync_all();
+  const int per_warp = kb_cdiv_i32(kb_max_i32(s.n, 1), a.cluster * warps * 32) * 32;
+  const int begin = kb_min_i32((team.rank * warps + warp) * per_warp, s.n), end = kb_min_i32(begin + per_warp, s.n);
   const uint32_t below = (1u << lane) - 1;
   int32_t newest = INT32_MIN;
   for (int i = begin + lane; i < end; i += 32) {
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs
     newest = max(newest, s.pos[i]);
   }
   if (s.n <= a.budget) {
-    if (threadIdx.x == 0) *s.count = 0;
+    if (threadIdx.x == 0 && team.rank == 0) *s.count = 0;
     return;
   }
   newest = team.max(__reduce_max_sync(0xffffffffu, newest));
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs
     if (pass == 0) {
       team.sum(holes, &hole_at);
       const int moves = team.sum(movers, &mover_at);
-      if (threadIdx.x == 0) *s.count = moves;
+      if (threadIdx.x == 0 && team.rank == 0) *s.count = moves;
     }
   }
 }
@@ -575,7 +576,6 @@ int launch_select(const EvictArgs& in, int32_t heads, int32_t B, cudaStream_t s)
   a.cluster = 1;
   while (a.cluster < kMostCluster && capacity > a.cluster * kBlockRows) a.cluster *= 2;
   const bool held = capacity <= a.cluster * kBlockRows;
-  if (!held) a.cluster = 1;
   cudaLaunchConfig_t c = {};
   c.blockDim = dim3(held && a.cluster == 1 ? 32 * kb_cdiv_i32(capacity, kWarpRows) : 1024);
   c.gridDim = dim3((unsigned)(heads * a.cluster), (unsigned)B);
