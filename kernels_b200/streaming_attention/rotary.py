@@ -5,7 +5,8 @@ for every sequence.  Tokens of a video or an image stand on several axes (time, 
 newest tokens of a batch of streams stand at positions of their own.  Here every token brings its position on each axis,
 and every axis turns its own band of the frequencies.
 
-One kernel (``kb_rotary``), differentiable in ``q`` and ``k``: the gradient is the same kernel turning the other way.
+One kernel (``kb_rotary``), differentiable in ``q`` and ``k``: the gradient is the same kernel turning the other way.  A
+backward pass can be captured into a CUDA graph as any of torch's can, while no eager graph of the same leaves is alive.
 There is no CPU path.
 """
 

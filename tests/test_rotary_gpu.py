@@ -211,6 +211,26 @@ def test_rotary_in_a_graph_and_on_another_stream():
     assert torch.equal(y, want[0])
 
 
+def test_rotary_backward_in_a_graph():
+    """Forward and gradient captured together (no eager graph of the same leaf is alive: torch ends the process then, whatever the operator)."""
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    q, _, positions, inv_freq = (x.cuda() for x in _inputs(2, 4, 2, 17, 64, 32, (32,), BF16, 500))
+    g = torch.randn_like(q)
+    leaf = torch.zeros_like(q).requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, _ = rotary_embedding(leaf, None, positions, inv_freq)
+        (d,) = torch.autograd.grad(y, leaf, g)
+    with torch.no_grad():
+        leaf.copy_(q)
+    for scale in (1.0, -2.0):
+        g.copy_(torch.randn_like(g) * scale)
+        graph.replay()
+        assert torch.equal(y, rotary_embedding(q, None, positions, inv_freq)[0])
+        assert torch.equal(d, rotary_embedding(g, None, -positions, inv_freq)[0])
+
+
 def test_rotary_refusals():
     from kernels_b200.streaming_attention import rotary_embedding
 
