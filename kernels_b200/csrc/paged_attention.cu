@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
 //
 // e4m3 elements become f16, exactly.  q does too (bf16 q after a multiplication by a power of two that brings its largest element to
 // 2^14: what is lost lies 2^-38 below the largest).  A row's value scale belongs to its weight: the weights that are
-// multiplied are p * v_scale, so the running maximum is taken over score + log2(v_scale), which keeps them within f16.
+// multiplied are p * v_scale, so the running maximum is taken over score + log2(v_scale), which keeps them within f16.  (The row of an infinite
+// value is written with an infinite scale: its heads come out NaN, as 0 times infinity does; their log-sum-exp and weights do not depend on values.)
 // f16 weights start at 2^7 and may grow to 2^15 before sums are rescaled: seven bits more for the small ones.
 // Weights are rounded to 16 bits for the product with V (as in the operator's forward kernel).  A 16-bit cache's output is divided by the sum of
 // the rounded weights, so that what their roundings have in common cancels (one row that outweighs the others comes out exact); the
@@ -685,7 +686,10 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
           if constexpr (kF8) {
             ks = lds_f32(at + 2 * kR * kRowBytes + key * 4);
             vs[u][r] = lds_f32(at + 2 * kR * kRowBytes + kR * 4 + key * 4);
-            lift = __log2f(fmaxf(fabsf(vs[u][r]), 7.9e-31f));  // 2^-100: no lower, or the sum of the weights leaves fp32
+            // (2^-100: no lower, or the sum of the weights leaves fp32.  A scale that is not finite makes the products with V NaN, whatever its
+            // weight: it has no part in the maximum, so that the sum of the weights stays what it is.)
+            const float size = fabsf(vs[u][r]);
+            lift = size < INFINITY ? __log2f(fmaxf(size, 7.9e-31f)) : 0.f;
           }
           const bool there = (live >> key) & 1;
 #pragma unroll

@@ -215,6 +215,39 @@ def test_attention_nan_and_infinite_rows_stay_in_their_heads():
         assert o[1, 2:].isnan().all() and lse[1, 2:].isnan().all() and not o[1, :2].isnan().any()
 
 
+@pytest.mark.parametrize("H,D,q_dtype", [(4, 64, BF16), (8, 128, F16), (20, 64, F16), (40, 128, BF16), (4, 32, BF16), (4, 64, F32)])
+@pytest.mark.parametrize("n", [1, 90, 9001])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_attention_over_8_bit_pages_with_an_infinite_value(H, D, q_dtype, n, bad):
+    """A value row with an infinity is written with an infinite scale: the heads that see it are NaN, cut into parts or not (0 times infinity), but
+    their log-sum-exp and their rows' weights, which do not depend on the values, are those of the definition."""
+    from kernels_b200.streaming_attention import paged_attention, paged_cache_write
+
+    lens = [n, 33]
+    c = make_cache(2, 2, D, 16, lens, F8)
+    g = cuda(c)
+    v = torch.randn(2, 2, 1, D)
+    v[0, 1, 0, 3] = bad
+    k = torch.randn(2, 2, 1, D)
+    paged_cache_write(k.cuda(), v.cuda(), g["k_pages"], g["v_pages"], g["page_table"], g["lens"], k_scale=g["k_scale"], v_scale=g["v_scale"])
+    scale = g["v_scale"].cpu()
+    assert int((~scale.isfinite()).sum()) == 1
+    c = {name: x.cpu() for name, x in g.items()}
+    q = torch.randn(2, H, D, generator=torch.Generator().manual_seed(7)).to(q_dtype)
+    L = c["page_table"].shape[1] * 16
+    ref_o, ref_lse, ref_w, (dots, _) = PO.attend(q, c["k_pages"], c["v_pages"], c["page_table"], c["lens"], k_scale=c["k_scale"], v_scale=c["v_scale"])
+    assert ref_o[0, H // 2:].isnan().all() and not ref_o[0, : H // 2].isnan().any() and not ref_o[1].isnan().any()
+    w = torch.zeros(2, 2, L, device="cuda")
+    o, lse = paged_attention(q.cuda(), *(g[name] for name in ("k_pages", "v_pages", "page_table", "lens")), return_lse=True,
+                             k_scale=g["k_scale"], v_scale=g["v_scale"], weights=w)
+    assert torch.equal(o.cpu().isnan(), ref_o.isnan())
+    rel = 2 * dots * (D + 4) * 2**-22 + 2**-20 + n * 2**-23  # as above
+    assert bool(((lse.cpu().double() - ref_lse).abs() <= (rel + ref_lse.abs() * 2**-22) * 1.5).all())
+    add = ref_w.view(2, 2, H // 2, L)
+    off = (add * rel.view(2, 2, H // 2, 1)).sum(2) * 1.01 + (H // 2 + 1) * 2**-23 * add.sum(2) + H // 2 * 2**-126
+    assert bool(((w.cpu().double() - add.sum(2)).abs() <= off).all())
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, F8])
 def test_attention_takes_any_layout(dtype):
     """A [P, page, H_kv, D] pool, pages apart, rows off the 16-byte boundaries; tables and lengths as views; q in another order."""
