@@ -686,10 +686,11 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
           if constexpr (kF8) {
             ks = lds_f32(at + 2 * kR * kRowBytes + key * 4);
             vs[u][r] = lds_f32(at + 2 * kR * kRowBytes + kR * 4 + key * 4);
-            // (2^-100: no lower, or the sum of the weights leaves fp32.  A scale that is not finite makes the products with V NaN, whatever its
-            // weight: it has no part in the maximum, so that the sum of the weights stays what it is.)
+            // (2^-80: no lower, or the sum of the weights leaves fp32.  A weight is 2^(offset + slack + 80) = 2^95 at most, and there are 2^30
+            // rows at most.  A scale that is not finite makes the products with V NaN, whatever its weight: it has no part in the maximum, so that
+            // the sum of the weights stays what it is.)
             const float size = fabsf(vs[u][r]);
-            lift = size < INFINITY ? __log2f(fmaxf(size, 7.9e-31f)) : 0.f;
+            lift = size < INFINITY ? __log2f(fmaxf(size, 8.3e-25f)) : 0.f;
           }
           const bool there = (live >> key) & 1;
 #pragma unroll

@@ -248,6 +248,92 @@ def test_attention_over_8_bit_pages_with_an_infinite_value(H, D, q_dtype, n, bad
     assert bool(((w.cpu().double() - add.sum(2)).abs() <= off).all())
 
 
+def test_attention_over_very_many_rows_of_scale_zero():
+    """Value scales of 0 leave the rows' weights as they are: their sum stays within fp32 however many there are.  (One sequence's pages read by 64
+    sequences, so that a stretch of the line is about fourteen thousand rows; the first rows' scores lie 7.9 below the others', just too little to raise the maximum.)"""
+    from kernels_b200.streaming_attention import paged_attention
+
+    B, H_kv, D, page, n = 64, 8, 64, 64, 32768
+    c = make_cache(1, H_kv, D, page, [n], F8)
+    c["k_pages"] = torch.zeros(c["k_pages"].shape).to(F8)
+    c["k_scale"].fill_(1.0)
+    c["v_scale"].zero_()
+    rows = torch.zeros(n)
+    rows[32:] = 1.0
+    k = c["k_pages"].float()
+    for m in range(n // page):
+        k[c["page_table"][0, m], :, :, 0] = rows[m * page: (m + 1) * page]
+    c["k_pages"] = k.to(F8)
+    g = cuda(c)
+    q = torch.zeros(B, H_kv, D, dtype=F16, device="cuda")
+    q[..., 0] = 1.0
+    step = 7.875  # base-2 steps between the two scores
+    o, lse = paged_attention(q, g["k_pages"], g["v_pages"], g["page_table"].expand(B, -1), g["lens"].expand(B), sm_scale=step / 1.4426950408889634, return_lse=True,
+                             k_scale=g["k_scale"], v_scale=g["v_scale"])
+    want = torch.log2(torch.tensor((n - 32) * 2.0**step + 32, dtype=torch.float64))
+    assert (o == 0).all()
+    # a weight is off by 2^-20 of itself (its argument, up to 2^7, is rounded to 2^-18 and less where it counts), a sum of n terms by n 2^-24
+    assert ((lse.cpu().double() - want).abs() <= (2**-17 + n * 2**-24) * 1.5).all()
+
+
+@pytest.mark.parametrize("D,H,q_dtype", [(64, 4, BF16), (128, 8, F16), (128, 40, BF16), (32, 4, BF16)])
+@pytest.mark.parametrize("low,high", [(-40, 40), (-75, 10), (0, 85), (-100, -90), (60, 62)])
+def test_attention_over_8_bit_pages_of_any_scales(D, H, q_dtype, low, high):
+    """Value scales spread over many powers of two within a sequence, some of them 0 or negative.
+
+    Weights are multiplied as f16 numbers p v_scale whose largest is 2^7 at least: what lies below f16's least step, 2^-24, is off by half of it,
+    2^-32 of the largest p |v_scale|, times an element of 448 at most.  Where all scales are below 2^-80 the largest is that much smaller, and so
+    are the outputs: 2^-80 in its place.  A weight's argument is at most 2^8 in magnitude: rounded by 2^-17, so the weight by 2^-17 of itself."""
+    from kernels_b200.streaming_attention import paged_attention
+
+    gen = torch.Generator().manual_seed(D + H)
+    lens = [700, 41, 1]
+    c = make_cache(3, 2, D, 16, lens, F8)
+    spread = torch.rand(c["v_scale"].shape, generator=gen) * (high - low) + low
+    c["v_scale"] = torch.exp2(spread) * torch.where(torch.rand(spread.shape, generator=gen) < 0.2, -1.0, 1.0)
+    c["v_scale"][torch.rand(spread.shape, generator=gen) < 0.05] = 0.0
+    q = torch.randn(3, H, D, generator=gen).to(q_dtype)
+    ref_o, ref_lse, ref_w, (dots, mass) = PO.attend(q, c["k_pages"], c["v_pages"], c["page_table"], c["lens"], k_scale=c["k_scale"], v_scale=c["v_scale"])
+    g = cuda(c)
+    L = c["page_table"].shape[1] * 16
+    w = torch.zeros(3, 2, L, device="cuda")
+    o, lse = paged_attention(q.cuda(), *(g[n] for n in ("k_pages", "v_pages", "page_table", "lens")), return_lse=True, k_scale=g["k_scale"],
+                             v_scale=g["v_scale"], weights=w)
+    o, lse = o.cpu().double(), lse.cpu().double()
+    group = H // 2
+    row_scale = torch.zeros(3, 2, L, dtype=torch.float64)
+    for b, n in enumerate(lens):
+        for r in range(n):
+            row_scale[b, :, r] = c["v_scale"][c["page_table"][b, r // 16], :, r % 16].double()
+    top = (ref_w.view(3, 2, group, L) * row_scale[:, :, None].abs().clamp_min(2.0**-80)).amax(-1).view(3, H)
+    rel = 2 * dots * (D + 4) * 2**-22 + 2**-16 + max(lens) * 2**-23
+    step = torch.finfo(q_dtype).eps / 2
+    least = torch.finfo(q_dtype).tiny * torch.finfo(q_dtype).eps
+    weight_step = 2.0**-11  # f16 weights
+    tol = mass * (rel[..., None] + weight_step) * 1.01 + ref_o.abs() * step * 1.01 + least + (top * max(lens) * 2.0**-32 * 448)[..., None]
+    fits = ref_o.abs() + tol < torch.finfo(q_dtype).max  # (what leaves fp16 is infinite)
+    assert bool(((o - ref_o).abs() <= tol)[fits].all()) and not o.isnan().any()
+    assert bool(((lse - ref_lse).abs() <= (rel + (ref_lse.abs() + 100) * 2**-22) * 1.5).all())
+    add = ref_w.view(3, 2, group, L)
+    off = (add * rel.view(3, 2, group, 1)).sum(2) * 1.5 + (group + 1) * 2**-23 * add.sum(2) + group * 2**-126
+    assert bool(((w.cpu().double() - add.sum(2)).abs() <= off).all())
+
+
+@pytest.mark.parametrize("q_dtype", [F16, BF16, F32])
+def test_attention_extreme_scores_over_8_bit_pages(q_dtype):
+    """Rows one after the other that raise the maximum by a little or a lot, and the other way round."""
+    c = make_cache(2, 1, 64, 16, [300, 300], F8)
+    k, ramp = c["k_pages"].float(), torch.linspace(-3, 3, 300)
+    for r in range(300):
+        for b, x in enumerate((ramp[r], ramp[299 - r])):
+            k[c["page_table"][b, r // 16], 0, r % 16] = float(x)
+    c["k_pages"] = k.to(F8)
+    c["k_scale"].fill_(1.0)
+    q = torch.full((2, 2, 64), 4.0, dtype=q_dtype)
+    for scale in (None, -1.0, 0.0, 0.02):
+        check_attend(c, q, sm_scale=scale, weights=torch.zeros(2, 1, c["page_table"].shape[1] * 16))
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, F8])
 def test_attention_takes_any_layout(dtype):
     """A [P, page, H_kv, D] pool, pages apart, rows off the 16-byte boundaries; tables and lengths as views; q in another order."""
