@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
           most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
           most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
           const int x = (int)(most >> 7) - 127;  // the largest lies in [2^x, 2^(x + 1))
-          const int by = most == 0 || x == 128 ? 0 : max(-100, min(100, 14 - x));
+          const int by = most == 0 || x == 128 ? 0 : min(126, 14 - x);  // (-113 to 126: a normal number either way up)
           const float up = __uint_as_float((uint32_t)(by + 127) << 23);
           down *= __uint_as_float((uint32_t)(127 - by) << 23);
 #pragma unroll

@@ -319,6 +319,15 @@ def test_attention_over_8_bit_pages_of_any_scales(D, H, q_dtype, low, high):
     assert bool(((w.cpu().double() - add.sum(2)).abs() <= off).all())
 
 
+@pytest.mark.parametrize("size", [1e-36, 1e-30, 1e-20, 1e20, 1e30, 1e36])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_over_8_bit_pages_of_far_queries(size, D):
+    """bf16 queries far from 1, with a scale that brings their scores back."""
+    c = make_cache(2, 2, D, 16, [300, 45], F8)
+    q = (torch.randn(2, 4, D, generator=torch.Generator().manual_seed(3)) * size).to(BF16)
+    check_attend(c, q, sm_scale=0.125 / size, weights=torch.zeros(2, 2, c["page_table"].shape[1] * 16))
+
+
 @pytest.mark.parametrize("q_dtype", [F16, BF16, F32])
 def test_attention_extreme_scores_over_8_bit_pages(q_dtype):
     """Rows one after the other that raise the maximum by a little or a lot, and the other way round."""
