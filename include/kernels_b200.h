@@ -478,7 +478,8 @@ KB_API int kb_paged_attention(const kb_paged_attention_params* p, void* stream);
 
 /*
  * Eviction down to `budget` rows per sequence and head.  Rows rank by (row_positions above the sequence's and head's largest
- * minus `recent`, first), then by weight (a NaN is below every number), then the lower row first; the first `budget` stay.
+ * minus `recent`, first, of these the largest position), then by weight (a NaN is below every number), then the lower row first; the first
+ * `budget` stay.
  * Kept rows below the budget do not move; the i-th kept row behind it, in the order of rows, goes to the i-th row below it that came
  * free.  Rows behind the budget are left as they were.  Lengths become min(lens, budget).
  * weights_out, row_positions_out, lens_out: the inputs themselves (in place, all three), or buffers that do not overlap them, whose

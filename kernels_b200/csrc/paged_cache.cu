@@ -5,7 +5,8 @@
 // once.  A row of one head is eight or sixteen elements per thread, a few neighbouring threads: its largest magnitude, which sets
 // the scale of an 8-bit row, is a few shuffles away.  The threads look up a token's place once and walk over its heads.
 //
-// EVICT.  Rows rank by (position among the newest `recent`, then weight, then the lower row); the first `budget` stay.
+// EVICT.  Rows rank by (position among the newest `recent`, then weight, then the lower row); the first `budget` stay.  Where the newest alone are
+// more than the budget they rank by position, so that a token just written is never the one that goes.
 // The kept rows below the budget stay where they are, and the i-th kept row behind it moves to the i-th place that came
 // free before it.  Attention does not depend on the rows' order, so nothing else has to move: a cache that is one row
 // over its budget moves one row, not half of them.  Sources lie behind the budget and destinations before it, so all
@@ -233,13 +234,17 @@ struct EvictArgs {
   bool in_place;
 };
 
-// Weights as whole numbers of the same order; a NaN is below them all, the newest rows are above.
+// Weights as whole numbers of the same order; a NaN is below them all, the newest rows are above.  (Where those alone are more than the budget, a second
+// search ranks them by their positions; see `by_position`.)
 __device__ __forceinline__ uint32_t rank_key(float w, bool newest) {
   if (newest) return 0xffffffffu;
   const uint32_t u = __float_as_uint(w + 0.f);  // (one zero)
   if (w != w) return 0u;
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+
+// The newest rows by their positions, the others behind them (0: does not count).
+__device__ __forceinline__ uint32_t position_key(int32_t position, int64_t from) { return position > from ? (uint32_t)(position - from) : 0u; }
 
 // What the warps of a cluster's blocks have in common.  Each value goes through shared memory once; buffers alternate, so that one
 // barrier per value is enough.
@@ -330,6 +335,7 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
   if (a.cluster > 1) sm100::cluster_sync_all();  // (a block's shared memory may be written once the block has started)
 
   uint32_t key[kKeys];
+  int64_t from;  // positions above it are among the newest
   {
     float x[kKeys];
     int32_t y[kKeys];
@@ -351,47 +357,55 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
       return;
     }
     newest = team.max(__reduce_max_sync(0xffffffffu, newest));
-    const int64_t from = (int64_t)newest - a.recent;  // positions above it are among the newest
+    from = (int64_t)newest - a.recent;
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) key[j] = row0 + j * 32 < n ? rank_key(x[j], y[j] > from) : 0u;  // (0: does not count below)
   }
-  uint32_t least = 0, bit = 0x80000000u;
-  int reached = n, over = 0;  // keys that reach `least`, and those above what the bits to come can make of it
-  for (; bit && reached != a.budget && reached - over > (int)blockDim.x; bit >>= 1) {
-    int reach = 0;
+  uint32_t least;
+  int reached, over;  // keys that reach `least`, and those above what the bits to come can make of it
+  for (bool by_position = false;; by_position = true) {
+    uint32_t bit = 0x80000000u;
+    least = 0, reached = n, over = 0;
+    for (; bit && reached != a.budget && reached - over > (int)blockDim.x; bit >>= 1) {
+      int reach = 0;
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) reach += key[j] >= (least | bit);
-    reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
-    if (reach >= a.budget) least |= bit, reached = reach;
-    else over = reach;
-  }
-  if (bit && reached != a.budget) {
-    // every block of the team gets all of them and goes on by itself
-    const uint32_t most = least + (bit - 1) + bit;  // (no more than 2^32 - 1)
-    const int many = reached - over, others = over;
-    uint32_t picked = 0;
-#pragma unroll
-    for (int j = 0; j < kKeys; ++j) picked |= (uint32_t)(key[j] >= least && key[j] <= most && row0 + j * 32 < n) << j;
-    int at = __popc(picked), before;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, at, x);
-      if (lane >= x) at += y;
-    }
-    team.sum(__shfl_sync(0xffffffffu, at, 31), &before);
-    at += before - __popc(picked);
-#pragma unroll
-    for (int j = 0; j < kKeys; ++j)
-      if ((picked >> j) & 1) team.tell(&few[at++], key[j]);
-    if (team.size > 1) sm100::cluster_sync_all();
-    else __syncthreads();
-    const bool here = threadIdx.x < many;
-    const uint32_t mine = here ? few[threadIdx.x] : 0u;
-    for (; bit && reached != a.budget; bit >>= 1) {
-      const int reach = others + __syncthreads_count(here && mine >= (least | bit));
+      for (int j = 0; j < kKeys; ++j) reach += key[j] >= (least | bit);
+      reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
       if (reach >= a.budget) least |= bit, reached = reach;
       else over = reach;
     }
+    if (bit && reached != a.budget) {
+      // every block of the team gets all of them and goes on by itself
+      const uint32_t most = least + (bit - 1) + bit;  // (no more than 2^32 - 1)
+      const int many = reached - over, others = over;
+      uint32_t picked = 0;
+#pragma unroll
+      for (int j = 0; j < kKeys; ++j) picked |= (uint32_t)(key[j] >= least && key[j] <= most && row0 + j * 32 < n) << j;
+      int at = __popc(picked), before;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, at, x);
+        if (lane >= x) at += y;
+      }
+      team.sum(__shfl_sync(0xffffffffu, at, 31), &before);
+      at += before - __popc(picked);
+#pragma unroll
+      for (int j = 0; j < kKeys; ++j)
+        if ((picked >> j) & 1) team.tell(&few[at++], key[j]);
+      if (team.size > 1) sm100::cluster_sync_all();
+      else __syncthreads();
+      const bool here = threadIdx.x < many;
+      const uint32_t mine = here ? few[threadIdx.x] : 0u;
+      for (; bit && reached != a.budget; bit >>= 1) {
+        const int reach = others + __syncthreads_count(here && mine >= (least | bit));
+        if (reach >= a.budget) least |= bit, reached = reach;
+        else over = reach;
+      }
+    }
+    if (by_position || least != 0xffffffffu || reached == a.budget) break;
+    // the newest rows are too many: the newest of them stay
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) key[j] = row0 + j * 32 < n ? position_key(s.pos[row0 + j * 32], from) : 0u;
   }
   let_next_launch_start();
   // which rows stay; of those that equal the threshold, where there are too many, the lowest
@@ -455,21 +469,26 @@ __global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs
   }
   newest = team.max(__reduce_max_sync(0xffffffffu, newest));
   const int64_t from = (int64_t)newest - a.recent;
+  bool by_position = false;
   // f(key, row, whether there is such a row) for the warp's rows, all lanes together
   auto each = [&](auto f) {
     for (int i0 = begin; i0 < end; i0 += 32) {
       const int i = i0 + lane;
-      f(i < end ? rank_key(s.w[i], s.pos[i] > from) : 0u, i, i < end);
+      f(i >= end ? 0u : by_position ? position_key(s.pos[i], from) : rank_key(s.w[i], s.pos[i] > from), i, i < end);
     }
   };
-  uint32_t least = 0;
-  int reached = s.n, over = 0;
-  for (uint32_t bit = 0x80000000u; bit && reached != a.budget; bit >>= 1) {
-    int reach = 0;
-    each([&](uint32_t k, int, bool) { reach += k >= (least | bit); });
-    reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
-    if (reach >= a.budget) least |= bit, reached = reach;
-    else over = reach;
+  uint32_t least;
+  int reached, over;
+  for (;; by_position = true) {
+    least = 0, reached = s.n, over = 0;
+    for (uint32_t bit = 0x80000000u; bit && reached != a.budget; bit >>= 1) {
+      int reach = 0;
+      each([&](uint32_t k, int, bool) { reach += k >= (least | bit); });
+      reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
+      if (reach >= a.budget) least |= bit, reached = reach;
+      else over = reach;
+    }
+    if (by_position || least != 0xffffffffu || reached == a.budget) break;
   }
   int ties = INT32_MAX, equal_before = 0;
   if (reached != a.budget) {

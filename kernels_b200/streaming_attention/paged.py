@@ -197,8 +197,8 @@ def paged_cache_evict(
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Cut every sequence down to ``budget`` rows per head; returns ``(lens, weights, row_positions)``, updated in place.
 
-    The rows whose position is among the newest ``recent`` stay (``row_positions`` above the head's largest minus ``recent``), then those
-    that have received most attention; of equals the lower row.  Every head keeps rows of its own.  Kept rows below the budget do not move; the kept
+    The rows whose position is among the newest ``recent`` stay (``row_positions`` above the head's largest minus ``recent``; where these are more
+    than ``budget``, the newest of them), then those that have received most attention; of equals the lower row.  Every head keeps rows of its own.  Kept rows below the budget do not move; the kept
     rows behind it fill, in order, the places that came free, so that afterwards rows ``0 .. budget - 1`` are the sequence and its later pages are
     free.  Rows are then no longer in the order of their tokens, which attention without a window does not depend on
     (rotary embedding has been applied before the write).

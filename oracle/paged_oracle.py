@@ -106,7 +106,7 @@ def evict(k_pages, v_pages, table, lens, weights, row_positions, budget, recent,
 
             def rank(r):
                 first = pos[r] > newest - recent
-                return (not first, 0 if first else w[r] != w[r], 0 if first or w[r] != w[r] else -w[r], r)
+                return (not first, -pos[r] if first else w[r] != w[r], 0 if first or w[r] != w[r] else -w[r], r)
 
             kept = sorted(range(n), key=rank)[:budget]
             src, dst = sorted(r for r in kept if r >= budget), sorted(set(range(budget)) - set(kept))

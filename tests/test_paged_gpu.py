@@ -589,6 +589,51 @@ def test_evict_matches_definition(H_kv, D, page, lens, dtype, budget, recent, ti
     check_evict(c, w, pos, budget, recent)
     check_evict(c, w, pos, budget, recent, in_place=False)
 
+@pytest.mark.parametrize("H_kv,page,lens,budget,recent", [
+    (2, 16, [65], 64, 100),                    # one row over, every one of them recent
+    (2, 16, [400, 70, 64], 64, 65),
+    (1, 64, [40000, 20000], 5000, 2**31 - 1),  # a cluster
+    (1, 64, [140000], 70000, 100000),          # longer than a cluster holds
+    (2, 16, [3000], 1000, 2000),               # more recent rows than the budget, and others besides
+])
+@pytest.mark.parametrize("shuffled", [False, True])
+def test_evict_keeps_the_newest_of_more_recent_rows_than_the_budget(H_kv, page, lens, budget, recent, shuffled):
+    """Weights say nothing where the recent rows alone pass the budget: the newest of them stay, so that a token just written is never the one that goes."""
+    c = make_cache(len(lens), H_kv, 16, page, lens, F16)
+    L = c["page_table"].shape[1] * page
+    w, pos = make_books(len(lens), H_kv, L)
+    if not shuffled:
+        pos = torch.arange(L, dtype=torch.int32).expand(len(lens), H_kv, L).contiguous()
+    g = check_evict(c, w, pos, budget, recent)
+    check_evict(c, w, pos, budget, recent, in_place=False)
+    for b, n in enumerate(lens):
+        for h in range(H_kv):
+            kept, rows = set(g["row_positions"][b, h, : min(n, budget)].tolist()), pos[b, h, :n]
+            newest = rows[rows > int(rows.max()) - recent].sort(descending=True).values[:budget]
+            assert set(newest.tolist()) <= kept and (n <= budget or len(newest) < budget or set(newest.tolist()) == kept)
+
+
+def test_a_cache_whose_budget_is_smaller_than_its_window_goes_on():
+    """Token after token, the cache holds the newest ``budget`` of them."""
+    from kernels_b200.streaming_attention import paged_cache_evict, paged_cache_write
+
+    c = make_cache(1, 2, 64, 16, [96], F16)
+    g = cuda(c)
+    g["lens"].zero_()
+    w, pos = torch.zeros(1, 2, 96, device="cuda"), torch.zeros(1, 2, 96, dtype=torch.int32, device="cuda")
+    pages = tuple(g[n] for n in ("k_pages", "v_pages", "page_table", "lens"))
+    for t in range(150):
+        g["lens"] += 1
+        x = torch.full((1, 2, 1, 64), float(t), dtype=F16, device="cuda")
+        paged_cache_write(x, x, *pages, positions=torch.tensor([[t]], dtype=torch.int32, device="cuda"), weights=w, row_positions=pos)
+        w[:, :, 0] = 100.0  # (the oldest place is the heaviest)
+        paged_cache_evict(*pages, w, pos, 64, 100)
+    assert g["lens"].tolist() == [64]
+    for h in range(2):
+        assert sorted(pos[0, h, :64].tolist()) == list(range(86, 150))
+        rows = [g["k_pages"][g["page_table"][0, r // 16], h, r % 16, 0].item() for r in range(64)]
+        assert rows == pos[0, h, :64].tolist()
+
 
 def test_evict_special_weights_and_positions():
     c = make_cache(3, 2, 64, 16, [100, 100, 100], F16)
