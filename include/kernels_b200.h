@@ -481,7 +481,8 @@ KB_API int kb_paged_attention(const kb_paged_attention_params* p, void* stream);
  * minus `recent`, first, of these the largest position), then by weight (a NaN is below every number), then the lower row first; the first
  * `budget` stay.
  * Kept rows below the budget do not move; the i-th kept row behind it, in the order of rows, goes to the i-th row below it that came
- * free.  Rows behind the budget are left as they were.  Lengths become min(lens, budget).
+ * free.  Rows behind the budget are left as they were.  Lengths become min(lens, budget).  Rows without a page are passed over: they are not
+ * kept in place of others, and nothing moves into one (as many rows stay as there are places with a page below the budget).
  * weights_out, row_positions_out, lens_out: the inputs themselves (in place, all three), or buffers that do not overlap them, whose
  * entries below the new length are written.  No page may stand in the table of two sequences that lose rows, or twice
  * in one.  `workspace`: kb_paged_evict_workspace_bytes bytes (host-only), 4-byte aligned.

@@ -31,6 +31,7 @@ struct PagedView {
     const int32_t id = table[b * table_b + m * table_m];
     return (uint32_t)id < (uint32_t)P ? id : -1;
   }
+  __device__ __forceinline__ bool has_page(int32_t b, int32_t m) const { return (uint32_t)table[b * table_b + m * table_m] < (uint32_t)P; }
 };
 
 inline PagedView make_paged_view(const kb_paged_cache& c) {

@@ -6,7 +6,8 @@
 // the scale of an 8-bit row, is a few shuffles away.  The threads look up a token's place once and walk over its heads.
 //
 // EVICT.  Rows rank by (position among the newest `recent`, then weight, then the lower row); the first `budget` stay.  Where the newest alone are
-// more than the budget they rank by position, so that a token just written is never the one that goes.
+// more than the budget they rank by position, so that a token just written is never the one that goes.  Rows without a page (an entry of the
+// table outside the pages) hold nothing: they are passed over, and so are places without one.
 // The kept rows below the budget stay where they are, and the i-th kept row behind it moves to the i-th place that came
 // free before it.  Attention does not depend on the rows' order, so nothing else has to move: a cache that is one row
 // over its budget moves one row, not half of them.  Sources lie behind the budget and destinations before it, so all
@@ -308,9 +309,9 @@ struct SelectHead {
   int32_t* po;
   int32_t* count;
   int64_t list;  // where its moves go
-  int32_t n;
+  int32_t b, n;
 
-  __device__ __forceinline__ SelectHead(const EvictArgs& a, int32_t b, int32_t h) {
+  __device__ __forceinline__ SelectHead(const EvictArgs& a, int32_t b, int32_t h) : b(b) {
     n = a.c.rows(b);
     w = a.weights + b * a.w_b + h * a.w_h;
     pos = a.positions + b * a.p_b + h * a.p_h;
@@ -319,6 +320,14 @@ struct SelectHead {
     count = a.counts + (int64_t)b * a.H_kv + h;
     list = ((int64_t)b * a.H_kv + h) * a.most_moves;
   }
+  // Whether some of the sequence's rows have no page (every thread of the block calls).
+  __device__ __forceinline__ bool lacks_pages(const EvictArgs& a) const {
+    const int32_t pages = kb_fastdiv(n - 1, a.c.fd_page) + 1;
+    bool lacks = false;
+    for (int32_t m = threadIdx.x; m < pages; m += blockDim.x) lacks |= !a.c.has_page(b, m);
+    return __syncthreads_or(lacks);
+  }
+  __device__ __forceinline__ bool has_page(const EvictArgs& a, int32_t row) const { return a.c.has_page(b, kb_fastdiv(row, a.c.fd_page)); }
 };
 
 // Keys in registers.  Warp w of the team has the rows [w kWarpRows, (w + 1) kWarpRows), 32 at a time so that ranks within it are ballots.
@@ -334,8 +343,9 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
   const int32_t n = s.n, row0 = (team.rank * warps + warp) * kWarpRows + lane;
   if (a.cluster > 1) sm100::cluster_sync_all();  // (a block's shared memory may be written once the block has started)
 
-  uint32_t key[kKeys];
-  int64_t from;  // positions above it are among the newest
+  uint32_t key[kKeys], live = 0;  // live: the rows that count
+  int64_t from;                   // positions above it are among the newest
+  int32_t rows = n, budget = a.budget;
   {
     float x[kKeys];
     int32_t y[kKeys];
@@ -344,6 +354,7 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
       const int i = row0 + j * 32;
       x[j] = i < n ? s.w[i] : 0.f;
       y[j] = i < n ? s.pos[i] : INT32_MIN;
+      live |= (uint32_t)(i < n) << j;
     }
     int32_t newest = INT32_MIN;
 #pragma unroll
@@ -358,29 +369,45 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
     }
     newest = team.max(__reduce_max_sync(0xffffffffu, newest));
     from = (int64_t)newest - a.recent;
+    if (s.lacks_pages(a)) {
+      // those rows hold nothing and can hold nothing: as many of the others stay as there are places with a page
+      int places = 0;
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) key[j] = row0 + j * 32 < n ? rank_key(x[j], y[j] > from) : 0u;  // (0: does not count below)
+      for (int j = 0; j < kKeys; ++j) {
+        const int i = row0 + j * 32;
+        if (i < n && !s.has_page(a, i)) live &= ~(1u << j);
+        places += ((live >> j) & 1) && i < a.budget;
+      }
+      budget = team.sum(__reduce_add_sync(0xffffffffu, places));
+      rows = team.sum(__reduce_add_sync(0xffffffffu, __popc(live)));
+      if (budget == 0 || budget == rows) {
+        if (threadIdx.x == 0 && team.rank == 0) *s.count = 0;
+        return;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) key[j] = (live >> j) & 1 ? rank_key(x[j], y[j] > from) : 0u;  // (0: does not count below)
   }
   uint32_t least;
   int reached, over;  // keys that reach `least`, and those above what the bits to come can make of it
   for (bool by_position = false;; by_position = true) {
     uint32_t bit = 0x80000000u;
-    least = 0, reached = n, over = 0;
-    for (; bit && reached != a.budget && reached - over > (int)blockDim.x; bit >>= 1) {
+    least = 0, reached = rows, over = 0;
+    for (; bit && reached != budget && reached - over > (int)blockDim.x; bit >>= 1) {
       int reach = 0;
 #pragma unroll
       for (int j = 0; j < kKeys; ++j) reach += key[j] >= (least | bit);
       reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
-      if (reach >= a.budget) least |= bit, reached = reach;
+      if (reach >= budget) least |= bit, reached = reach;
       else over = reach;
     }
-    if (bit && reached != a.budget) {
+    if (bit && reached != budget) {
       // every block of the team gets all of them and goes on by itself
       const uint32_t most = least + (bit - 1) + bit;  // (no more than 2^32 - 1)
       const int many = reached - over, others = over;
       uint32_t picked = 0;
 #pragma unroll
-      for (int j = 0; j < kKeys; ++j) picked |= (uint32_t)(key[j] >= least && key[j] <= most && row0 + j * 32 < n) << j;
+      for (int j = 0; j < kKeys; ++j) picked |= (uint32_t)(key[j] >= least && key[j] <= most && (live >> j & 1)) << j;
       int at = __popc(picked), before;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
@@ -396,31 +423,32 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
       else __syncthreads();
       const bool here = threadIdx.x < many;
       const uint32_t mine = here ? few[threadIdx.x] : 0u;
-      for (; bit && reached != a.budget; bit >>= 1) {
+      for (; bit && reached != budget; bit >>= 1) {
         const int reach = others + __syncthreads_count(here && mine >= (least | bit));
-        if (reach >= a.budget) least |= bit, reached = reach;
+        if (reach >= budget) least |= bit, reached = reach;
         else over = reach;
       }
     }
-    if (by_position || least != 0xffffffffu || reached == a.budget) break;
+    if (by_position || least != 0xffffffffu || reached == budget) break;
     // the newest rows are too many: the newest of them stay
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) key[j] = row0 + j * 32 < n ? position_key(s.pos[row0 + j * 32], from) : 0u;
+    for (int j = 0; j < kKeys; ++j) key[j] = (live >> j) & 1 ? position_key(s.pos[row0 + j * 32], from) : 0u;
   }
   let_next_launch_start();
   // which rows stay; of those that equal the threshold, where there are too many, the lowest
   uint32_t keep = 0;
 #pragma unroll
-  for (int j = 0; j < kKeys; ++j) keep |= (uint32_t)(key[j] >= least && row0 + j * 32 < n) << j;
-  if (reached != a.budget) {
+  for (int j = 0; j < kKeys; ++j) keep |= (uint32_t)(key[j] >= least) << j;
+  keep &= live;
+  if (reached != budget) {
     int equal = 0, before;
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) equal += key[j] == least && row0 + j * 32 < n;
+    for (int j = 0; j < kKeys; ++j) equal += key[j] == least && (live >> j & 1);
     team.sum(__reduce_add_sync(0xffffffffu, equal), &before);
-    const int ties = a.budget - over;
+    const int ties = budget - over;
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
-      const bool tie = key[j] == least && row0 + j * 32 < n;
+      const bool tie = key[j] == least && (live >> j & 1);
       const uint32_t eq = __ballot_sync(0xffffffffu, tie);
       if (tie && before + __popc(eq & ((1u << lane) - 1)) >= ties) keep &= ~(1u << j);
       before += __popc(eq);
@@ -431,9 +459,10 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
   for (int j = 0; j < kKeys; ++j) {
     const int i = row0 + j * 32;
     const bool stays = (keep >> j) & 1;
-    hole |= (uint32_t)(i < a.budget && i < n && !stays) << j;
+    hole |= (uint32_t)(i < a.budget && !stays) << j;
     mover |= (uint32_t)(i >= a.budget && stays) << j;
   }
+  hole &= live;
   int hole_at, mover_at;
   team.sum(__reduce_add_sync(0xffffffffu, __popc(hole)), &hole_at);
   const int moves = team.sum(__reduce_add_sync(0xffffffffu, __popc(mover)), &mover_at);
@@ -469,33 +498,46 @@ __global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs
   }
   newest = team.max(__reduce_max_sync(0xffffffffu, newest));
   const int64_t from = (int64_t)newest - a.recent;
+  const bool lacks = s.lacks_pages(a);
   bool by_position = false;
   // f(key, row, whether there is such a row) for the warp's rows, all lanes together
   auto each = [&](auto f) {
     for (int i0 = begin; i0 < end; i0 += 32) {
       const int i = i0 + lane;
-      f(i >= end ? 0u : by_position ? position_key(s.pos[i], from) : rank_key(s.w[i], s.pos[i] > from), i, i < end);
+      const bool in = i < end && (!lacks || s.has_page(a, i));
+      f(!in ? 0u : by_position ? position_key(s.pos[i], from) : rank_key(s.w[i], s.pos[i] > from), i, in);
     }
   };
+  int32_t rows = s.n, budget = a.budget;
+  if (lacks) {  // as above
+    int places = 0, there = 0;
+    each([&](uint32_t, int i, bool in) { places += in && i < a.budget, there += in; });
+    budget = team.sum(__reduce_add_sync(0xffffffffu, places));
+    rows = team.sum(__reduce_add_sync(0xffffffffu, there));
+    if (budget == 0 || budget == rows) {
+      if (threadIdx.x == 0 && team.rank == 0) *s.count = 0;
+      return;
+    }
+  }
   uint32_t least;
   int reached, over;
   for (;; by_position = true) {
-    least = 0, reached = s.n, over = 0;
-    for (uint32_t bit = 0x80000000u; bit && reached != a.budget; bit >>= 1) {
+    least = 0, reached = rows, over = 0;
+    for (uint32_t bit = 0x80000000u; bit && reached != budget; bit >>= 1) {
       int reach = 0;
       each([&](uint32_t k, int, bool) { reach += k >= (least | bit); });
       reach = team.sum(__reduce_add_sync(0xffffffffu, reach));
-      if (reach >= a.budget) least |= bit, reached = reach;
+      if (reach >= budget) least |= bit, reached = reach;
       else over = reach;
     }
-    if (by_position || least != 0xffffffffu || reached == a.budget) break;
+    if (by_position || least != 0xffffffffu || reached == budget) break;
   }
   int ties = INT32_MAX, equal_before = 0;
-  if (reached != a.budget) {
+  if (reached != budget) {
     int equal = 0;
     each([&](uint32_t k, int, bool in) { equal += in && k == least; });
     team.sum(__reduce_add_sync(0xffffffffu, equal), &equal_before);
-    ties = a.budget - over;
+    ties = budget - over;
   }
   let_next_launch_start();
   int holes = 0, movers = 0, hole_at = 0, mover_at = 0;

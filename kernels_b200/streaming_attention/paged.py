@@ -201,7 +201,8 @@ def paged_cache_evict(
     than ``budget``, the newest of them), then those that have received most attention; of equals the lower row.  Every head keeps rows of its own.  Kept rows below the budget do not move; the kept
     rows behind it fill, in order, the places that came free, so that afterwards rows ``0 .. budget - 1`` are the sequence and its later pages are
     free.  Rows are then no longer in the order of their tokens, which attention without a window does not depend on
-    (rotary embedding has been applied before the write).
+    (rotary embedding has been applied before the write).  Rows without a page are passed over, and nothing moves into one: as many rows stay
+    as the first ``budget`` places have pages for.
 
     ``out``: a ``(lens, weights, row_positions)`` to be written instead, not overlapping the given ones (entries of
     the rows that remain; the pages change all the same).  Sequences that share pages need copies of their own first.

@@ -108,14 +108,15 @@ def evict(k_pages, v_pages, table, lens, weights, row_positions, budget, recent,
                 first = pos[r] > newest - recent
                 return (not first, -pos[r] if first else w[r] != w[r], 0 if first or w[r] != w[r] else -w[r], r)
 
-            kept = sorted(range(n), key=rank)[:budget]
-            src, dst = sorted(r for r in kept if r >= budget), sorted(set(range(budget)) - set(kept))
+            # rows without a page hold nothing and places without one take nothing
+            held = [r for r in range(n) if place(table[b], r, page, P) is not None]
+            places = [r for r in held if r < budget]
+            kept = sorted(held, key=rank)[:len(places)]
+            src, dst = sorted(r for r in kept if r >= budget), sorted(set(places) - set(kept))
             assert len(src) == len(dst)
             for s, d in zip(src, dst):
                 weights[b, h, d], row_positions[b, h, d] = weights[b, h, s], row_positions[b, h, s]
                 sp, dp = place(table[b], s, page, P), place(table[b], d, page, P)
-                if sp is None or dp is None:
-                    continue
                 for x in (k_pages, v_pages, k_scale, v_scale):
                     if x is not None:
                         x = x.view(torch.uint8) if x.dtype == torch.float8_e4m3fn else x

@@ -656,6 +656,35 @@ def test_evict_leaves_rows_without_a_page_alone():
     c["lens"] = torch.tensor([-1, 100, -2**31], dtype=torch.int32)
     check_evict(c, w, pos, 60, 5)
 
+@pytest.mark.parametrize("page,n,budget,recent,gone", [
+    (16, 100, 50, 5, [1, 5]), (16, 100, 50, 5, [6]), (16, 100, 50, 0, [0, 1, 2]), (16, 100, 50, 5, [0, 1, 2, 3]), (16, 100, 50, 200, [0, 4]), (1, 60, 30, 3, [0, 3, 7, 29, 30, 31, 59]),
+    (16, 100, 50, 5, [3, 4, 5, 6]), (64, 40000, 5000, 100, [0, 9, 78, 79, 300, 624]), (64, 140000, 70000, 0, [3, 1093, 1094, 2000]),
+])
+def test_evict_passes_over_rows_without_a_page(page, n, budget, recent, gone):
+    """A row without a page holds nothing: it is not kept in a place that others could fill, and no kept row moves into a place without one.  Every visible
+    row that is left has its own keys and values beside its own weight and position."""
+    c = make_cache(2, 2, 16, page, [n, n], F32)
+    c["page_table"][0, gone] = torch.tensor([-1, c["k_pages"].shape[0], 2**31 - 1, -2**31])[torch.arange(len(gone)) % 4].to(torch.int32)
+    L = c["page_table"].shape[1] * page
+    w, pos = make_books(2, 2, L)
+    for h in range(2):  # rows are told by their positions (below 2^24)
+        for b in range(2):
+            for name in ("k_pages", "v_pages"):
+                at = c["page_table"][b].long()
+                held = (at >= 0) & (at < c["k_pages"].shape[0])
+                c[name][at[held], h] = pos[b, h].view(-1, page)[held][..., None].expand(-1, -1, 16).float()
+    g = check_evict(c, w, pos, budget, recent)
+    check_evict(c, w, pos, budget, recent, in_place=False)
+    held = torch.tensor([PO.place(c["page_table"][0], r, page, c["k_pages"].shape[0]) is not None for r in range(n)])
+    for h in range(2):
+        seen = held[:budget].nonzero()[:, 0]
+        at = c["page_table"][0].long()[seen // page]
+        for name in ("k_pages", "v_pages"):
+            rows = g[name].cpu()[at, h, seen % page]
+            assert torch.equal(rows, g["row_positions"].cpu()[0, h, seen][:, None].expand(-1, 16).float())
+        left = set(g["row_positions"][0, h, seen.cuda()].tolist())
+        assert len(left) == len(seen) and left <= set(pos[0, h, :n][held].tolist())
+
 
 def test_evict_layouts():
     c = make_cache(2, 2, 64, 16, [200, 150], F16)
