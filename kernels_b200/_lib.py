@@ -347,6 +347,17 @@ def transforms_active() -> bool:
     return _can_tell_plain and _transforms_active()
 
 
+def looked_into(*tensors) -> bool:
+    """Whether something records or intercepts operators (compilation, jit tracing, dispatch modes, tensor subclasses): a launch that goes past the
+    dispatcher would be missing from what it records."""
+    if torch.compiler.is_compiling() or not _can_tell_plain or _tracing_state() is not None or _dispatch_modes():
+        return True
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return True
+    return False
+
+
 def launch_count() -> int:
     return int(load().kb_launch_count())
 

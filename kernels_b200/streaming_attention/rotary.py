@@ -5,14 +5,15 @@ for every sequence.  Tokens of a video or an image stand on several axes (time, 
 newest tokens of a batch of streams stand at positions of their own.  Here every token brings its position on each axis,
 and every axis turns its own band of the frequencies.
 
-One kernel (``kb_rotary``), differentiable in ``q`` and ``k``: the gradient is the same kernel turning the other way.  A
+One kernel (``kb_rotary``), differentiable in ``q`` and ``k``: the gradient is the same kernel turning the other way.  What traces,
+compiles or intercepts operators meets it as ``kernels_b200::rotary_embedding``.  A
 backward pass can be captured into a CUDA graph as any of torch's can, while no eager graph of the same leaves is alive.
 There is no CPU path.
 """
 
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -42,6 +43,53 @@ def _rotate(q, k, positions, inv_freq, ends, inverse):
     return q_out, k_out
 
 
+@torch.library.custom_op("kernels_b200::rotary_embedding", mutates_args=(), device_types=("cuda",))
+def _rotary_op(
+    q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, ends: Sequence[int], inverse: bool
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    q_out, k_out = _rotate(q, k, positions, inv_freq, ends, inverse)
+    return q_out, q.new_empty(0) if k_out is None else k_out
+
+
+@torch.library.register_fake("kernels_b200::rotary_embedding")
+def _rotary_op_abstract(q, k, positions, inv_freq, ends, inverse):
+    q_out, k_out = (None if x is None else torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
+    return q_out, q.new_empty(0) if k_out is None else k_out
+
+
+def _op(q, k, *rest):
+    """The operator, where something looks into the call: the others go past the dispatcher, which takes 30 microseconds."""
+    q_out, k_out = torch.ops.kernels_b200.rotary_embedding(q, k, *rest)
+    return q_out, None if k is None else k_out
+
+
+def _op_setup(ctx, inputs, output):
+    _, k, positions, inv_freq, ctx.ends, ctx.inverse = inputs
+    ctx.save_for_backward(positions, inv_freq)
+
+
+def _op_backward(ctx, dq, dk):
+    return _gradients(ctx, dq, dk, _op)
+
+
+def _gradients(ctx, dq, dk, go):
+    positions, inv_freq = ctx.saved_tensors
+    turn = lambda q, k: go(q, k, positions, inv_freq, ctx.ends, not ctx.inverse)  # noqa: E731
+    need_q, need_k = ctx.needs_input_grad[:2]
+    if need_q:
+        dq, dk = turn(dq, dk if need_k else None)
+    else:
+        dq, dk = None, turn(dk, None)[0]
+    return dq, dk, None, None, None, None
+
+
+torch.library.register_autograd("kernels_b200::rotary_embedding", _op_backward, setup_context=_op_setup)
+
+
+def _rotate_or_op(q, k, *rest):
+    return (_op if _lib.looked_into(q, k) else _rotate)(q, k, *rest)
+
+
 def _keep(ctx, inputs):
     _, _, positions, inv_freq, ctx.ends, ctx.inverse = inputs
     ctx.save_for_backward(positions, inv_freq)
@@ -53,24 +101,19 @@ def _turn(*inputs):
     return (_RotaryEmbeddingTransformed if _lib.transforms_active() else _RotaryEmbedding).apply(*inputs)
 
 
+_turn_uncompiled = torch.compiler.disable(_turn)
+
+
 class _RotaryEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *inputs):
         _keep(ctx, inputs)
-        return _rotate(*inputs)
+        return _rotate_or_op(*inputs)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        positions, inv_freq = ctx.saved_tensors
         # (turned by the same function where gradients are to have gradients)
-        go = _turn if torch.is_grad_enabled() else _rotate
-        turn = lambda q, k: go(q, k, positions, inv_freq, ctx.ends, not ctx.inverse)  # noqa: E731
-        need_q, need_k = ctx.needs_input_grad[:2]
-        if need_q:
-            dq, dk = turn(dq, dk if need_k else None)
-        else:
-            dq, dk = None, turn(dk, None)[0]
-        return dq, dk, None, None, None, None
+        return _gradients(ctx, dq, dk, _turn if torch.is_grad_enabled() else _rotate_or_op)
 
     @staticmethod
     def jvp(ctx, tq, tk, *_):
@@ -84,7 +127,7 @@ class _RotaryEmbeddingTransformed(_RotaryEmbedding):
 
     @staticmethod
     def forward(q, k, positions, inv_freq, ends, inverse):
-        return _rotate(q, k, positions, inv_freq, ends, inverse)
+        return _rotate_or_op(q, k, positions, inv_freq, ends, inverse)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -129,6 +172,12 @@ def rotary_embedding(
     assert 1 <= len(ends) <= 8 and len(ends) == pos_shape[0], "one section of frequencies per axis, at most 8"
     assert end == R and min(sections) >= 0, "the sections share out inv_freq"
     inv_freq = inv_freq.contiguous()
-    if _lib.forward_ad_active() or (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))):
+    looked_into = _lib.looked_into(q, k)
+    if _lib.forward_ad_active() or (looked_into and _lib.transforms_active()):
+        # (the function's gradients: the operator has none of these; a compiled caller steps out for them)
+        return (_turn_uncompiled if torch.compiler.is_compiling() else _turn)(q, k, positions, inv_freq, ends, False)
+    if looked_into:
+        return _op(q, k, positions, inv_freq, ends, False)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _turn(q, k, positions, inv_freq, ends, False)
     return _rotate(q, k, positions, inv_freq, ends, False)

@@ -191,6 +191,91 @@ def test_rotary_under_transforms():
     assert all(torch.equal(a, b) for a, b in zip(compiled(q, k), want))
 
 
+def _second_inputs(sections, seed):
+    return [x.cuda() for x in _inputs(2, 4, 2, 17, 64, sum(sections), sections, F32, 500, seed=seed)]
+
+
+@pytest.mark.parametrize("keys", [True, False])
+@pytest.mark.parametrize("grad", [False, True])
+def test_rotary_is_recorded_by_whatever_traces(keys, grad):
+    """A traced function computes on the tensors that it is called with, with gradients and without."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    sections = (8, 24)
+
+    def turn(q, k, positions, inv_freq):
+        y, z = rotary_embedding(q, k if keys else None, positions, inv_freq, sections)
+        return (y, z) if keys else (y,)
+
+    first, second = _second_inputs(sections, 1), _second_inputs(sections, 2)
+    if grad:
+        first[0].requires_grad_(), first[1].requires_grad_(), second[0].requires_grad_(), second[1].requires_grad_()
+    want = turn(*second)
+    traced = {
+        "jit.trace": lambda: torch.jit.trace(turn, tuple(first), check_trace=False), "make_fx": lambda: make_fx(turn)(*first),
+        "make_fx, fake": lambda: make_fx(turn, tracing_mode="fake")(*first), "compile": lambda: torch.compile(turn, fullgraph=True),
+    }
+    for what, trace in traced.items():
+        got = trace()(*second)
+        got = got if isinstance(got, (tuple, list)) else (got,)
+        assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want)), what
+        if grad and what in ("jit.trace", "compile"):
+            leaves = second[: len(want)]
+            g = [torch.randn(x.shape, generator=torch.Generator().manual_seed(5)).cuda() for x in want]
+            a, b = torch.autograd.grad(got, leaves, g), torch.autograd.grad(turn(*second), leaves, g)
+            assert all(torch.equal(x, y) for x, y in zip(a, b)), what
+
+
+def test_rotary_under_modes_and_subclasses():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    class Sub(torch.Tensor):
+        pass
+
+    q, k, positions, inv_freq = _second_inputs((32,), 3)
+    want = rotary_embedding(q, k, positions, inv_freq)
+    with Mode():
+        got = rotary_embedding(q, k, positions, inv_freq)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and any("rotary" in s for s in seen)
+    got = rotary_embedding(q.as_subclass(Sub), k, positions, inv_freq)
+    assert all(torch.equal(a.as_subclass(torch.Tensor), b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):  # no rule for batches of calls
+        torch.func.vmap(lambda x: rotary_embedding(x, None, positions, inv_freq)[0])(q[None])
+    x = q.clone().requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t):
+        (d,) = torch.autograd.grad(rotary_embedding(x, k, positions, inv_freq)[0], x, q)
+    assert torch.equal(d, torch.autograd.grad(rotary_embedding(x, k, positions, inv_freq)[0], x, q)[0])
+    (d,) = torch.autograd.grad(torch.ops.kernels_b200.rotary_embedding(x, None, positions, inv_freq, [32], False)[0], x, q, create_graph=True)
+    assert torch.equal(d, torch.autograd.grad(rotary_embedding(x, None, positions, inv_freq)[0], x, q)[0]) and d.requires_grad is False
+
+
+def test_rotary_gradients_of_transforms_are_recorded_too():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    q, k, positions, inv_freq = _second_inputs((32,), 3)
+    t, other = torch.randn_like(q), torch.randn_like(q)
+    loss = lambda x, y: (rotary_embedding(x, None, y, inv_freq)[0] * t).sum()  # noqa: E731
+    leaf = q.clone().requires_grad_()
+    (want,) = torch.autograd.grad(loss(leaf, positions), leaf)
+    grad = torch.func.grad(loss)
+    assert torch.equal(grad(q, positions), want)
+    assert torch.equal(make_fx(grad)(other, positions.flip(-1))(q, positions), want)
+    assert torch.equal(torch.compile(grad)(q, positions), want)
+    tangent = lambda x, d: torch.func.jvp(lambda z: rotary_embedding(z, None, positions, inv_freq)[0], (x,), (d,))[1]  # noqa: E731
+    turned = rotary_embedding(t, None, positions, inv_freq)[0]
+    assert torch.equal(tangent(q, t), turned) and torch.equal(torch.compile(tangent)(q, t), turned)
+
+
 def test_rotary_in_a_graph_and_on_another_stream():
     from kernels_b200.streaming_attention import rotary_embedding
 
