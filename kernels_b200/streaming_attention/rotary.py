@@ -24,6 +24,8 @@ _pack = _lib.packer(_lib.RotaryParams).pack
 
 
 def _rotate(q, k, positions, inv_freq, ends, inverse):
+    if q.is_neg() or inv_freq.is_neg() or (k is not None and k.is_neg()):  # the sign is a mark on the tensor, which memory does not show
+        q, k, inv_freq = (x if x is None else x.resolve_neg() for x in (q, k, inv_freq))
     shape = q.shape
     B, H, T, D = shape
     q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), None

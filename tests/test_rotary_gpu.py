@@ -276,6 +276,28 @@ def test_rotary_gradients_of_transforms_are_recorded_too():
     assert torch.equal(tangent(q, t), turned) and torch.equal(torch.compile(tangent)(q, t), turned)
 
 
+def test_rotary_of_lazily_negated_tensors():
+    """The imaginary part of a conjugate carries its sign as a mark on the tensor: inputs, frequencies, gradients and tangents alike."""
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    q, k, positions, inv_freq = (x.cuda() for x in _inputs(2, 4, 2, 17, 64, 32, (32,), F32, 500))
+
+    def marked(x):
+        y = torch.complex(torch.zeros_like(x), -x).conj().imag
+        assert y.is_neg() and torch.equal(y, x)
+        return y
+
+    want = rotary_embedding(q, k, positions, inv_freq)
+    for change in (dict(q=marked(q)), dict(k=marked(k)), dict(inv_freq=marked(inv_freq))):
+        got = rotary_embedding(**(dict(q=q, k=k, positions=positions, inv_freq=inv_freq) | change))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), tuple(change)
+    x, y = q.clone().requires_grad_(), k.clone().requires_grad_()
+    out = rotary_embedding(x, y, positions, inv_freq)
+    plain = torch.autograd.grad(out, (x, y), (q, k), retain_graph=True)
+    got = torch.autograd.grad(out, (x, y), (marked(q), marked(k)))
+    assert all(torch.equal(a, b) for a, b in zip(got, plain))
+
+
 def test_rotary_in_a_graph_and_on_another_stream():
     from kernels_b200.streaming_attention import rotary_embedding
 
