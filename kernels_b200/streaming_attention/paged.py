@@ -46,6 +46,7 @@ def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
     P, H_kv, page, D = shape
     ks, vs = k_pages.stride(), v_pages.stride()
     assert page >= 1 and (ks[3] == vs[3] == 1 or 0 in shape), "rows of the pages are dense"
+    assert not (k_pages.is_neg() or v_pages.is_neg()), "the pages' memory holds their numbers, not the negated ones"
     table_shape, lens_shape = page_table.shape, lens.shape
     assert len(table_shape) == 2 and len(lens_shape) == 1 and page_table.dtype == lens.dtype == torch.int32
     B, M = table_shape
@@ -55,7 +56,7 @@ def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
     scales, code = _NO_SCALES, _lib.KB_E4M3
     if f8:
         assert k_scale.shape == v_scale.shape == shape[:3] and k_scale.dtype == v_scale.dtype == torch.float32
-        assert k_scale.get_device() == v_scale.get_device() == index
+        assert k_scale.get_device() == v_scale.get_device() == index and not (k_scale.is_neg() or v_scale.is_neg())
         scales = k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride()
     else:
         code = _lib.dtype_code(dtype)
@@ -67,7 +68,7 @@ def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
 def _per_row(name, x, dtype, B, H_kv, rows, index):
     """Pointer and strides of ``weights`` or ``row_positions``."""
     shape, strides = x.shape, x.stride()
-    assert x.dtype == dtype and x.get_device() == index and len(shape) == 3 and shape[0] == B and shape[1] == H_kv, f"{name} is [B, H_kv, M * page]"
+    assert x.dtype == dtype and x.get_device() == index and not x.is_neg() and len(shape) == 3 and shape[0] == B and shape[1] == H_kv, f"{name} is [B, H_kv, M * page]"
     assert shape[2] >= rows and (strides[2] == 1 or shape[2] <= 1), f"{name} has an entry for every row, side by side"
     assert (strides[0] or B <= 1) and (strides[1] or H_kv <= 1), f"{name} is written: every sequence and head has entries of its own"
     return x.data_ptr(), strides[0], strides[1]
@@ -112,6 +113,8 @@ def paged_cache_write(
     """
     cache, index, rows = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale)
     shape, dtype = k.shape, k.dtype
+    if k.is_neg() or v.is_neg():  # (the sign is a mark on the tensor, which memory does not show)
+        k, v = k.resolve_neg(), v.resolve_neg()
     assert len(shape) == 4 and v.shape == shape and v.dtype == dtype and k.get_device() == v.get_device() == index
     B, H_kv, T, D = shape
     pages_shape, lens_shape = k_pages.shape, lens.shape
@@ -168,8 +171,8 @@ def paged_attention(
     assert context_size is None or context_size >= 1
     assert back_contexts >= 0
     strides = q.stride()
-    if strides[2] != 1 or strides[0] % 2 or strides[1] % 2 or q.data_ptr() % 4:
-        q = q.contiguous()  # (the tensor-core kernel takes pairs of elements)
+    if strides[2] != 1 or strides[0] % 2 or strides[1] % 2 or q.data_ptr() % 4 or q.is_neg():
+        q = q.resolve_neg().contiguous()  # (the tensor-core kernel takes pairs of elements)
         strides = q.stride()
     o = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     lse = lens.new_empty((B, H), dtype=torch.float32) if return_lse or weights is not None else None

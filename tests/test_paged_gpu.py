@@ -822,6 +822,36 @@ def test_two_streams_at_once():
     for a, b in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
+def test_lazily_negated_tensors():
+    """A tensor whose sign is a mark on it (the imaginary part of a conjugate): new tokens and queries are taken as the numbers that they are, a cache
+    like that is refused."""
+    from kernels_b200.streaming_attention import paged_attention, paged_cache_evict, paged_cache_write
+
+    def marked(x):
+        y = torch.complex(torch.zeros_like(x), -x).conj().imag
+        assert y.is_neg() and torch.equal(y, x)
+        return y
+
+    c = make_cache(2, 2, 64, 16, [40, 30], F32)
+    k, v, q = torch.randn(2, 2, 3, 64), torch.randn(2, 2, 3, 64), torch.randn(2, 4, 64)
+    check_write(c, k, v, kg=marked(k.cuda()))
+    check_write(c, k, v, vg=marked(v.cuda()))
+    g = cuda(c)
+    pages = dict(k_pages=g["k_pages"], v_pages=g["v_pages"], page_table=g["page_table"], lens=g["lens"])
+    want = paged_attention(q.cuda(), **pages)
+    assert torch.equal(paged_attention(marked(q.cuda()), **pages), want)
+    w, pos = torch.zeros(2, 2, 48, device="cuda"), torch.zeros(2, 2, 48, dtype=torch.int32, device="cuda")
+    for change in (dict(k_pages=marked(g["k_pages"])), dict(v_pages=marked(g["v_pages"])), dict(weights=marked(w))):
+        with pytest.raises(AssertionError):
+            paged_attention(**(dict(q=q.cuda()) | pages | change))
+        with pytest.raises(AssertionError):
+            paged_cache_write(**(dict(k=k.cuda(), v=v.cuda()) | pages | change))
+        with pytest.raises(AssertionError):
+            paged_cache_evict(**(dict(weights=w, row_positions=pos, budget=8) | pages | change))
+    f8 = cuda(make_cache(2, 2, 64, 16, [40, 30], F8))
+    with pytest.raises(AssertionError):
+        paged_attention(q.cuda(), f8["k_pages"], f8["v_pages"], f8["page_table"], f8["lens"], k_scale=marked(f8["k_scale"]), v_scale=f8["v_scale"])
+
 
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
