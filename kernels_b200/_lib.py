@@ -358,6 +358,20 @@ def looked_into(*tensors) -> bool:
     return False
 
 
+def refuse_recording(what: str) -> None:
+    """Raise where jit tracing or ``make_fx`` records operators: ``what`` is none, and would be missing from the record."""
+    if _can_tell_plain and _tracing_state() is None:
+        if not _dispatch_modes():
+            return
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is None:
+            return
+    elif not torch.jit.is_tracing():
+        return
+    raise RuntimeError(f"{what}: not an operator, cannot be traced")
+
+
 def launch_count() -> int:
     return int(load().kb_launch_count())
 

@@ -14,7 +14,8 @@ pages that every sequence lists in a table of its own:
   that each cached row has received and its token's position.  They belong to sequences, as the table's rows do.
 
 The calls read lengths and tables on the device, so a decoding step can be captured into a graph and replayed.  They allocate their
-workspace with torch on the current stream.  Forward only (inference).  There is no CPU path.
+workspace with torch on the current stream.  Forward only (inference): outputs have no gradient, and a call under ``jit.trace`` or ``make_fx``,
+which it would be missing from, is refused (a compiled function steps out for it).  There is no CPU path.
 """
 
 from __future__ import annotations
@@ -40,6 +41,7 @@ def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
     of calls that take about ten: every property of a tensor is asked for once, devices by their index.)"""
     if not (k_pages.is_cuda and v_pages.is_cuda):
         raise RuntimeError(f"{what}: the tensors must live on a CUDA device (there is no CPU path)")
+    _lib.refuse_recording(what)
     index, shape, dtype = k_pages.get_device(), k_pages.shape, k_pages.dtype
     assert len(shape) == 4 and v_pages.shape == shape and v_pages.dtype == dtype, "k_pages and v_pages are [P, H_kv, page, D]"
     assert v_pages.get_device() == page_table.get_device() == lens.get_device() == index

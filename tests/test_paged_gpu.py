@@ -853,6 +853,50 @@ def test_lazily_negated_tensors():
         paged_attention(q.cuda(), f8["k_pages"], f8["v_pages"], f8["page_table"], f8["lens"], k_scale=marked(f8["k_scale"]), v_scale=f8["v_scale"])
 
 
+def test_calls_under_whatever_traces_are_refused():
+    """What records operators would record nothing of these calls."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from kernels_b200.streaming_attention import paged_attention, paged_cache_evict, paged_cache_write
+
+    g = cuda(make_cache(2, 2, 64, 16, [40, 30], F32))
+    pages, q = dict(k_pages=g["k_pages"], v_pages=g["v_pages"], page_table=g["page_table"], lens=g["lens"]), torch.randn(2, 4, 64)
+    w, pos = torch.zeros(2, 2, 48, device="cuda"), torch.zeros(2, 2, 48, dtype=torch.int32, device="cuda")
+    calls = (lambda x: paged_attention(x, **pages), lambda x: paged_cache_write(x[:, :2, None], x[:, :2, None], **pages) or x,
+             lambda x: paged_cache_evict(**pages, weights=w, row_positions=pos, budget=8)[1] + x[0, 0, 0])
+    before = {n: x.clone() for n, x in g.items()}
+    for call in calls:
+        with pytest.raises(RuntimeError, match="trac"):
+            torch.jit.trace(call, (q.cuda(),), check_trace=False)
+        with pytest.raises(RuntimeError, match="trac"):
+            make_fx(call)(q.cuda())
+    for call in calls[:2]:  # (no rule for batches of calls; the third has none of a batch's tensors)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(q.cuda()[None])
+    assert all(torch.equal(before[n], g[n]) for n in g)
+
+
+def test_calls_from_a_compiled_function():
+    """A compiled function steps out for these calls: the eager results."""
+    from kernels_b200.streaming_attention import paged_attention, paged_cache_evict, paged_cache_write
+
+    c = make_cache(2, 2, 64, 16, [90, 70], F16)
+    w, pos = make_books(2, 2, c["page_table"].shape[1] * 16)
+    q, k = torch.randn(2, 4, 64).half().cuda(), torch.randn(2, 2, 3, 64).half().cuda()
+
+    def step(g, w, pos, q, k):
+        paged_cache_write(k * 2, k, g["k_pages"], g["v_pages"], g["page_table"], g["lens"], weights=w, row_positions=pos)
+        o = paged_attention(q * 2, g["k_pages"], g["v_pages"], g["page_table"], g["lens"], weights=w) + 1
+        paged_cache_evict(g["k_pages"], g["v_pages"], g["page_table"], g["lens"], w, pos, 50, 4)
+        return o
+
+    results = []
+    for f in (step, torch.compile(step)):
+        g = cuda(c | dict(w=w, pos=pos))
+        results.append((f(g, g["w"], g["pos"], q, k), g))
+    (a, x), (b, y) = results
+    assert torch.equal(a, b) and all(torch.equal(x[n], y[n]) for n in x)
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------------
 
 
