@@ -451,7 +451,8 @@ KB_API int kb_paged_write(const kb_paged_write_params* p, void* stream);
  * rows r with (lens[b] - 1) / context_size - r / context_size <= back_contexts.  A sequence without rows gives 0 and lse 0.
  * `lse` is base 2.  With `weights`, every seen row's softmax weight, summed over the query heads of its key/value head, is
  * added to weights[b][head][row]; `lse` must then be given.  `workspace`: kb_paged_attention_workspace_bytes bytes of the same, otherwise
- * filled-in block (host-only; it looks at sizes, strides, alignment and at whether `weights` is NULL), 16-byte aligned.
+ * filled-in block (host-only; it looks at sizes, strides, alignment and at whether `weights` is NULL; 0 for a block that would be refused),
+ * 16-byte aligned.
  * The tensor-core kernel takes head dims 64 and 128 where q's heads are dense and keys and values have one layout with rows on
  * 16-byte boundaries (an e4m3 cache: and a 16-bit q); everything else goes to a CUDA-core kernel.  fp32 is multiplied in three tf32 products,
  * as exact as fp32 for numbers, but an infinity in a row counts as a NaN there.

@@ -49,6 +49,22 @@ int check_paged_cache(const kb_paged_cache& c) {
 }
 bool no_rows(const kb_paged_cache& c) { return c.M == 0; }
 
+// What the launch and the query of its workspace ask alike: sizes and types, no pointers but the cache's.
+int check_paged_attention_sizes(const kb_paged_attention_params* p) {
+  if (!p || p->H < 0 || p->context_size < 0 || p->back_contexts < 0) return KB_ERR_BAD_ARGUMENT;
+  if (int rc = check_paged_cache(p->cache)) return rc;
+  if (!dtype_ok(p->dtype) || (p->cache.dtype != KB_E4M3 && p->cache.dtype != p->dtype)) return KB_ERR_UNSUPPORTED;
+  if (empty(p->cache.B, 1, p->H)) return KB_OK;
+  if (p->cache.H_kv < 1 || p->H % p->cache.H_kv) return KB_ERR_BAD_ARGUMENT;
+  if (p->H > 65535 || (int64_t)p->cache.B * p->H > (int64_t)1 << 30) return KB_ERR_TOO_LARGE;
+  return KB_OK;
+}
+int check_paged_evict_sizes(const kb_paged_evict_params* p) {
+  if (!p || p->budget < 1 || p->recent < 0) return KB_ERR_BAD_ARGUMENT;
+  if (int rc = check_paged_cache(p->cache)) return rc;
+  return p->cache.B > 0 && p->cache.H_kv < 1 ? KB_ERR_BAD_ARGUMENT : KB_OK;
+}
+
 // The tcgen05 path wants 16-bit inputs, a head dim of 64 or 128, unit stride along the head
 // dim and 16-byte aligned rows (TMA's requirements on the tensor map).
 bool tma_ok(const kb_tensor4& t, size_t elsize) {
@@ -442,32 +458,28 @@ int kb_paged_write(const kb_paged_write_params* p, void* stream) {
 }
 
 uint64_t kb_paged_attention_workspace_bytes(const kb_paged_attention_params* p) {
-  if (!p || p->H < 0 || kb::check_paged_cache(p->cache) || kb::empty(p->cache.B, p->cache.H_kv, p->H)) return 0;
+  if (kb::check_paged_attention_sizes(p) || kb::empty(p->cache.B, 1, p->H)) return 0;
   return kb::paged_attention_workspace_bytes(*p);
 }
 
 int kb_paged_attention(const kb_paged_attention_params* p, void* stream) {
-  if (!p || p->H < 0 || p->context_size < 0 || p->back_contexts < 0) return KB_ERR_BAD_ARGUMENT;
-  if (int rc = kb::check_paged_cache(p->cache)) return rc;
-  if (!kb::dtype_ok(p->dtype) || (p->cache.dtype != KB_E4M3 && p->cache.dtype != p->dtype)) return KB_ERR_UNSUPPORTED;
+  if (int rc = kb::check_paged_attention_sizes(p)) return rc;
   if (kb::empty(p->cache.B, 1, p->H)) return KB_OK;
-  if (p->cache.H_kv < 1 || p->H % p->cache.H_kv || !p->q || !p->o || (p->weights && !p->lse)) return KB_ERR_BAD_ARGUMENT;
-  if (p->H > 65535 || (int64_t)p->cache.B * p->H > (int64_t)1 << 30) return KB_ERR_TOO_LARGE;
+  if (!p->q || !p->o || (p->weights && !p->lse)) return KB_ERR_BAD_ARGUMENT;
   const uint64_t need = kb::paged_attention_workspace_bytes(*p);
   if (need && (!p->workspace || p->workspace_bytes < need || reinterpret_cast<uintptr_t>(p->workspace) % 16)) return KB_ERR_BAD_ARGUMENT;
   return kb::paged_attention(*p, static_cast<cudaStream_t>(stream));
 }
 
 uint64_t kb_paged_evict_workspace_bytes(const kb_paged_evict_params* p) {
-  if (!p || p->budget < 1 || kb::check_paged_cache(p->cache)) return 0;
+  if (kb::check_paged_evict_sizes(p) || p->cache.B == 0) return 0;
   return kb::paged_evict_workspace_bytes(p->cache, p->budget);
 }
 
 int kb_paged_evict(const kb_paged_evict_params* p, void* stream) {
-  if (!p || p->budget < 1 || p->recent < 0) return KB_ERR_BAD_ARGUMENT;
-  if (int rc = kb::check_paged_cache(p->cache)) return rc;
+  if (int rc = kb::check_paged_evict_sizes(p)) return rc;
   if (p->cache.B == 0) return KB_OK;
-  if (!p->lens_out || p->cache.H_kv < 1) return KB_ERR_BAD_ARGUMENT;
+  if (!p->lens_out) return KB_ERR_BAD_ARGUMENT;
   if (!kb::no_rows(p->cache) && (!p->weights || !p->row_positions || !p->weights_out || !p->row_positions_out)) return KB_ERR_BAD_ARGUMENT;
   const bool in_place = p->weights == p->weights_out;
   if (!kb::no_rows(p->cache) && (in_place != (p->row_positions == p->row_positions_out) || in_place != (p->cache.lens == p->lens_out)))

@@ -95,6 +95,44 @@ def test_call_refusals():
         r.section_end[:] = [32] + [0] * 7
         assert lib.kb_rotary(C.byref(r), None) == status, change
 
+def test_workspace_queries_refuse_what_the_calls_refuse():
+    """The host-only queries are asked before the call: 0 for every block that the call does not take, head counts of which nothing can be shared out among them."""
+    lib = _lib.load()
+
+    def attention(**change):
+        p = _lib.PagedAttentionParams()
+        p.cache = change.pop("cache", _cache())
+        p.q = p.o = p.lse = p.weights = 4096
+        p.H, p.dtype, p.sm_scale = 4, _lib.KB_F16, 1.0
+        for n, x in change.items():
+            setattr(p, n, x)
+        return lib.kb_paged_attention_workspace_bytes(C.byref(p))
+
+    def evict(**change):
+        p = _lib.PagedEvictParams()
+        p.cache = change.pop("cache", _cache())
+        p.budget, p.recent = 8, 2
+        for n, x in change.items():
+            setattr(p, n, x)
+        return lib.kb_paged_evict_workspace_bytes(C.byref(p))
+
+    assert attention() > 0 and evict() > 0
+    for change, _ in CACHE_REFUSALS:
+        assert attention(cache=_cache(**change)) == 0 and evict(cache=_cache(**change)) == 0, change
+    heads = _cache(H_kv=4)
+    for change in (dict(H=-4), dict(H=3), dict(H=2, cache=heads), dict(H=1, cache=heads), dict(H=0), dict(H=65538), dict(context_size=-1), dict(back_contexts=-1),
+                   dict(dtype=_lib.KB_BF16), dict(dtype=3), dict(dtype=-1), dict(cache=_cache(H_kv=0)), dict(cache=_cache(B=0)), dict(cache=_cache(B=40000), H=32768)):
+        assert attention(**change) == 0, change
+    for dtype in (_lib.KB_F32, _lib.KB_F16, _lib.KB_BF16):
+        for H_kv in (2, 4, 64):
+            for D in (16, 64, 128, 256):
+                c = _cache(H_kv=H_kv, D=D, dtype=dtype)
+                c.k_stride[:] = c.v_stride[:] = [16 * D * H_kv, 16 * D, D]
+                for H in range(1, 3 * H_kv + 1):
+                    assert (attention(H=H, dtype=dtype, cache=c) > 0) == (H % H_kv == 0), (dtype, H_kv, D, H)
+    for change in (dict(budget=0), dict(budget=-1), dict(recent=-1), dict(cache=_cache(H_kv=0)), dict(cache=_cache(B=0))):
+        assert evict(**change) == 0, change
+
 
 @pytest.mark.parametrize("cls", [_lib.PagedCache, _lib.RotaryParams, _lib.PagedWriteParams, _lib.PagedAttentionParams, _lib.PagedEvictParams, _lib.SaBwdParams])
 def test_packed_blocks_are_the_structures_bytes(cls):
