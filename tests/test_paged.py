@@ -104,6 +104,7 @@ def test_workspace_queries_refuse_what_the_calls_refuse():
         p.cache = change.pop("cache", _cache())
         p.q = p.o = p.lse = p.weights = 4096
         p.H, p.dtype, p.sm_scale = 4, _lib.KB_F16, 1.0
+        p.q_stride[:] = [256, 64, 1]  # (dense heads: the tensor-core kernel's, where the head dim is)
         for n, x in change.items():
             setattr(p, n, x)
         return lib.kb_paged_attention_workspace_bytes(C.byref(p))
