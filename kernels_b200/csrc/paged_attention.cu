@@ -41,7 +41,8 @@ struct AttendArgs {
   int4* join;       // [items] with by_item, otherwise by the unit that starts the item, [units]: {first part (-1: none), its unit, last unit, item}
   float* part_o;    // [2 units, heads, D]
   float4* part_ml;  // [2 units, heads]: maximum, sum of the weights, sum of what was multiplied with V (the weights as rounded), 0
-  float* scores;    // [B, H, capacity], base-2 logits
+  float* scores;    // [B, H, most_rows], base-2 logits, from the first row that is seen
+  int32_t most_rows;  // that a token can see
   KbFastDiv fd_context;
   uint32_t row16[3], scale_at[3];  // tensor-core kernel: page, head and row strides of keys and values in 16 bytes, of their scales in elements
 };
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
     const int32_t n = (int32_t)min((int64_t)(at.tiles - at.tile), at.left);
     const int32_t b = at.b, hk = at.hy / a.head_tiles, h0 = hk * a.group + (at.hy - hk * a.head_tiles) * G, heads = min(G, (hk + 1) * a.group - h0);
     const int32_t slot = part_of_item(a, stretch, at, unit, seen, n, threadIdx.x == 0);
-    const int32_t begin = at.first + at.tile * kRows, end = kb_min_i32(at.end, begin + n * kRows);
+    const int32_t first = at.first, begin = first + at.tile * kRows, end = kb_min_i32(at.end, begin + n * kRows);
     at.advance(a, kRows, n);
     seen += n;
 
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) paged_attend_kernel(const AttendArgs
 #pragma unroll
           for (int x = kLanes / 2; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
           s = live ? s * ks[j] : -INFINITY;
-          if (a.scores && piece == 0 && r < end && g < heads) a.scores[((int64_t)b * a.H + h0 + g) * a.c.capacity + r] = s;
+          if (a.scores && piece == 0 && r < end && g < heads) a.scores[((int64_t)b * a.H + h0 + g) * a.most_rows + (r - first)] = s;
           if (!live) continue;
           const float top = fmaxf(m[g], s), base = top == -INFINITY ? 0.f : top;
           const float p = exp2f(s - base), keep = exp2f(m[g] - base);
@@ -526,8 +527,8 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
     const int32_t n = (int32_t)min((int64_t)(now.tiles - now.tile), now.left);
     const int32_t b = now.b, hk = now.hy / a.head_tiles, h0 = hk * a.group + (now.hy - hk * a.head_tiles) * kHeads, heads = min(kHeads, (hk + 1) * a.group - h0);
     const int32_t slot = part_of_item(a, stretch, now, unit, seen, n, lane == 0);
-    int32_t r0 = now.first + now.tile * kR;
-    const int32_t end = now.end;
+    int32_t r0 = now.tile * kR;  // counted from the first row that is seen, as the scores lie
+    const int32_t end = now.end - now.first;
     now.advance(a, kR, n);
     seen += n;
 
@@ -710,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
           for (int i = 0; i < 2; ++i) {
             const int g = 8 * e + 2 * quad + i;
             if (g >= heads) continue;
-            float* out = a.scores + ((int64_t)b * a.H + h0 + g) * a.c.capacity + r0 + oct;
+            float* out = a.scores + ((int64_t)b * a.H + h0 + g) * a.most_rows + r0 + oct;
 #pragma unroll
             for (int u = 0; u < kU; ++u)
 #pragma unroll
@@ -932,12 +933,12 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const AttendArgs a) {
   wait_for_launch_before();
   const int32_t r0 = first + blockIdx.x * kWeighRows + threadIdx.x;
   if (r0 >= end) return;
-  const float *scores = a.scores + bh * a.c.capacity + r0, *lse = a.lse + bh;
+  const float *scores = a.scores + bh * a.most_rows + (r0 - first), *lse = a.lse + bh;
   float* to = a.weights + b * a.w_b + hk * a.w_h + r0;
   float w[kEach], x[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) w[i] = 0.f;
-  for (int g = 0; g < a.group; ++g, scores += a.c.capacity) {
+  for (int g = 0; g < a.group; ++g, scores += a.most_rows) {
     const float base = lse[g];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) x[i] = r0 + i * 256 < end ? __ldcs(scores + i * 256) : -INFINITY;
@@ -1075,7 +1076,8 @@ Plan make_plan(const kb_paged_attention_params& p) {
   n.join_bytes = entries * sizeof(int4);
   n.part_bytes = parts * c.D * sizeof(float);
   n.ml_bytes = parts * sizeof(float4);
-  n.score_bytes = p.weights ? (size_t)c.B * p.H * capacity * sizeof(float) : 0;
+  // (a window's first row is the first of a chunk: from there to the last row there are most_rows at most)
+  n.score_bytes = p.weights ? (size_t)c.B * p.H * n.most_rows * sizeof(float) : 0;
   return n;
 }
 
@@ -1110,7 +1112,7 @@ int paged_attention(const kb_paged_attention_params& p, cudaStream_t s) {
     a.join = reinterpret_cast<int4*>(w), w += n.join_bytes;
     a.part_o = reinterpret_cast<float*>(w), w += n.part_bytes;
     a.part_ml = reinterpret_cast<float4*>(w), w += n.ml_bytes;
-    if (p.weights) a.scores = reinterpret_cast<float*>(w);
+    if (p.weights) a.scores = reinterpret_cast<float*>(w), a.most_rows = n.most_rows;
     if (int rc = kernel.launch(a, paged_rows_aligned(c, dtype_size(c.dtype)), s)) return rc;
     if (n.joins) {
       const dim3 grid((unsigned)(n.join_bytes / sizeof(int4)), kb_min_i32(n.heads, a.group));

@@ -157,7 +157,7 @@ def paged_attention(
     operator's mask applies (``kernel.py:1540-1542``): the token sees its own chunk and ``back_contexts`` chunks before it, counted in rows.
     Returns ``o`` ``[B, H, D]`` and, on request, the base-2 log-sum-exp ``[B, H]``; both are 0 for a sequence that sees
     no row.  With ``weights``, the softmax weight of every row that is seen, summed over the query heads of its key/value
-    head, is added to ``weights`` in place.
+    head, is added to ``weights`` in place; that takes 4 bytes of workspace per query head and row that a token can see (of the window, or of the table).
 
     Sums are held in fp32.  16-bit and e4m3 caches: weights are rounded to 16 bits before they are multiplied with ``v``.  fp32 caches of head dim 64
     and 128 are multiplied on the tensor cores in three parts, as exactly as in fp32; an infinity in a row counts as a NaN there.

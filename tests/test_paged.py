@@ -164,6 +164,20 @@ def test_workspace_of_a_long_cache_passes_32_bits():
     p.H, p.dtype, p.weights, p.lse = 64, _lib.KB_F16, 4096, 4096
     assert lib.kb_paged_attention_workspace_bytes(C.byref(p)) >= 64 * 64 * (1 << 20) * 4
 
+def test_workspace_of_a_window_does_not_follow_the_table():
+    """Scores take the room of the rows that a token can see."""
+    lib = _lib.load()
+    sizes = []
+    for M in (1 << 6, 1 << 14):
+        p = _lib.PagedAttentionParams()
+        p.cache = _cache(B=64, M=M, page=64, H_kv=8, D=128)
+        p.q_stride[:] = [32 * 128, 128, 1]
+        p.H, p.dtype, p.weights, p.lse, p.context_size, p.back_contexts = 32, _lib.KB_F16, 4096, 4096, 512, 1
+        sizes.append(lib.kb_paged_attention_workspace_bytes(C.byref(p)))
+        p.weights = None
+        sizes.append(lib.kb_paged_attention_workspace_bytes(C.byref(p)))
+    assert sizes[0] == sizes[2] and sizes[0] - sizes[1] == sizes[2] - sizes[3] == 64 * 32 * 1024 * 4
+
 
 def test_cpu_tensors_are_refused():
     from kernels_b200.streaming_attention import paged_attention, paged_cache_evict, paged_cache_write, rotary_embedding

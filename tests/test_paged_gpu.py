@@ -179,6 +179,30 @@ def test_attention_masks_rows_without_a_page(dtype):
     check_attend(c, q, weights=torch.zeros(4, 2, c["page_table"].shape[1] * 16))
     check_attend(c, q, 16, 1)
 
+def test_a_windows_weights_need_no_workspace_of_the_tables_width():
+    """Room for scores follows the rows that a token can see: a table for a long context costs a windowed step nothing."""
+    from kernels_b200.streaming_attention import paged_attention
+
+    lens, M = [1000, 64, 129, 0, 700], 65536
+    c = make_cache(5, 2, 64, 16, lens, BF16)
+    wide = torch.full((5, M), -1, dtype=torch.int32)
+    wide[:, : c["page_table"].shape[1]] = c["page_table"]
+    q = torch.randn(5, 8, 64).bfloat16()
+    for context_size, back in ((128, 1), (1, 0), (64, 3)):
+        weights = torch.rand(5, 2, 1008)
+        check_attend(c, q, context_size, back, weights=weights)
+        g = cuda(c)
+        tight, broad = (torch.zeros(5, 2, n, device="cuda") for n in (1008, M * 16))
+        args = (q.cuda(), g["k_pages"], g["v_pages"])
+        a = paged_attention(*args, g["page_table"], g["lens"], context_size, back, weights=tight)
+        table = wide.cuda()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        b = paged_attention(*args, table, g["lens"], context_size, back, weights=broad)
+        assert torch.cuda.max_memory_allocated() - before < 32 << 20  # (scores for the table's width: 160 MB)
+        assert torch.equal(a, b) and torch.equal(tight, broad[..., :1008]) and not broad[..., 1008:].any()
+
 
 def test_attention_lengths_beyond_the_table_are_clamped():
     c = make_cache(3, 2, 64, 16, [64, 64, 64], F16)
