@@ -36,7 +36,7 @@ _pack_evict = _lib.packer(_lib.PagedEvictParams).pack
 _NO_SCALES = (0,) * 8
 
 
-def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
+def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale, written=False):
     """The checked cache: the numbers of the C ABI's ``kb_paged_cache``, the device's index and the rows that a table names.  (A few microseconds
     of calls that take about ten: every property of a tensor is asked for once, devices by their index.)"""
     if not (k_pages.is_cuda and v_pages.is_cuda):
@@ -62,6 +62,9 @@ def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
         scales = k_scale.data_ptr(), v_scale.data_ptr(), *k_scale.stride(), *v_scale.stride()
     else:
         code = _lib.dtype_code(dtype)
+    if written and (0 in ks or 0 in vs or (f8 and 0 in scales)):
+        for name, s in (("k_pages", ks), ("v_pages", vs), ("k_scale", scales[2:5]), ("v_scale", scales[5:]))[: 4 if f8 else 2]:
+            assert (s[0] or P <= 1) and (s[1] or H_kv <= 1) and (s[2] or page <= 1), f"{name} is written: every page, head and row has memory of its own"
     cache = (k_pages.data_ptr(), v_pages.data_ptr(), *ks[:3], *vs[:3], *scales, page_table.data_ptr(), *page_table.stride(), lens.data_ptr(), lens.stride(0),
              B, H_kv, D, P, M, page, code)
     return cache, index, M * page
@@ -70,7 +73,7 @@ def _pages(what, k_pages, v_pages, page_table, lens, k_scale, v_scale):
 def _per_row(name, x, dtype, B, H_kv, rows, index):
     """Pointer and strides of ``weights`` or ``row_positions``."""
     shape, strides = x.shape, x.stride()
-    assert x.dtype == dtype and x.get_device() == index and not x.is_neg() and len(shape) == 3 and shape[0] == B and shape[1] == H_kv, f"{name} is [B, H_kv, M * page]"
+    assert x.dtype == dtype and x.get_device() == index and not (dtype.is_floating_point and x.is_neg()) and len(shape) == 3 and shape[0] == B and shape[1] == H_kv, f"{name} is [B, H_kv, M * page]"
     assert shape[2] >= rows and (strides[2] == 1 or shape[2] <= 1), f"{name} has an entry for every row, side by side"
     assert (strides[0] or B <= 1) and (strides[1] or H_kv <= 1), f"{name} is written: every sequence and head has entries of its own"
     return x.data_ptr(), strides[0], strides[1]
@@ -113,7 +116,7 @@ def paged_cache_write(
     0, those of ``row_positions`` the tokens' ``positions`` (int32 ``[B, T]``, None for the rows themselves).  Rows outside the table
     are dropped; two tokens of one call must not share a row of a page.
     """
-    cache, index, rows = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale)
+    cache, index, rows = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale, True)
     shape, dtype = k.shape, k.dtype
     if k.is_neg() or v.is_neg():  # (the sign is a mark on the tensor, which memory does not show)
         k, v = k.resolve_neg(), v.resolve_neg()
@@ -212,7 +215,7 @@ def paged_cache_evict(
     ``out``: a ``(lens, weights, row_positions)`` to be written instead, not overlapping the given ones (entries of
     the rows that remain; the pages change all the same).  Sequences that share pages need copies of their own first.
     """
-    cache, index, rows = _pages("paged_cache_evict", k_pages, v_pages, page_table, lens, k_scale, v_scale)
+    cache, index, rows = _pages("paged_cache_evict", k_pages, v_pages, page_table, lens, k_scale, v_scale, True)
     assert budget >= 1 and recent >= 0, "at least one row stays"
     B, H_kv = lens.shape[0], k_pages.shape[1]
     w = _per_row("weights", weights, torch.float32, B, H_kv, rows, index)
@@ -222,6 +225,7 @@ def paged_cache_evict(
         w_out, p_out = w, p
     else:
         assert len(out) == 3 and out[0].shape == lens.shape and out[0].dtype == torch.int32 and out[0].get_device() == index
+        assert out[0].stride(0) or B <= 1, "out[0] is written: every sequence has a length of its own"
         w_out = _per_row("out[1]", out[1], torch.float32, B, H_kv, rows, index)
         p_out = _per_row("out[2]", out[2], torch.int32, B, H_kv, rows, index)
     block = _pack_evict(*cache, *w, *p, *w_out, *p_out, out[0].data_ptr(), out[0].stride(0), 0, 0, _clamp_i32(budget), _clamp_i32(recent))

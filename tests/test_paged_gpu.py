@@ -965,3 +965,33 @@ def test_refusals():
         with pytest.raises(RuntimeError, match="unsupported"):
             paged_attention(**(pages | change))
     assert all(torch.equal(before[n], g[n]) for n in g)
+
+
+def test_written_tensors_that_overlap_themselves_are_refused():
+    """One place in memory for several rows, heads or lengths: reading them is fine, writing them would depend on the order."""
+    from kernels_b200.streaming_attention import paged_attention, paged_cache_evict, paged_cache_write
+
+    c = make_cache(2, 2, 64, 16, [40, 30], F8)
+    g = cuda(c)
+    w, pos = torch.zeros(2, 2, 48, device="cuda"), torch.zeros(2, 2, 48, dtype=torch.int32, device="cuda")
+    k = torch.randn(2, 2, 3, 64, device="cuda")
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    pages = {n: g[n] for n in ("k_pages", "v_pages", "page_table", "lens", "k_scale", "v_scale")}
+    one = lambda x, d: x.narrow(d, 0, 1).expand(x.shape)  # noqa: E731
+    for name in ("k_pages", "v_pages", "k_scale", "v_scale"):
+        for d in range(3):
+            change = {name: one(g[name], d)}
+            assert paged_attention(q, **(pages | change)).shape == q.shape
+            with pytest.raises(AssertionError):
+                paged_cache_write(k, k, **(pages | change))
+            with pytest.raises(AssertionError):
+                paged_cache_evict(**(pages | change), weights=w, row_positions=pos, budget=8)
+    with pytest.raises(AssertionError):
+        paged_cache_evict(**pages, weights=w, row_positions=pos, budget=8, out=(g["lens"][:1].expand(2), w.clone(), pos.clone()))
+    # a single page, head or row may have any stride
+    small = {n: torch.zeros(1, 1, 1, *s, dtype=t, device="cuda").expand(1, 1, 1, *s) for n, s, t in (("k_pages", (64,), F16), ("v_pages", (64,), F16))}
+    small = {n: x.as_strided(x.shape, (0, 0, 0, 1)) for n, x in small.items()}
+    i = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    x = torch.randn(1, 1, 1, 64, device="cuda").half()
+    paged_cache_write(x, x, **small, page_table=i([[0]]), lens=i([1]))
+    assert torch.equal(small["k_pages"], x) and torch.equal(small["v_pages"], x)
