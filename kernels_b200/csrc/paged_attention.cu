@@ -506,6 +506,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
       }
     }
     look_up();
+    __syncwarp();  // (the matrix loads and products want the warp together again)
     return live;
   };
   look_up();
@@ -718,6 +719,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
               for (int r = 0; r < 2; ++r)
                 if (r0 + u * 16 + r * 8 + oct < end) out[u * 16 + r * 8] = sc[u][e][2 * r + i];
           }
+        __syncwarp();
       }
       bool raise = false;
 #pragma unroll

@@ -254,6 +254,11 @@ struct Team {
   int (*of_rank)[8];    // [2][ranks]
   int size, rank, turn; // of the cluster
 
+  // Every thread of the cluster's blocks.  (The barrier wants whole warps that are together again, which code that only some lanes run leaves open.)
+  static __device__ __forceinline__ void meet() {
+    __syncwarp();
+    sm100::cluster_sync_all();
+  }
   // `x` into `to`, a variable of every block's shared memory
   __device__ __forceinline__ void tell(uint32_t* to, uint32_t x) const {
     if (size == 1) {
@@ -282,7 +287,7 @@ struct Team {
         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(sm100::smem_u32(&of_rank[turn][rank])), "r"(threadIdx.x));
         asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to), "r"(sum) : "memory");
       }
-      sm100::cluster_sync_all();
+      meet();
       const int theirs = lane < size ? of_rank[turn][lane] : none;
       if (before) {
         const int lower = op(lane < rank ? theirs : none);
@@ -341,7 +346,7 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
   Team team{red, of_rank, a.cluster, (int)blockIdx.x % a.cluster, 0};
   const SelectHead s(a, blockIdx.y, blockIdx.x / a.cluster);
   const int32_t n = s.n, row0 = (team.rank * warps + warp) * kWarpRows + lane;
-  if (a.cluster > 1) sm100::cluster_sync_all();  // (a block's shared memory may be written once the block has started)
+  if (a.cluster > 1) team.meet();  // (a block's shared memory may be written once the block has started)
 
   uint32_t key[kKeys], live = 0;  // live: the rows that count
   int64_t from;                   // positions above it are among the newest
@@ -419,7 +424,7 @@ __global__ void __launch_bounds__(1024) paged_select_kernel(const EvictArgs a) {
 #pragma unroll
       for (int j = 0; j < kKeys; ++j)
         if ((picked >> j) & 1) team.tell(&few[at++], key[j]);
-      if (team.size > 1) sm100::cluster_sync_all();
+      if (team.size > 1) team.meet();
       else __syncthreads();
       const bool here = threadIdx.x < many;
       const uint32_t mine = here ? few[threadIdx.x] : 0u;
@@ -483,7 +488,7 @@ __global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   Team team{red, of_rank, a.cluster, (int)blockIdx.x % a.cluster, 0};
   const SelectHead s(a, blockIdx.y, blockIdx.x / a.cluster);
-  if (a.cluster > 1) sm100::cluster_sync_all();
+  if (a.cluster > 1) team.meet();
   const int per_warp = kb_cdiv_i32(kb_max_i32(s.n, 1), a.cluster * warps * 32) * 32;
   const int begin = kb_min_i32((team.rank * warps + warp) * per_warp, s.n), end = kb_min_i32(begin + per_warp, s.n);
   const uint32_t below = (1u << lane) - 1;
