@@ -444,7 +444,8 @@ struct MmaTile {
   static constexpr int kSmem = kWarps * kWarpBytes;
   // per SM: what shared memory and registers allow
   static constexpr int kBlocks = kRowBytes == 512 ? 1 : kRowBytes == 256 && kN == 1 ? 3 : 2;
-  static_assert(kStageBytes % 128 == 0, "matrix loads address a tile by exclusive or");
+  // Matrix loads address chunks of a row by exclusive or, within a row's bytes: rows start on multiples of them, from the ring's start on.
+  static_assert(kStageBytes % kRowBytes == 0 && kStageBytes % 128 == 0 && kRowBytes <= 512, "rows start on multiples of their bytes");
   // Where chunk c of row r lies: at c ^ swizzle(r), so that what a matrix load (eight rows of a chunk) or a quarter of a 16-byte
   // load takes (two keys by four chunks; in fp32 also four rows by two chunks) lies in different banks.
   static __device__ __forceinline__ int swizzle(int r) {
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
   constexpr int kR = Tile::kR, kStages = Tile::kStages, kChunks = Tile::kChunks, kRowBytes = Tile::kRowBytes, kHeads = Tile::kHeads;
   constexpr int kSteps = kD / 16, kU = kR / 16, kDt = kD / 16;
   constexpr float kOffset = kF8 || kType == KB_F16 ? 7.f : 0.f, kSlack = 8.f;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(512) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane & 3, oct = lane >> 2;
   const int32_t unit = blockIdx.x * kWarps + warp;
   if (lane == 0 && unit < a.units && !a.by_item) a.join[unit].x = -1;
@@ -877,7 +878,8 @@ constexpr int kMostJoinThreads = 1024;
 
 // A block per item and head.  Groups of D / 4 threads take every so many-th part, four elements per thread; the groups are added up in order.
 __global__ void __launch_bounds__(kMostJoinThreads) paged_join_kernel(const AttendArgs a) {
-  __shared__ float red[kMostJoinThreads / 32], sums[kMostJoinThreads / 4][2], o_s[kMostJoinThreads * 4];
+  __shared__ float red[kMostJoinThreads / 32], sums[kMostJoinThreads / 4][2];
+  __shared__ __align__(16) float o_s[kMostJoinThreads * 4];
   const int threads = blockDim.x;
   let_next_launch_start();
   wait_for_launch_before();

@@ -42,7 +42,7 @@ struct WriteArgs {
 };
 
 template <typename T, int N>
-struct Several { T v[N]; };
+struct alignas(N * sizeof(T) % 16 == 0 ? 16 : alignof(T)) Several { T v[N]; };
 
 template <typename T, int N, bool kAligned>
 __device__ __forceinline__ void load_several(Several<T, N>& e, const T* x, int64_t sd) {

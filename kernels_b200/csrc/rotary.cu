@@ -33,7 +33,7 @@ struct RotaryArgs {
   KbFastDiv fd_T, fd_R;
 };
 
-template <typename T, int E> struct Elems { T v[E]; };
+template <typename T, int E> struct alignas(E * sizeof(T)) Elems { T v[E]; };
 
 template <typename T, int E>
 __device__ __forceinline__ void load_elems(const T* p, int64_t sd, Elems<T, E>& e) {
