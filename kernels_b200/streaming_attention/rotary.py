@@ -100,7 +100,8 @@ def _keep(ctx, inputs):
 
 def _turn(*inputs):
     """:func:`_rotate` with gradients."""
-    return (_RotaryEmbeddingTransformed if _lib.transforms_active() else _RotaryEmbedding).apply(*inputs)
+    special = _lib.transforms_active() or _lib.looked_into(*inputs[:2])
+    return (_RotaryEmbeddingTransformed if special else _RotaryEmbedding).apply(*inputs)
 
 
 _turn_uncompiled = torch.compiler.disable(_turn)
@@ -110,7 +111,7 @@ class _RotaryEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *inputs):
         _keep(ctx, inputs)
-        return _rotate_or_op(*inputs)
+        return _rotate(*inputs)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -125,7 +126,7 @@ class _RotaryEmbedding(torch.autograd.Function):
 
 
 class _RotaryEmbeddingTransformed(_RotaryEmbedding):
-    """The form that functorch's transforms ask for (a call of it takes 20 microseconds more)."""
+    """The form that functorch's transforms ask for (a call of it takes 20 microseconds more), and that calls the operator where something looks into it."""
 
     @staticmethod
     def forward(q, k, positions, inv_freq, ends, inverse):
@@ -181,5 +182,5 @@ def rotary_embedding(
     if looked_into:
         return _op(q, k, positions, inv_freq, ends, False)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _turn(q, k, positions, inv_freq, ends, False)
+        return (_RotaryEmbeddingTransformed if _lib.transforms_active() else _RotaryEmbedding).apply(q, k, positions, inv_freq, ends, False)
     return _rotate(q, k, positions, inv_freq, ends, False)
