@@ -427,7 +427,8 @@ KB_API int kb_rotary(const kb_rotary_params* p, void* stream);
  * New tokens into the cache.  `lens` counts them already: token t < new_lens[b] (NULL: T) of sequence b goes to row
  * lens[b] - new_lens[b] + t; rows outside [0, M * page) and rows without a page are dropped.  The pages have the tokens' type,
  * or e4m3 with scale = max(|x| of the row) / 448 (at least 1e-12).  A written row's entry of `weights` (or NULL) becomes 0 and its
- * entry of `row_positions` (or NULL) the token's position (positions NULL: the row).
+ * entry of `row_positions` (or NULL) the token's position (positions NULL: the row, which is not the token's position once rows have been
+ * evicted).
  */
 typedef struct kb_paged_write_params {
   kb_paged_cache cache;
@@ -448,14 +449,15 @@ KB_API int kb_paged_write(const kb_paged_write_params* p, void* stream);
 
 /*
  * Attention of one token per sequence, the one in row lens[b] - 1, over the sequence's rows; with context_size > 0 over those
- * rows r with (lens[b] - 1) / context_size - r / context_size <= back_contexts.  A sequence without rows gives 0 and lse 0.
+ * rows r with (lens[b] - 1) / context_size - r / context_size <= back_contexts (rows, whatever tokens an eviction has left in them).  A sequence without rows gives 0 and lse 0.
  * `lse` is base 2.  With `weights`, every seen row's softmax weight, summed over the query heads of its key/value head, is
  * added to weights[b][head][row]; `lse` must then be given.  `workspace`: kb_paged_attention_workspace_bytes bytes of the same, otherwise
  * filled-in block (host-only; it looks at sizes, strides, alignment and at whether `weights` is NULL; 0 for a block that would be refused),
  * 16-byte aligned.
  * The tensor-core kernel takes head dims 64 and 128 where q's heads are dense and keys and values have one layout with rows on
  * 16-byte boundaries (an e4m3 cache: and a 16-bit q); everything else goes to a CUDA-core kernel.  fp32 is multiplied in three tf32 products,
- * as exact as fp32 for numbers, but an infinity in a row counts as a NaN there.
+ * as exact as fp32 for numbers, but an infinity in a row, or a number within 2^-12 of the largest, counts as a NaN there.  An infinite value
+ * scale makes its heads' outputs NaN; their log-sum-exp and weights do not depend on it.
  */
 typedef struct kb_paged_attention_params {
   kb_paged_cache cache;

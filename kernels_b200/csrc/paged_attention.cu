@@ -689,9 +689,10 @@ __global__ void __launch_bounds__(kThreads, MmaTile<kType, kD, kN>::kBlocks) pag
           if constexpr (kF8) {
             ks = lds_f32(at + 2 * kR * kRowBytes + key * 4);
             vs[u][r] = lds_f32(at + 2 * kR * kRowBytes + kR * 4 + key * 4);
-            // (2^-80: no lower, or the sum of the weights leaves fp32.  A weight is 2^(offset + slack + 80) = 2^95 at most, and there are 2^30
-            // rows at most.  A scale that is not finite makes the products with V NaN, whatever its weight: it has no part in the maximum, so that
-            // the sum of the weights stays what it is.)
+            // (2^-80: no lower, or the sum of the weights leaves fp32: a weight is 2^(offset + slack + 80) = 2^95 at most, and there are 2^30
+            // rows at most.  What is multiplied with V then loses bits where all scales are below that.  With a scale of 2^L the largest weight is
+            // 2^(offset - L) at least, and those below 2^(L - 133) of it are 0 in fp32: too little to show up to L = 88.  A scale that is not
+            // finite makes the products with V NaN, whatever its weight: it has no part in the maximum, so that the sum of the weights stays what it is.)
             const float size = fabsf(vs[u][r]);
             lift = size < INFINITY ? __log2f(fmaxf(size, 8.3e-25f)) : 0.f;
           }

@@ -11,8 +11,8 @@
 // The kept rows below the budget stay where they are, and the i-th kept row behind it moves to the i-th place that came
 // free before it.  Attention does not depend on the rows' order, so nothing else has to move: a cache that is one row
 // over its budget moves one row, not half of them.  Sources lie behind the budget and destinations before it, so all
-// moves are independent.  Two kernels: one block per (sequence, head) picks the rows, then the moves are spread over
-// the GPU.
+// moves are independent.  Two kernels: a block per (sequence, head), or a cluster of blocks where the table is long, picks the rows, then the
+// moves are spread over the GPU.
 #include "common.cuh"
 #include "paged.cuh"
 #include "sm100_ptx.cuh"
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(1024) paged_select_long_kernel(const EvictArgs
 }
 
 // A warp takes 32 moves at a time: a lane looks up one of them and moves its entries of the bookkeeping, then the lanes copy the rows together.
-// HBM-bound: 163 000 rows of 512 bytes (keys and values) in 60 us, 5.6 TB/s read and written.
+// HBM-bound: some 314 000 rows of 512 bytes (keys and values) in 60 us, 5.4 TB/s read and written.
 template <bool kAligned>
 __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const EvictArgs a) {
   constexpr int kUnit = kAligned ? 16 : 1, kAtOnce = 4;

@@ -113,7 +113,8 @@ def paged_cache_write(
     ``k``, ``v``: ``[B, H_kv, T, D]``, any strides, of the pages' type, or fp32, fp16 or bf16 for e4m3 pages: every row is
     then scaled so that its largest magnitude maps to 448.  ``lens`` counts the new tokens already: token ``t < new_lens[b]``
     (int32 ``[B]``, None for ``T``) goes to row ``lens[b] - new_lens[b] + t``.  The entries of ``weights`` that belong to written rows become
-    0, those of ``row_positions`` the tokens' ``positions`` (int32 ``[B, T]``, None for the rows themselves).  Rows outside the table
+    0, those of ``row_positions`` the tokens' ``positions`` (int32 ``[B, T]``, None for the rows themselves; once rows have been evicted these are no
+    longer the tokens' positions, and new tokens need their own to be the newest).  Rows outside the table
     are dropped; two tokens of one call must not share a row of a page.
     """
     cache, index, rows = _pages("paged_cache_write", k_pages, v_pages, page_table, lens, k_scale, v_scale, True)
@@ -157,13 +158,16 @@ def paged_attention(
     """Attention of the newest token of every sequence, the one in row ``lens[b] - 1``, over the sequence's cached rows.
 
     ``q``: ``[B, H, D]``, ``H`` a multiple of ``H_kv``, of the pages' type (fp32, fp16 or bf16 for e4m3 pages).  With ``context_size`` the
-    operator's mask applies (``kernel.py:1540-1542``): the token sees its own chunk and ``back_contexts`` chunks before it, counted in rows.
+    operator's mask applies (``kernel.py:1540-1542``): the token sees its own chunk and ``back_contexts`` chunks before it, counted in rows
+    (not in tokens: an eviction leaves rows in another order, and a window after one is a window of rows).
     Returns ``o`` ``[B, H, D]`` and, on request, the base-2 log-sum-exp ``[B, H]``; both are 0 for a sequence that sees
     no row.  With ``weights``, the softmax weight of every row that is seen, summed over the query heads of its key/value
     head, is added to ``weights`` in place; that takes 4 bytes of workspace per query head and row that a token can see (of the window, or of the table).
 
     Sums are held in fp32.  16-bit and e4m3 caches: weights are rounded to 16 bits before they are multiplied with ``v``.  fp32 caches of head dim 64
-    and 128 are multiplied on the tensor cores in three parts, as exactly as in fp32; an infinity in a row counts as a NaN there.
+    and 128 are multiplied on the tensor cores in three parts, as exactly as in fp32; an infinity in a row counts as a NaN there, and so does a number
+    within 2^-12 of fp32's largest.  The row of an infinite value, whose scale in e4m3 pages is infinite, makes its heads NaN, and leaves the
+    log-sum-exp and weights alone.  (Value scales from 2^-80 to 2^88 lose nothing; smaller ones alone cost the outputs accuracy, larger ones the other two.)
     """
     cache, index, rows = _pages("paged_attention", k_pages, v_pages, page_table, lens, k_scale, v_scale)
     shape, dtype, pages_shape = q.shape, q.dtype, k_pages.shape
