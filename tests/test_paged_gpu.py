@@ -140,6 +140,15 @@ def test_attention_with_the_operators_mask(dtype, q_dtype, H, D, context_size, b
     check_attend(c, q, context_size, back, weights=torch.zeros(len(lens), 2, c["page_table"].shape[1] * 16))
 
 
+@pytest.mark.parametrize("dtype,q_dtype,D", [(F32, F32, 256), (BF16, BF16, 32), (F8, F32, 64), (F16, F16, 16)])
+@pytest.mark.parametrize("context_size,back", [(10, 3), (64, 1), (1, 0)])
+def test_windows_and_weights_of_the_cuda_core_kernel(dtype, q_dtype, D, context_size, back):
+    lens = [1, 64, 65, 0, 640, 500]
+    c = make_cache(len(lens), 2, D, 16, lens, dtype, stale=float("nan"), M=60)
+    q = torch.randn(len(lens), 6, D, generator=torch.Generator().manual_seed(8)).to(q_dtype)
+    check_attend(c, q, context_size, back, weights=torch.rand(len(lens), 2, 60 * 16))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F8])
 def test_attention_splits_long_rows(dtype):
     """One sequence over many blocks, beside short ones that leave most blocks without rows."""
@@ -708,6 +717,23 @@ def test_evict_passes_over_rows_without_a_page(page, n, budget, recent, gone):
             assert torch.equal(rows, g["row_positions"].cpu()[0, h, seen][:, None].expand(-1, 16).float())
         left = set(g["row_positions"][0, h, seen.cuda()].tolist())
         assert len(left) == len(seen) and left <= set(pos[0, h, :n][held].tolist())
+
+
+def test_evict_from_strided_tables_and_from_no_pages_at_all():
+    c = make_cache(2, 2, 64, 16, [100, 90], F16)
+    w, pos = make_books(2, 2, c["page_table"].shape[1] * 16)
+    from kernels_b200.streaming_attention import paged_cache_evict
+
+    for gone in ([], [1, 5]):
+        c["page_table"][0, gone] = -1
+        want, g = check_evict(c, w, pos, 50, 5), cuda(c | dict(weights=w, row_positions=pos))
+        wide = torch.full((2, 3 * c["page_table"].shape[1]), 10**6, dtype=torch.int32, device="cuda")[:, ::3]
+        wide.copy_(g["page_table"])
+        paged_cache_evict(g["k_pages"], g["v_pages"], wide, g["lens"], g["weights"], g["row_positions"], 50, 5)
+        assert all(torch.equal(want[n], g[n]) for n in g)
+    none = dict(c, k_pages=c["k_pages"][:0], v_pages=c["v_pages"][:0])
+    g = check_evict(none, w, pos, 50, 5)
+    assert g["lens"].tolist() == [50, 50] and torch.equal(g["weights"].cpu(), w) and torch.equal(g["row_positions"].cpu(), pos)
 
 
 def test_evict_layouts():

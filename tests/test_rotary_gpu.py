@@ -276,6 +276,21 @@ def test_rotary_gradients_of_transforms_are_recorded_too():
     assert torch.equal(tangent(q, t), turned) and torch.equal(torch.compile(tangent)(q, t), turned)
 
 
+@pytest.mark.parametrize("keys", [True, False])
+def test_rotary_operator_is_what_it_says(keys):
+    """Schema, fake form, gradient and compiled form agree with the operator; a compiled caller takes other lengths."""
+    from kernels_b200.streaming_attention import rotary_embedding
+
+    q, k, positions, inv_freq = _second_inputs((8, 24), 4)
+    q.requires_grad_(), k.requires_grad_()
+    torch.library.opcheck(torch.ops.kernels_b200.rotary_embedding.default, (q, k if keys else None, positions, inv_freq, [8, 32], False))
+    compiled = torch.compile(lambda q, k, p: rotary_embedding(q, k if keys else None, p, inv_freq, (8, 24)), fullgraph=True, dynamic=True)
+    for T in (17, 5, 1):
+        args = (q[:, :, :T], k[:, :, :T], positions[:, :, :T])
+        got, want = compiled(*args), rotary_embedding(args[0], args[1] if keys else None, args[2], inv_freq, (8, 24))
+        assert torch.equal(got[0], want[0]) and (torch.equal(got[1], want[1]) if keys else got[1] is None)
+
+
 def test_rotary_of_lazily_negated_tensors():
     """The imaginary part of a conjugate carries its sign as a mark on the tensor: inputs, frequencies, gradients and tangents alike."""
     from kernels_b200.streaming_attention import rotary_embedding
