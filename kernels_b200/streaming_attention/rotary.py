@@ -66,7 +66,7 @@ def _op(q, k, *rest):
 
 
 def _op_setup(ctx, inputs, output):
-    _, k, positions, inv_freq, ctx.ends, ctx.inverse = inputs
+    _, _, positions, inv_freq, ctx.ends, ctx.inverse = inputs
     ctx.save_for_backward(positions, inv_freq)
 
 
